@@ -31,7 +31,9 @@ typedef struct CUstream_st* tb200_stream_t; /* same type as cudaStream_t */
 
 typedef enum tb200_dtype {
   TB200_I8 = 0, TB200_U8 = 1, TB200_I16 = 2, TB200_U16 = 3, TB200_I32 = 4, TB200_U32 = 5,
-  TB200_I64 = 6, TB200_U64 = 7, TB200_F32 = 8, TB200_F64 = 9, TB200_BOOL = 10
+  TB200_I64 = 6, TB200_U64 = 7, TB200_F32 = 8, TB200_F64 = 9, TB200_BOOL = 10,
+  /* activations, gates and logits of the model operators below; no other algorithm takes them */
+  TB200_F16 = 11, TB200_BF16 = 12
 } tb200_dtype;
 
 typedef enum tb200_error {
@@ -248,6 +250,61 @@ int tb200_reduce(void* d_temp, size_t* temp_bytes, const void* d_in, uint64_t n,
 int tb200_histogram_sorted(const void* d_sorted, uint64_t n, int dtype, const void* d_bin_values,
                            uint32_t num_bins, uint32_t* d_counts, tb200_stream_t stream);
 
+/* ---- gated linear recurrence ------------------------------------------------------------
+ * The inclusive scan whose operator composes affine maps, by sequence and channel:
+ *   y[t] = a[t] * y[t-1] + x[t],   a = gate, or exp(gate) with log_gate != 0,
+ * y[-1] = d_initial (zero where NULL: the first row is then x itself). Sums and states are held
+ * in 32 bits, y is rounded once. No counterpart in the reference, whose closest form is
+ * thrust::inclusive_scan_by_key with a functor over pairs (thrust/scan.h).
+ *
+ * Rows: `sequences` x `rows` (every sequence `rows` long), or, with offset_bytes 4 or 8, `rows`
+ * rows of packed sequences in which sequence s owns rows d_offsets[s] .. d_offsets[s+1]-1
+ * (sequences + 1 ascending DEVICE integers of offset_bytes, from 0 to at most `rows`; empty
+ * sequences allowed). Rows behind the last sequence are left as they were, or written as zeros
+ * where fill_outside != 0. A tb200_rows names an array by its first element and its strides in
+ * elements; the channels of a row are adjacent; sequence_stride is ignored for packed rows.
+ * heads gates a row: heads == channels is a gate for each channel, otherwise heads divides
+ * channels and channels / heads neighbouring channels share a gate. dtype (x, y and their
+ * gradients): F32, F16 or BF16; gate_dtype: dtype or F32. d_initial, d_final and their
+ * gradients: sequences x channels float32. The final state of an empty sequence is its initial
+ * one. Gates beyond one in magnitude are allowed as long as their products over some hundred
+ * neighbouring rows stay in the range of float32. y may be x itself; no other overlap.
+ * Rows of one sequence are combined in an order that only the shape fixes: results are
+ * reproducible from run to run. Offsets that descend, do not begin at 0 or end beyond `rows` set
+ * the status to TB200_ERR_INVALID_ARGUMENT (outputs are then unspecified, memory is safe). */
+typedef struct tb200_recurrence_shape {
+  uint64_t sequences, rows, channels, heads;
+  int dtype, gate_dtype, log_gate, offset_bytes, fill_outside;
+} tb200_recurrence_shape;
+typedef struct tb200_rows {
+  void* data;
+  uint64_t row_stride, sequence_stride;
+} tb200_rows;
+int tb200_linear_recurrence(void* d_temp, size_t* temp_bytes, const tb200_recurrence_shape* shape,
+                            const void* d_offsets, const tb200_rows* gate, const tb200_rows* x, const tb200_rows* y,
+                            const float* d_initial, float* d_final, tb200_stream_t stream);
+
+/* Gradients of the recurrence, from its gates and its OUTPUT y (x is not needed): with dy the
+ * gradient of y and d_dfinal that of d_final (NULL: zero), G[t] = dy[t] + a[t+1] * G[t+1] gives
+ * dx[t] = G[t], dgate[t] = G[t] * y[t-1] (times a[t] with log_gate; summed over the channels that
+ * share the gate) and dinitial = a[0] * G[0] (d_dinitial may be NULL; an empty sequence hands
+ * d_dfinal through). y[-1] is d_initial as in the forward call. dx may be dy itself. */
+int tb200_linear_recurrence_backward(void* d_temp, size_t* temp_bytes, const tb200_recurrence_shape* shape,
+                                     const void* d_offsets, const tb200_rows* gate, const tb200_rows* y,
+                                     const tb200_rows* dy, const tb200_rows* dx, const tb200_rows* dgate,
+                                     const float* d_initial, const float* d_dfinal, float* d_dinitial,
+                                     tb200_stream_t stream);
+
+/* One row of each of `rows` sequences whose states lie in a pool of `slots` states of `channels`
+ * float32 (slot_stride elements apart), in place: row r works on state d_slots[r] (DEVICE integers
+ * of slot_bytes 4 or 8, at most 65536 rows then; slot_bytes 0: state r), y = state = a * state + x. A row whose slot lies
+ * outside [0, slots) belongs to no request: its y is zero. Rows that name the same slot are
+ * applied in their order. Gates and types as above; strides in elements; no scratch. */
+int tb200_linear_recurrence_step(float* d_state, uint64_t slots, uint64_t slot_stride, const void* d_slots,
+                                 int slot_bytes, const tb200_rows* gate, const tb200_rows* x, const tb200_rows* y,
+                                 uint64_t rows, uint64_t channels, uint64_t heads, int dtype, int gate_dtype,
+                                 int log_gate, tb200_stream_t stream);
+
 /* Status word of the last call that used d_temp: 0 or a tb200_error. Synchronises the
  * stream (one 4-byte copy). Mirrors the reference's end-of-call synchronize + error check
  * (thrust/system/cuda/detail/util.h:113-140, 251-299). */
@@ -278,7 +335,9 @@ int tb200_selftest_wait_timeout(uint32_t limit_polls, tb200_stream_t stream);
  * to kinds[i] (may be NULL) for i < capacity and returns the number of launches (negative:
  * -cudaError_t). kinds: 1 sort histogram, 2 radix pass, 3 sort copy-back, 4 scan,
  * 5 reduce_by_key, 6 histogram of sorted data, 7 partition histogram, 8 partition pass,
- * 9 reduce, 10 scan_by_key, 11 unique_by_key, 12 copy of flagged elements. */
+ * 9 reduce, 10 scan_by_key, 11 unique_by_key, 12 copy of flagged elements, 13 sort in one CTA,
+ * 14 plan of a large sort, 15 sort of its tiles, 16 linear recurrence, 17 its step, 18 tokens per
+ * expert, 19 balance loss. */
 int tb200_trace_begin(tb200_stream_t stream);
 int tb200_trace_end(float* ms, int* kinds, int capacity);
 

@@ -1,0 +1,74 @@
+"""Refusals of the recurrence's entry points: nothing here touches a GPU."""
+import ctypes as C
+
+import pytest
+import torch
+
+import thrust_b200 as tb
+from thrust_b200 import _capi as capi
+
+
+def shape(sequences=2, rows=10, channels=8, heads=8, dtype=capi.F32, gate_dtype=capi.F32, log=0, offset_bytes=0, fill=0):
+    return capi.RecurrenceShape(sequences, rows, channels, heads, dtype, gate_dtype, log, offset_bytes, fill)
+
+
+def size(s, back=False):
+    need = C.c_size_t(0)
+    call = capi.lib.tb200_linear_recurrence_backward if back else capi.lib.tb200_linear_recurrence
+    return call(None, C.byref(need), C.byref(s), *(None,) * (10 if back else 7)), need.value
+
+
+def test_size_queries_answer_without_a_gpu():
+    for back in (False, True):
+        rc, need = size(shape(), back)
+        assert rc == 0 and need >= 256
+        for bad in (dict(dtype=capi.F64), dict(dtype=capi.BF16, gate_dtype=capi.F16), dict(dtype=capi.I32)):
+            assert size(shape(**bad), back)[0] == capi.ERR_UNSUPPORTED
+        for bad in (dict(channels=0), dict(heads=0), dict(heads=3), dict(offset_bytes=2)):
+            assert size(shape(**bad), back)[0] == capi.ERR_INVALID_ARGUMENT
+        for bad in (dict(channels=1 << 25, heads=1), dict(sequences=1 << 40), dict(rows=1 << 50)):
+            assert size(shape(**bad), back)[0] == capi.ERR_UNSUPPORTED
+    assert capi.lib.tb200_linear_recurrence(None, None, C.byref(shape()), *(None,) * 7) == capi.ERR_INVALID_ARGUMENT
+
+
+def test_arguments_are_checked_before_any_device_work():
+    s, need = shape(), C.c_size_t(1 << 20)
+    fake = 0x7f0000000100  # never dereferenced
+    good, odd = capi.Rows(fake, 8, 80), capi.Rows(fake + 2, 8, 80)
+    call = capi.lib.tb200_linear_recurrence
+
+    def run(temp=fake, bytes_=need, shp=s, off=None, g=good, x=good, y=good):
+        return call(temp, C.byref(bytes_), C.byref(shp), off, C.byref(g), C.byref(x), C.byref(y), None, None, None)
+
+    assert run(temp=fake + 8) == capi.ERR_INVALID_ARGUMENT
+    assert run(bytes_=C.c_size_t(16)) == capi.ERR_TEMP_TOO_SMALL
+    assert run(x=odd) == capi.ERR_INVALID_ARGUMENT
+    assert run(y=capi.Rows(None, 8, 80)) == capi.ERR_INVALID_ARGUMENT
+    assert run(shp=shape(offset_bytes=4)) == capi.ERR_INVALID_ARGUMENT           # no offsets
+    assert run(shp=shape(offset_bytes=8), off=fake + 4) == capi.ERR_INVALID_ARGUMENT
+    step = capi.lib.tb200_linear_recurrence_step
+
+    def one(state=fake, slots=4, stride=8, idx=None, bytes_=0, rows=3, channels=8, heads=8, dt=capi.F32, gd=capi.F32, x=good):
+        return step(state, slots, stride, idx, bytes_, C.byref(good), C.byref(x), C.byref(good), rows, channels, heads, dt, gd,
+                    0, None)
+
+    assert one(rows=0) == 0
+    assert one(dt=capi.F64) == capi.ERR_UNSUPPORTED and one(dt=capi.F16, gd=capi.BF16) == capi.ERR_UNSUPPORTED
+    assert one(rows=5) == capi.ERR_INVALID_ARGUMENT and one(stride=7) == capi.ERR_INVALID_ARGUMENT
+    assert one(bytes_=4) == capi.ERR_INVALID_ARGUMENT and one(bytes_=3) == capi.ERR_INVALID_ARGUMENT
+    assert one(heads=5) == capi.ERR_INVALID_ARGUMENT and one(x=odd) == capi.ERR_INVALID_ARGUMENT
+    assert one(idx=fake, bytes_=4, rows=65537) == capi.ERR_UNSUPPORTED
+    assert one(state=fake + 2) == capi.ERR_INVALID_ARGUMENT
+
+
+def test_python_front_end_refuses_cpu_tensors():
+    z = torch.zeros(2, 3, 4)
+    with pytest.raises(ValueError, match="CUDA"):
+        tb.linear_recurrence(z, z)
+    with pytest.raises(ValueError, match="CUDA"):
+        tb.linear_recurrence_backward(z, z, z)
+    with pytest.raises(ValueError, match="CUDA"):
+        tb.linear_recurrence_step(z[0], z[0], z[0])
+    with pytest.raises(TypeError):  # no other algorithm takes the 16-bit floating types
+        tb.tb200_dtype(torch.zeros(2, dtype=torch.bfloat16))
+    assert capi.lib.tb200_scan(None, C.byref(C.c_size_t(0)), None, None, 4, capi.BF16, 0, None, None) == capi.ERR_UNSUPPORTED

@@ -16,14 +16,17 @@ _ALGORITHMS = (
     "inclusive_scan_by_key", "exclusive_scan_by_key",
     "reduce_by_key", "unique_by_key", "unique", "copy_flagged", "histogram_sorted", "dense_histogram", "tb200_dtype",
 )
-__all__ = ["Tb200Error", "_capi", "algorithms", "datagen", "sample_sort", *_ALGORITHMS]
+_MODEL_OPS = ("linear_recurrence", "linear_recurrence_backward", "linear_recurrence_step")
+__all__ = ["Tb200Error", "_capi", "algorithms", "datagen", "model_ops", "sample_sort", *_ALGORITHMS, *_MODEL_OPS]
 
 
 def __getattr__(name):
     if name in _ALGORITHMS:
         return getattr(importlib.import_module(".algorithms", __name__), name)
+    if name in _MODEL_OPS:
+        return getattr(importlib.import_module(".model_ops", __name__), name)
     if name == "Tb200Error":
         return importlib.import_module("._capi", __name__).Tb200Error
-    if name in ("_capi", "algorithms", "datagen", "sample_sort", "build"):
+    if name in ("_capi", "algorithms", "datagen", "model_ops", "sample_sort", "build"):
         return importlib.import_module("." + name, __name__)
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -10,11 +10,23 @@ from pathlib import Path
 _LIB_PATH = Path(__file__).resolve().parent / "libthrust_b200.so"
 
 # tb200_dtype
-I8, U8, I16, U16, I32, U32, I64, U64, F32, F64, BOOL = range(11)
+I8, U8, I16, U16, I32, U32, I64, U64, F32, F64, BOOL, F16, BF16 = range(13)  # the last two: model operators only
 DTYPE_BYTES = {I8: 1, U8: 1, I16: 2, U16: 2, I32: 4, U32: 4, I64: 8, U64: 8, F32: 4, F64: 8, BOOL: 1}
 
 OK = 0
 ERR_UNSUPPORTED, ERR_INVALID_ARGUMENT, ERR_TEMP_TOO_SMALL, ERR_WAIT_TIMEOUT, ERR_OVERFLOW = -1, -2, -3, -4, -5
+
+
+class Rows(C.Structure):
+    """tb200_rows: an array of rows by its first element and its strides in elements."""
+    _fields_ = [("data", C.c_void_p), ("row_stride", C.c_uint64), ("sequence_stride", C.c_uint64)]
+
+
+class RecurrenceShape(C.Structure):
+    """tb200_recurrence_shape"""
+    _fields_ = [("sequences", C.c_uint64), ("rows", C.c_uint64), ("channels", C.c_uint64), ("heads", C.c_uint64),
+                ("dtype", C.c_int), ("gate_dtype", C.c_int), ("log_gate", C.c_int), ("offset_bytes", C.c_int),
+                ("fill_outside", C.c_int)]
 
 
 class Tb200Error(RuntimeError):
@@ -30,7 +42,7 @@ def _load() -> C.CDLL:
             "(thrust_b200 has no CPU or PyTorch fallback)")
     lib = C.CDLL(str(_LIB_PATH))
     vp, sz, u64, i32, u32 = C.c_void_p, C.c_size_t, C.c_uint64, C.c_int, C.c_uint32
-    psz = C.POINTER(C.c_size_t)
+    psz, rows = C.POINTER(C.c_size_t), C.POINTER(Rows)
     sigs = {
         "tb200_version": ([], i32),
         "tb200_error_string": ([i32], C.c_char_p),
@@ -53,6 +65,10 @@ def _load() -> C.CDLL:
         "tb200_unique_by_key": ([vp, psz, vp, vp, vp, vp, vp, u64, i32, i32, vp], i32),
         "tb200_copy_flagged": ([vp, psz, vp, vp, vp, vp, u64, i32, i32, vp], i32),
         "tb200_histogram_sorted": ([vp, u64, i32, vp, u32, vp, vp], i32),
+        "tb200_linear_recurrence": ([vp, psz, C.POINTER(RecurrenceShape), vp, rows, rows, rows, vp, vp, vp], i32),
+        "tb200_linear_recurrence_backward": ([vp, psz, C.POINTER(RecurrenceShape), vp, rows, rows, rows, rows, rows,
+                                              vp, vp, vp, vp], i32),
+        "tb200_linear_recurrence_step": ([vp, u64, u64, vp, i32, rows, rows, rows, u64, u64, u64, i32, i32, i32, vp], i32),
         "tb200_temp_status": ([vp, vp], i32),
         "tb200_read_result": ([vp, vp, sz, vp, vp], i32),
         "tb200_read_result_in_front": ([vp, sz, vp, vp], i32),
@@ -81,7 +97,8 @@ EXPORTS = [
     "tb200_histogram_sorted", "tb200_temp_status", "tb200_read_result", "tb200_read_result_in_front", "tb200_selftest_wait_timeout", "tb200_trace_begin", "tb200_trace_end",
     "tb200_workspace_acquire",
     "tb200_workspace_release", "tb200_workspace_stats", "tb200_workspace_release_all", "tb200_radix_sort_host", "tb200_scan_host",
-    "tb200_reduce_by_key_host",
+    "tb200_reduce_by_key_host", "tb200_linear_recurrence", "tb200_linear_recurrence_backward",
+    "tb200_linear_recurrence_step",
 ]
 
 

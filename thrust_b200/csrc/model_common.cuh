@@ -1,0 +1,96 @@
+// What the kernels of the model operators share: 16-bit types, rows by strides, gates in registers.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace tb200 {
+
+struct RowsOf {  // an array of rows: strides in elements
+  char* data;
+  uint64_t row, seq;
+};
+
+template <typename T> __device__ __forceinline__ float to_f32(T v);
+template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Pack {
+  T v[V];
+};
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> load_pack(const char* base, uint64_t element) {  // read once
+  using P = Pack<T, V>;
+  P p;
+  const void* at = base + element * sizeof(T);
+  if constexpr (sizeof(P) == 16) {
+    const uint4 w = __ldcs(static_cast<const uint4*>(at));
+    p = *reinterpret_cast<const P*>(&w);
+  } else if constexpr (sizeof(P) == 8) {
+    const uint2 w = __ldcs(static_cast<const uint2*>(at));
+    p = *reinterpret_cast<const P*>(&w);
+  } else if constexpr (sizeof(P) == 4) {
+    const unsigned w = __ldcs(static_cast<const unsigned*>(at));
+    p = *reinterpret_cast<const P*>(&w);
+  } else {
+    const unsigned short w = __ldcs(static_cast<const unsigned short*>(at));
+    p = *reinterpret_cast<const P*>(&w);
+  }
+  return p;
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_floats(char* base, uint64_t element, const float (&f)[V]) {
+  Pack<T, V> p;
+#pragma unroll
+  for (int i = 0; i < V; ++i) p.v[i] = from_f32<T>(f[i]);
+  *reinterpret_cast<Pack<T, V>*>(base + element * sizeof(T)) = p;
+}
+
+// exp(g) - 1 for g in [-0.3, 0]: its power series up to g^7 (the next term is 5e-9 of the value).
+__device__ __forceinline__ float exp_minus_1(float g) {
+  float p = 1.0f / 5040;
+  p = fmaf(p, g, 1.0f / 720);
+  p = fmaf(p, g, 1.0f / 120);
+  p = fmaf(p, g, 1.0f / 24);
+  p = fmaf(p, g, 1.0f / 6);
+  p = fmaf(p, g, 0.5f);
+  p = fmaf(p, g, 1.0f);
+  return p * g;
+}
+constexpr float kNear = -0.3f;  // log gates from here to 0 are held as a - 1
+
+// A gate in registers. Plain: a itself. Log: a - 1 with the sign bit set where the gate is near one, else a.
+__device__ __forceinline__ float hold_gate(float g, bool log_gate) {
+  if (!log_gate) return g;
+  const bool near = g >= kNear && g <= 0.0f;
+  const float m = __uint_as_float(__float_as_uint(exp_minus_1(g)) | 0x80000000u);
+  return near ? m : __expf(g);
+}
+__device__ __forceinline__ bool held_near(float c, bool log_gate) { return log_gate && (__float_as_uint(c) >> 31); }
+// a * h + x
+__device__ __forceinline__ float advance(float c, bool near, float h, float x) {
+  const float u = fmaf(c, h, x);
+  return near ? h + u : u;
+}
+
+inline bool good_rows(const tb200_rows* r, int bytes) {
+  return r != nullptr && r->data != nullptr && reinterpret_cast<uintptr_t>(r->data) % bytes == 0;
+}
+inline RowsOf rows_of(const tb200_rows* r, bool packed) {
+  return RowsOf{static_cast<char*>(r->data), r->row_stride, packed ? 0 : r->sequence_stride};
+}
+// every row begins on a boundary of `bytes`
+inline bool rows_on(const RowsOf& r, int elem, int bytes) {
+  return (reinterpret_cast<uintptr_t>(r.data) | (r.row * elem) | (r.seq * elem)) % bytes == 0;
+}
+inline int model_bytes(int dtype) { return dtype == TB200_F32 ? 4 : dtype == TB200_F16 || dtype == TB200_BF16 ? 2 : 0; }
+
+}  // namespace tb200

@@ -1,0 +1,543 @@
+// Gated linear recurrence y[t] = a[t] * y[t-1] + x[t] by sequence and channel, forward and backward.
+//
+// A stretch of rows maps the state in front of it to the state behind it: h -> A * h + B, with A the product of its
+// gates and B what the stretch makes of a zero state. The backward pass is the same in the other direction: with
+// P = a[t] * G[t] as the state (G[t] = dy[t] + P[t+1]), a stretch maps the P behind it to the P of its first row,
+// with the same A. So one kernel serves both: logical rows run with the recurrence, forward in memory or backward.
+//
+// The unit of work is a tile of kWarps * R rows by a block of channels. Every warp keeps R rows in registers, a lane V
+// neighbouring channels of them: one pass over the rows gives the stretch's (A, B), the warps' stretches are joined
+// through shared memory, and a second pass over the same registers gives the outputs. Every input is read once and
+// every output written once: the kernel is bound by HBM.
+//
+// Gates close to one. A state remembers 1 / (1 - a) rows, so an error of a counts relative to 1 - a: a rounding of
+// 2^-25 in a = 0.9995 is 6e-5 of it, and a library exponential whose last bit leans to one side adds up over the whole
+// memory. With log gates in [-0.3, 0] the state therefore advances by its change, h + ((a - 1) * h + x), with a - 1
+// from its own series, and A is the exponential of the SUM of the gates, in the same two forms; with plain gates
+// A - 1 is carried beside A. States, products and sums are held in 32 bits; outputs are rounded once.
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "model_common.cuh"
+
+namespace tb200 {
+namespace {
+
+constexpr int kWarps = 8;
+constexpr int kThreads = kWarps * kWarp;
+
+struct RecArgs {
+  const void* offsets;
+  int offset_bytes;
+  int log_gate, fill;
+  uint64_t sequences;   // of them
+  uint64_t length;      // rows of a sequence; packed: of all
+  uint64_t chain_rows;  // rows of a chain: of one sequence, or of all sequences behind one another
+  int chain_is_sequence;
+  uint32_t channels, heads, head_size;
+  uint32_t block_heads, parts;  // heads in a block of channels; blocks that share one head
+  RowsOf gate, in, out;         // forward: x -> y; backward: dy -> dx
+  RowsOf y, dgate;              // backward only
+  const float* first;           // forward: initial states; backward: gradient of the final states
+  const float* initial;         // backward: initial states (y[-1])
+  float* last;                  // forward: final states; backward: gradient of the initial states
+  float* partial;               // backward, a head over several blocks: their sums, [rows][heads][parts]
+  TempHeader* hdr;
+};
+
+// A of a stretch in one word: A - 1 with the lowest bit set where A >= 1/2, else A with it clear. The bit costs at
+// most one unit of the last place, of A - 1 where that is what matters.
+__device__ __forceinline__ unsigned word_of(float a, float m) {
+  return a >= 0.5f ? (__float_as_uint(m) | 1u) : (__float_as_uint(a) & ~1u);
+}
+__device__ __forceinline__ float apply(unsigned word, float h, float b) {  // A * h + b
+  const float u = fmaf(__uint_as_float(word), h, b);
+  return (word & 1u) ? h + u : u;
+}
+
+struct Marks {           // of the rows of a tile; packed sequences fill it in shared memory
+  int seq[kWarps * 16];  // sequence of a first or last row
+  unsigned char kind[kWarps * 16];  // bit 0: first row of its sequence, bit 1: last
+};
+
+__device__ __forceinline__ uint64_t offset_at(const RecArgs& p, uint64_t i) {
+  const int64_t v = p.offset_bytes == 4 ? (int64_t)static_cast<const int32_t*>(p.offsets)[i]
+                                        : static_cast<const int64_t*>(p.offsets)[i];
+  return v < 0 ? 0 : (uint64_t)v > p.length ? p.length : (uint64_t)v;
+}
+
+// Marks the first and last rows of sequences among rows [r0, r1), in memory order; hands the states of empty sequences
+// that lie here through for channels [c0, c0 + count).
+__device__ void mark_rows(const RecArgs& p, uint64_t r0, uint64_t r1, bool at_end, uint32_t c0, uint32_t count, Marks& m) {
+  for (int i = threadIdx.x; i < (int)(sizeof(m.kind) / sizeof(m.kind[0])); i += kThreads) m.kind[i] = 0;
+  __syncthreads();
+  uint64_t lo = 0, hi = p.sequences + 1;  // first boundary at or behind r0
+  while (lo < hi) {
+    const uint64_t mid = (lo + hi) / 2;
+    if (offset_at(p, mid) < r0) lo = mid + 1; else hi = mid;
+  }
+  for (uint64_t j = lo + threadIdx.x; j <= p.sequences; j += kThreads) {
+    const uint64_t v = offset_at(p, j);
+    if (v > r1) break;
+    if (j > 0 && v > r0 && offset_at(p, j - 1) < v) {  // sequence j - 1 ends in front of boundary j
+      m.seq[v - 1 - r0] = (int)(j - 1);
+      atomicOr(reinterpret_cast<unsigned*>(m.kind) + (v - 1 - r0) / 4, 2u << (8 * ((v - 1 - r0) % 4)));
+    }
+    if (j < p.sequences && (v < r1 || at_end)) {
+      const uint64_t end = offset_at(p, j + 1);
+      if (end > v && v < r1 && v >= r0) {
+        m.seq[v - r0] = (int)j;
+        atomicOr(reinterpret_cast<unsigned*>(m.kind) + (v - r0) / 4, 1u << (8 * ((v - r0) % 4)));
+      } else if (end <= v && p.last != nullptr) {
+        for (uint32_t c = c0; c < c0 + count; ++c) p.last[j * p.channels + c] = p.first ? p.first[j * p.channels + c] : 0.0f;
+      }
+    }
+  }
+}
+
+template <typename T, typename G, int V, bool SHARED, bool BACK, int R>
+__global__ void __launch_bounds__(kThreads) recurrence_kernel(RecArgs p) {
+  constexpr int WIDTH = kWarp * V;
+  constexpr int GV = SHARED ? 1 : V;  // gates of a lane in a row
+  constexpr int TILE = kWarps * R;
+  static_assert(TILE <= kWarps * 16 && R <= kWarp, "marks and row information are sized for this");
+  __shared__ Marks s_marks;
+  __shared__ unsigned s_word[kWarps][WIDTH];
+  __shared__ float s_b[kWarps][WIDTH];
+  __shared__ float s_carry[kWarps][WIDTH];
+  __shared__ int s_reset[kWarps];
+  __shared__ float s_state[WIDTH];
+
+  const unsigned lane = lane_id(), warp = threadIdx.x / kWarp;
+  const bool logg = p.log_gate != 0;
+  const uint64_t chain = blockIdx.y;
+
+  // the block's channels
+  uint32_t c0, count;
+  if (!SHARED) {
+    c0 = blockIdx.x * WIDTH;
+    count = min((uint32_t)WIDTH, p.channels - c0);
+  } else if (p.parts == 1) {
+    const uint32_t h0 = blockIdx.x * p.block_heads;
+    c0 = h0 * p.head_size;
+    count = min(p.block_heads, p.heads - h0) * p.head_size;
+  } else {
+    const uint32_t h0 = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
+    c0 = h0 * p.head_size + part * WIDTH;
+    count = min((uint32_t)WIDTH, p.head_size - part * WIDTH);
+  }
+  const uint32_t ch = c0 + lane * V;
+  const bool live = lane * V < count;
+  const uint32_t head = SHARED ? ch / p.head_size : 0;
+  const uint32_t gate_at = SHARED ? head : ch;
+
+  if (p.offsets != nullptr && blockIdx.x == 0) {  // bad offsets are reported, and cannot lead outside the arrays
+    bool bad = false;
+    for (uint64_t i = threadIdx.x; i <= p.sequences; i += kThreads) {
+      const int64_t v = p.offset_bytes == 4 ? (int64_t)static_cast<const int32_t*>(p.offsets)[i]
+                                            : static_cast<const int64_t*>(p.offsets)[i];
+      bad = bad || v < 0 || (uint64_t)v > p.length || (i == 0 ? v != 0 : (uint64_t)v < offset_at(p, i - 1));
+    }
+    if (bad) atomicExch(&p.hdr->status, (int)TB200_ERR_INVALID_ARGUMENT);
+  }
+
+  if (threadIdx.x < WIDTH) s_state[threadIdx.x] = 0.0f;
+  const uint64_t tiles = (p.chain_rows + TILE - 1) / TILE;
+  const uint64_t used_from = p.offsets ? offset_at(p, 0) : 0;
+  const uint64_t used_to = p.offsets ? offset_at(p, p.sequences) : p.chain_rows;
+
+  for (uint64_t tile = 0; tile < tiles; ++tile) {
+    // ---- what the warp's rows are: lane l holds logical row l --------------------------------------
+    const uint64_t q = tile * TILE + warp * R + lane;
+    const bool valid = lane < R && q < p.chain_rows;
+    const uint64_t row = valid ? (BACK ? p.chain_rows - 1 - q : q) : 0;  // in the chain
+    uint64_t b = 0, t = row;
+    if (p.chain_is_sequence) {
+      b = chain;
+    } else if (p.offsets == nullptr) {
+      b = row / p.length;
+      t = row - b * p.length;
+    }
+    const unsigned m_valid = __ballot_sync(0xffffffffu, valid);
+
+    // ---- load ---------------------------------------------------------------------------------------
+    float c[R][GV];
+    Pack<T, V> x[R];
+    Pack<T, V> yprev[BACK ? R : 1];
+    float sum_g[GV] = {};
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const uint64_t rb = __shfl_sync(0xffffffffu, b, r), rt = __shfl_sync(0xffffffffu, t, r);
+      const bool on = live && (m_valid >> r & 1);
+      Pack<G, GV> g;
+      if (on) {
+        g = load_pack<G, GV>(p.gate.data, rb * p.gate.seq + rt * p.gate.row + gate_at);
+        x[r] = load_pack<T, V>(p.in.data, rb * p.in.seq + rt * p.in.row + ch);
+        if constexpr (BACK)
+          if (rt > 0) yprev[r] = load_pack<T, V>(p.y.data, rb * p.y.seq + (rt - 1) * p.y.row + ch);
+      }
+#pragma unroll
+      for (int i = 0; i < GV; ++i) c[r][i] = on ? to_f32<G>(g.v[i]) : 0.0f;
+    }
+
+    // ---- first and last rows of sequences -------------------------------------------------------------
+    bool first, last, inside = valid;
+    int seq = (int)b;
+    if (p.offsets != nullptr) {
+      const uint64_t lo = tile * TILE, hi = min(lo + TILE, p.chain_rows);
+      const uint64_t r0 = BACK ? p.chain_rows - hi : lo, r1 = BACK ? p.chain_rows - lo : hi;
+      mark_rows(p, r0, r1, r1 == p.chain_rows, c0, count, s_marks);
+      __syncthreads();
+      const unsigned kind = valid ? s_marks.kind[row - r0] : 0;
+      first = kind & 1;
+      last = kind & 2;
+      if (kind) seq = s_marks.seq[row - r0];
+      inside = valid && row >= used_from && row < used_to;
+    } else {
+      first = valid && t == 0;
+      last = valid && t == p.length - 1;
+    }
+    const unsigned m_inside = __ballot_sync(0xffffffffu, inside);
+    const unsigned m_first = __ballot_sync(0xffffffffu, first), m_last = __ballot_sync(0xffffffffu, last);
+    const unsigned m_begin = BACK ? m_last : m_first, m_end = BACK ? m_first : m_last;  // with the recurrence
+
+    // the state that a sequence begins with
+    auto first_state = [&](int r, float (&h)[V]) {
+      const int s = __shfl_sync(0xffffffffu, seq, r);
+      const float* at = p.first + (uint64_t)s * p.channels + ch;
+#pragma unroll
+      for (int i = 0; i < V; ++i) h[i] = live ? at[i] : 0.0f;
+    };
+
+    // ---- first pass: the stretch's A and B --------------------------------------------------------------
+    float A[GV], M[GV], B[V];
+#pragma unroll
+    for (int i = 0; i < GV; ++i) A[i] = 1.0f, M[i] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) B[i] = 0.0f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (!(m_inside >> r & 1)) continue;
+      const bool begin = m_begin >> r & 1;
+      float h[V];
+      if (begin && p.first) first_state(r, h);
+#pragma unroll
+      for (int i = 0; i < GV; ++i) {
+        const float g = c[r][i];
+        if (logg) {
+          sum_g[i] += g;
+        } else {
+          A[i] *= g;
+          M[i] = fmaf(M[i], g, g - 1.0f);
+        }
+        c[r][i] = hold_gate(g, logg);
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float cc = c[r][SHARED ? 0 : i];
+        const bool near = held_near(cc, logg);
+        const float xv = to_f32<T>(x[r].v[i]);
+        if (begin) B[i] = p.first ? h[i] : 0.0f;
+        if constexpr (BACK) {
+          B[i] = advance(cc, near, xv + B[i], 0.0f);
+        } else {
+          B[i] = begin && !p.first ? xv : advance(cc, near, B[i], xv);
+        }
+      }
+    }
+    if (logg) {
+#pragma unroll
+      for (int i = 0; i < GV; ++i) {
+        const float cc = hold_gate(sum_g[i], true);
+        const bool near = held_near(cc, true);
+        A[i] = near ? 1.0f + cc : cc;
+        M[i] = near ? cc : cc - 1.0f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      s_word[warp][lane * V + i] = word_of(A[SHARED ? 0 : i], M[SHARED ? 0 : i]);
+      s_b[warp][lane * V + i] = B[i];
+    }
+    if (lane == 0) s_reset[warp] = (m_begin & m_inside) != 0;
+    __syncthreads();
+
+    // ---- the states in front of the warps' stretches -------------------------------------------------------
+    if (threadIdx.x < WIDTH) {
+      float h = s_state[threadIdx.x];
+      for (int w = 0; w < kWarps; ++w) {
+        s_carry[w][threadIdx.x] = h;
+        h = s_reset[w] ? s_b[w][threadIdx.x] : apply(s_word[w][threadIdx.x], h, s_b[w][threadIdx.x]);
+      }
+      s_state[threadIdx.x] = h;
+    }
+    __syncthreads();
+
+    // ---- second pass: outputs ----------------------------------------------------------------------------
+    float h[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) h[i] = s_carry[warp][lane * V + i];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (!(m_valid >> r & 1)) continue;
+      const uint64_t rb = __shfl_sync(0xffffffffu, b, r), rt = __shfl_sync(0xffffffffu, t, r);
+      const bool in = m_inside >> r & 1;
+      if (!in && !p.fill) continue;
+      const bool begin = m_begin >> r & 1;
+      const int s = __shfl_sync(0xffffffffu, seq, r);
+      if (begin) {
+        if (p.first) {
+          first_state(r, h);
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; ++i) h[i] = 0.0f;
+        }
+      }
+      float out[V], dg[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float cc = c[r][SHARED ? 0 : i];
+        const bool near = held_near(cc, logg);
+        const float xv = to_f32<T>(x[r].v[i]);
+        if constexpr (BACK) {
+          const float g = xv + h[i];
+          h[i] = advance(cc, near, g, 0.0f);
+          out[i] = g;
+          float prev = 0.0f;
+          if (m_first >> r & 1) {
+            if (p.initial && live) prev = p.initial[(uint64_t)s * p.channels + ch + i];
+          } else if (rt > 0) {
+            prev = to_f32<T>(yprev[r].v[i]);
+          }
+          dg[i] = (logg ? h[i] : g) * prev;
+        } else {
+          h[i] = begin && !p.first ? xv : advance(cc, near, h[i], xv);
+          out[i] = h[i];
+        }
+      }
+      if (!in) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) out[i] = dg[i] = 0.0f;
+      }
+      if (live) store_floats<T, V>(p.out.data, rb * p.out.seq + rt * p.out.row + ch, out);
+      if constexpr (BACK) {
+        if constexpr (!SHARED) {
+          if (live) store_floats<G, V>(p.dgate.data, rb * p.dgate.seq + rt * p.dgate.row + ch, dg);
+        } else {
+          // the head's lanes are neighbours; the first of them gathers the sum
+          float sum = 0.0f;
+#pragma unroll
+          for (int i = 0; i < V; ++i) sum += dg[i];
+          if (!live) sum = 0.0f;
+          const uint32_t per = p.parts == 1 ? p.head_size / V : kWarp;
+          const uint32_t at = lane % per;
+          for (uint32_t off = 1; off < per; off *= 2) {
+            const float other = __shfl_down_sync(0xffffffffu, sum, off);
+            if (at + off < per) sum += other;
+          }
+          if (live && at == 0) {
+            if (p.parts == 1) {
+              const float one[1] = {sum};
+              store_floats<G, 1>(p.dgate.data, rb * p.dgate.seq + rt * p.dgate.row + head, one);
+            } else {
+              const uint64_t flat = rb * (p.chain_is_sequence || !p.offsets ? p.length : 0) + rt;
+              p.partial[(flat * p.heads + head) * p.parts + blockIdx.x % p.parts] = sum;
+            }
+          }
+        }
+      }
+      if (in && (m_end >> r & 1) && p.last && live) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) p.last[(uint64_t)s * p.channels + ch + i] = h[i];
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// dgate of heads that span several blocks of channels: the blocks' sums, in their order.
+template <typename G>
+__global__ void __launch_bounds__(kThreads) join_gate_kernel(RecArgs p, uint64_t rows) {
+  const uint64_t n = rows * p.heads;
+  const uint64_t used = p.offsets && !p.fill ? offset_at(p, p.sequences) : rows;
+  for (uint64_t i = blockIdx.x * (uint64_t)kThreads + threadIdx.x; i < n; i += (uint64_t)gridDim.x * kThreads) {
+    const uint64_t row = i / p.heads, head = i - row * p.heads;
+    if (row >= used) continue;
+    float sum[1] = {0.0f};
+    for (uint32_t k = 0; k < p.parts; ++k) sum[0] += p.partial[i * p.parts + k];
+    const uint64_t b = p.offsets ? 0 : row / p.length, t = row - b * p.length;
+    store_floats<G, 1>(p.dgate.data, b * p.dgate.seq + t * p.dgate.row + head, sum);
+  }
+}
+
+struct Call {
+  tb200_recurrence_shape shape;
+  RecArgs args;
+  uint64_t rows;  // of all sequences
+  uint32_t blocks;
+};
+
+template <typename T, typename G, int V, bool SHARED, bool BACK>
+int launch_kernel(Call& k, cudaStream_t stream) {
+  RecArgs& p = k.args;
+  constexpr uint32_t WIDTH = kWarp * V;
+  if (!SHARED) {
+    k.blocks = (p.channels + WIDTH - 1) / WIDTH;
+    p.parts = 1;
+  } else if (p.head_size <= WIDTH) {
+    p.block_heads = WIDTH / p.head_size;
+    p.parts = 1;
+    k.blocks = (p.heads + p.block_heads - 1) / p.block_heads;
+  } else {
+    p.parts = (p.head_size + WIDTH - 1) / WIDTH;
+    k.blocks = p.heads * p.parts;
+  }
+  const uint64_t chains = p.chain_is_sequence ? p.sequences : 1;
+  if (chains > 65535) return TB200_ERR_UNSUPPORTED;
+  recurrence_kernel<T, G, V, SHARED, BACK, 8><<<dim3(k.blocks, (unsigned)chains), kThreads, 0, stream>>>(p);
+  trace_mark(stream, kTraceRecurrence);
+  TB200_CUDA_TRY(cudaGetLastError());
+  if (BACK && SHARED && p.parts > 1) {
+    const uint64_t n = k.rows * p.heads;
+    const uint64_t grid = (n + kThreads - 1) / kThreads;
+    join_gate_kernel<G><<<(unsigned)(grid < 4096 ? grid : 4096), kThreads, 0, stream>>>(p, k.rows);
+    trace_mark(stream, kTraceRecurrence);
+    TB200_CUDA_TRY(cudaGetLastError());
+  }
+  return TB200_OK;
+}
+
+template <typename T, typename G, bool BACK>
+int launch_typed(Call& k, cudaStream_t stream) {
+  RecArgs& p = k.args;
+  const bool shared = p.heads != p.channels;
+  constexpr int ST = 4 * sizeof(T), SG = 4 * sizeof(G);
+  // four channels a lane where every row of every array begins on that many elements and a head's channels divide so
+  bool wide = p.channels % 4 == 0 && rows_on(p.in, sizeof(T), ST) && rows_on(p.out, sizeof(T), ST);
+  if (BACK) wide = wide && rows_on(p.y, sizeof(T), ST);
+  if (shared) {
+    wide = wide && p.head_size % 4 == 0;
+  } else {
+    wide = wide && rows_on(p.gate, sizeof(G), SG);
+    if (BACK) wide = wide && rows_on(p.dgate, sizeof(G), SG);
+  }
+  if (shared)
+    return wide ? launch_kernel<T, G, 4, true, BACK>(k, stream) : launch_kernel<T, G, 1, true, BACK>(k, stream);
+  return wide ? launch_kernel<T, G, 4, false, BACK>(k, stream) : launch_kernel<T, G, 1, false, BACK>(k, stream);
+}
+
+template <bool BACK>
+int launch(Call& k, cudaStream_t stream) {
+  const int t = k.shape.dtype, g = k.shape.gate_dtype;
+  if (t == TB200_F32) return launch_typed<float, float, BACK>(k, stream);
+  if (t == TB200_BF16)
+    return g == TB200_F32 ? launch_typed<__nv_bfloat16, float, BACK>(k, stream)
+                          : launch_typed<__nv_bfloat16, __nv_bfloat16, BACK>(k, stream);
+  return g == TB200_F32 ? launch_typed<__half, float, BACK>(k, stream) : launch_typed<__half, __half, BACK>(k, stream);
+}
+
+// The checks that both directions share. *go is set where there are rows to work on.
+int prepare(void* d_temp, size_t* temp_bytes, const tb200_recurrence_shape* shape, bool back, Call& k) {
+  if (temp_bytes == nullptr || shape == nullptr) return TB200_ERR_INVALID_ARGUMENT;
+  const tb200_recurrence_shape& s = *shape;
+  if (model_bytes(s.dtype) == 0 || (s.gate_dtype != s.dtype && s.gate_dtype != TB200_F32)) return TB200_ERR_UNSUPPORTED;
+  if (s.offset_bytes != 0 && s.offset_bytes != 4 && s.offset_bytes != 8) return TB200_ERR_INVALID_ARGUMENT;
+  if (s.channels == 0 || s.heads == 0 || s.channels % s.heads) return TB200_ERR_INVALID_ARGUMENT;
+  if (s.channels > (1u << 24) || s.sequences > 0x7fffffffull || s.rows > (1ull << 40)) return TB200_ERR_UNSUPPORTED;
+  k.shape = s;
+  k.rows = s.offset_bytes ? s.rows : s.sequences * s.rows;
+  const uint64_t head_size = s.channels / s.heads;
+  size_t need = kHeaderBytes;
+  // a head over several blocks of channels leaves a sum for each of them; the narrowest blocks have 32 channels
+  if (back && s.heads != s.channels && head_size > kWarp)
+    need += align_up(k.rows * s.heads * ((head_size + kWarp - 1) / kWarp) * sizeof(float), 256);
+  if (d_temp == nullptr) {
+    *temp_bytes = need;
+    return TB200_OK;
+  }
+  if (*temp_bytes < need) return TB200_ERR_TEMP_TOO_SMALL;
+  if (reinterpret_cast<uintptr_t>(d_temp) % 256) return TB200_ERR_INVALID_ARGUMENT;
+  RecArgs& p = k.args;
+  p = RecArgs{};
+  p.offset_bytes = s.offset_bytes;
+  p.log_gate = s.log_gate;
+  p.fill = s.fill_outside;
+  p.sequences = s.sequences;
+  p.length = s.rows;
+  p.chain_is_sequence = s.offset_bytes == 0;
+  p.chain_rows = s.rows;
+  p.channels = (uint32_t)s.channels;
+  p.heads = (uint32_t)s.heads;
+  p.head_size = (uint32_t)head_size;
+  p.hdr = static_cast<TempHeader*>(d_temp);
+  p.partial = reinterpret_cast<float*>(static_cast<char*>(d_temp) + kHeaderBytes);
+  return TB200_OK;
+}
+
+// States of sequences that have no rows at all.
+int hand_through(const Call& k, const float* from, float* to, cudaStream_t stream) {
+  const size_t bytes = k.shape.sequences * k.shape.channels * sizeof(float);
+  if (to == nullptr || bytes == 0) return TB200_OK;
+  if (from == nullptr) return (int)cudaMemsetAsync(to, 0, bytes, stream);
+  return from == to ? TB200_OK : (int)cudaMemcpyAsync(to, from, bytes, cudaMemcpyDeviceToDevice, stream);
+}
+
+}  // namespace
+}  // namespace tb200
+
+extern "C" int tb200_linear_recurrence(void* d_temp, size_t* temp_bytes, const tb200_recurrence_shape* shape,
+                                       const void* d_offsets, const tb200_rows* gate, const tb200_rows* x,
+                                       const tb200_rows* y, const float* d_initial, float* d_final,
+                                       tb200_stream_t stream) {
+  using namespace tb200;
+  Call k{};
+  const int rc = prepare(d_temp, temp_bytes, shape, false, k);
+  if (rc || d_temp == nullptr) return rc;
+  const bool packed = k.shape.offset_bytes != 0;
+  if (packed && (!d_offsets || reinterpret_cast<uintptr_t>(d_offsets) % k.shape.offset_bytes)) return TB200_ERR_INVALID_ARGUMENT;
+  const bool some = k.rows != 0 && k.shape.sequences + (packed && k.shape.fill_outside) != 0;
+  const int tb = model_bytes(k.shape.dtype);
+  if (some && !(good_rows(gate, model_bytes(k.shape.gate_dtype)) && good_rows(x, tb) && good_rows(y, tb)))
+    return TB200_ERR_INVALID_ARGUMENT;
+  TB200_CUDA_TRY(cudaMemsetAsync(d_temp, 0, kHeaderBytes, stream));
+  if (!some) return hand_through(k, d_initial, d_final, stream);
+  RecArgs& p = k.args;
+  p.offsets = packed ? d_offsets : nullptr;
+  p.gate = rows_of(gate, packed);
+  p.in = rows_of(x, packed);
+  p.out = rows_of(y, packed);
+  p.first = d_initial;
+  p.last = d_final;
+  return launch<false>(k, stream);
+}
+
+extern "C" int tb200_linear_recurrence_backward(void* d_temp, size_t* temp_bytes, const tb200_recurrence_shape* shape,
+                                                const void* d_offsets, const tb200_rows* gate, const tb200_rows* y,
+                                                const tb200_rows* dy, const tb200_rows* dx, const tb200_rows* dgate,
+                                                const float* d_initial, const float* d_dfinal, float* d_dinitial,
+                                                tb200_stream_t stream) {
+  using namespace tb200;
+  Call k{};
+  const int rc = prepare(d_temp, temp_bytes, shape, true, k);
+  if (rc || d_temp == nullptr) return rc;
+  const bool packed = k.shape.offset_bytes != 0;
+  if (packed && (!d_offsets || reinterpret_cast<uintptr_t>(d_offsets) % k.shape.offset_bytes)) return TB200_ERR_INVALID_ARGUMENT;
+  const bool some = k.rows != 0 && k.shape.sequences + (packed && k.shape.fill_outside) != 0;
+  const int tb = model_bytes(k.shape.dtype), gb = model_bytes(k.shape.gate_dtype);
+  if (some && !(good_rows(gate, gb) && good_rows(y, tb) && good_rows(dy, tb) && good_rows(dx, tb) && good_rows(dgate, gb)))
+    return TB200_ERR_INVALID_ARGUMENT;
+  TB200_CUDA_TRY(cudaMemsetAsync(d_temp, 0, kHeaderBytes, stream));
+  if (!some) return hand_through(k, d_dfinal, d_dinitial, stream);
+  RecArgs& p = k.args;
+  p.offsets = packed ? d_offsets : nullptr;
+  p.gate = rows_of(gate, packed);
+  p.in = rows_of(dy, packed);
+  p.out = rows_of(dx, packed);
+  p.y = rows_of(y, packed);
+  p.dgate = rows_of(dgate, packed);
+  p.initial = d_initial;
+  p.first = d_dfinal;
+  p.last = d_dinitial;
+  return launch<true>(k, stream);
+}
