@@ -305,6 +305,39 @@ int tb200_linear_recurrence_step(float* d_state, uint64_t slots, uint64_t slot_s
                                  uint64_t rows, uint64_t channels, uint64_t heads, int dtype, int gate_dtype,
                                  int log_gate, tb200_stream_t stream);
 
+/* ---- tokens per expert and balance loss ---------------------------------------------------
+ * Histogram of the experts that tokens were routed to: `rows` tokens with k ids each (DEVICE
+ * integers of id_bytes 4 or 8; the ids of a token are adjacent, tokens id_stride ids apart),
+ * d_counts[e] = number of ids equal to e in tokens whose d_mask byte is not 0 (d_mask NULL: all),
+ * d_begins (may be NULL; experts + 1 of them) its exclusive prefix sums: where each expert's
+ * tokens begin once the ids are sorted (tb200_radix_sort). Ids outside [0, experts) are not
+ * counted. experts <= 8192. The sort-based counterpart is tb200_histogram_sorted. */
+int tb200_expert_counts(void* d_temp, size_t* temp_bytes, const void* d_ids, uint64_t rows, uint32_t k,
+                        uint64_t id_stride, int id_bytes, const uint8_t* d_mask, uint32_t experts,
+                        uint64_t* d_counts, uint64_t* d_begins, tb200_stream_t stream);
+
+/* Balance loss of router logits (rows x experts of F32, F16 or BF16, experts <= 1024, by strides;
+ * sequence_stride ignored) and the ids chosen, for each of `sequences` sequences of packed rows
+ * (d_offsets as for the recurrence; offset_bytes 0: one sequence of all rows). With p the softmax
+ * of a token's logits (zero where all of them are -inf), n the sequence's tokens with a mask that
+ * is not 0 and c[e] its counts over these, as above:
+ *   loss = experts / (k n^2) * sum_e c[e] * sum_t p[t][e]   (0 where n is 0; 1 when balanced)
+ * Writes per sequence d_loss, d_counts (experts of them) and d_weights[e] = experts c[e] / (k n^2),
+ * the derivative of the loss by any p[t][e], which is all that the backward call needs. Masked
+ * tokens are not looked at. Sums are exact in 64-bit fixed point over the CTAs' 32-bit sums:
+ * results are reproducible from run to run. Bad offsets set the status as for the recurrence. */
+int tb200_balance_loss(void* d_temp, size_t* temp_bytes, const tb200_rows* logits, int dtype, const void* d_ids,
+                       uint32_t k, uint64_t id_stride, int id_bytes, const uint8_t* d_mask, const void* d_offsets,
+                       int offset_bytes, uint64_t sequences, uint64_t rows, uint32_t experts, float* d_loss,
+                       uint64_t* d_counts, float* d_weights, tb200_stream_t stream);
+
+/* dlogits[t][e] = dloss * p[t][e] * (w[e] - sum_j p[t][j] w[j]), with the weights and dloss of t's
+ * sequence; zero for masked tokens and tokens of no sequence. dlogits may be logits itself. No
+ * scratch. */
+int tb200_balance_loss_backward(const tb200_rows* logits, int dtype, const float* d_weights, const float* d_dloss,
+                                const uint8_t* d_mask, const void* d_offsets, int offset_bytes, uint64_t sequences,
+                                uint64_t rows, uint32_t experts, const tb200_rows* dlogits, tb200_stream_t stream);
+
 /* Status word of the last call that used d_temp: 0 or a tb200_error. Synchronises the
  * stream (one 4-byte copy). Mirrors the reference's end-of-call synchronize + error check
  * (thrust/system/cuda/detail/util.h:113-140, 251-299). */

@@ -16,7 +16,8 @@ _ALGORITHMS = (
     "inclusive_scan_by_key", "exclusive_scan_by_key",
     "reduce_by_key", "unique_by_key", "unique", "copy_flagged", "histogram_sorted", "dense_histogram", "tb200_dtype",
 )
-_MODEL_OPS = ("linear_recurrence", "linear_recurrence_backward", "linear_recurrence_step")
+_MODEL_OPS = ("linear_recurrence", "linear_recurrence_backward", "linear_recurrence_step", "expert_counts",
+              "balance_loss", "balance_loss_backward")
 __all__ = ["Tb200Error", "_capi", "algorithms", "datagen", "model_ops", "sample_sort", *_ALGORITHMS, *_MODEL_OPS]
 
 

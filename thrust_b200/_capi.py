@@ -69,6 +69,9 @@ def _load() -> C.CDLL:
         "tb200_linear_recurrence_backward": ([vp, psz, C.POINTER(RecurrenceShape), vp, rows, rows, rows, rows, rows,
                                               vp, vp, vp, vp], i32),
         "tb200_linear_recurrence_step": ([vp, u64, u64, vp, i32, rows, rows, rows, u64, u64, u64, i32, i32, i32, vp], i32),
+        "tb200_expert_counts": ([vp, psz, vp, u64, u32, u64, i32, vp, u32, vp, vp, vp], i32),
+        "tb200_balance_loss": ([vp, psz, rows, i32, vp, u32, u64, i32, vp, vp, i32, u64, u64, u32, vp, vp, vp, vp], i32),
+        "tb200_balance_loss_backward": ([rows, i32, vp, vp, vp, vp, i32, u64, u64, u32, rows, vp], i32),
         "tb200_temp_status": ([vp, vp], i32),
         "tb200_read_result": ([vp, vp, sz, vp, vp], i32),
         "tb200_read_result_in_front": ([vp, sz, vp, vp], i32),
@@ -98,7 +101,7 @@ EXPORTS = [
     "tb200_workspace_acquire",
     "tb200_workspace_release", "tb200_workspace_stats", "tb200_workspace_release_all", "tb200_radix_sort_host", "tb200_scan_host",
     "tb200_reduce_by_key_host", "tb200_linear_recurrence", "tb200_linear_recurrence_backward",
-    "tb200_linear_recurrence_step",
+    "tb200_linear_recurrence_step", "tb200_expert_counts", "tb200_balance_loss", "tb200_balance_loss_backward",
 ]
 
 

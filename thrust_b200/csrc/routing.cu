@@ -1,0 +1,569 @@
+// Statistics of routing tokens to experts: how many tokens each expert gets, the balance loss, its gradient.
+//
+// The loss of a sequence is experts / (k n^2) * sum_e count[e] * sum_t p[t][e] with p = softmax(logits), so one pass
+// over the logits gives column sums of p, one over the ids a histogram, and both end in `experts` numbers. The backward
+// pass is local to a row: p * (w - p . w). All of it is bound by HBM (or by the launch, for a decoding batch).
+//
+// Layout. A row of logits is spread over 1 to 32 lanes, eight experts to a lane and step, so that a lane loads 16 bytes
+// of a 16-bit type at once, sums over a row are shuffles among its lanes, and the column sums stay in the lane's own
+// registers for all rows of a CTA. Registers are summed over warps in a fixed order, and the CTAs' sums are added as
+// 64-bit integers, whose order does not matter: reproducible, and finished by whichever CTA is last.
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "model_common.cuh"
+
+namespace tb200 {
+namespace {
+
+constexpr int kRouteThreads = 256;
+constexpr int kRouteWarps = kRouteThreads / kWarp;
+constexpr uint32_t kMaxCountExperts = 8192;  // counters of a CTA in 32 KB
+constexpr uint32_t kMaxBalanceExperts = 1024;
+
+struct Ids {
+  const void* ids;
+  uint64_t stride;
+  uint32_t k;
+  int bytes;
+};
+__device__ __forceinline__ int64_t id_at(const Ids& d, uint64_t row, uint32_t slot) {
+  const uint64_t i = row * d.stride + slot;
+  return d.bytes == 4 ? (int64_t)static_cast<const int32_t*>(d.ids)[i] : static_cast<const int64_t*>(d.ids)[i];
+}
+
+// The ids of rows [r0, r1) into a CTA's counters.
+__device__ __forceinline__ void count_rows(const Ids& d, const uint8_t* mask, uint64_t r0, uint64_t r1, uint32_t experts,
+                                           unsigned* counters) {
+  const uint64_t n = (r1 - r0) * d.k;
+  auto count = [&](auto i) {  // 32-bit indices where they suffice: a division of 64 bits costs more than the rest
+    const uint64_t row = r0 + i / (decltype(i))d.k;
+    if (mask && !mask[row]) return;
+    const int64_t id = id_at(d, row, (uint32_t)(i % (decltype(i))d.k));
+    if (id >= 0 && id < (int64_t)experts) atomicAdd(&counters[id], 1u);
+  };
+  if (n < (1ull << 31)) {
+    for (uint32_t i = threadIdx.x; i < (uint32_t)n; i += kRouteThreads) count(i);
+  } else {
+    for (uint64_t i = threadIdx.x; i < n; i += kRouteThreads) count(i);
+  }
+}
+
+// ---- tokens per expert ------------------------------------------------------------------------------
+
+__device__ __forceinline__ void write_counts(const unsigned long long* sums, const unsigned* counters, uint32_t experts,
+                                             uint64_t* counts, uint64_t* begins) {
+  // exclusive prefix sums by strips: thread t has the experts of strip t
+  __shared__ unsigned long long s_strip[kRouteThreads];
+  const uint32_t per = (experts + kRouteThreads - 1) / kRouteThreads;
+  const uint32_t e0 = min(threadIdx.x * per, experts), e1 = min(e0 + per, experts);
+  auto at = [&](uint32_t e) { return sums ? __ldcg(&sums[e]) : (unsigned long long)counters[e]; };
+  unsigned long long mine = 0;
+  for (uint32_t e = e0; e < e1; ++e) {
+    const unsigned long long v = at(e);
+    counts[e] = v;
+    mine += v;
+  }
+  if (begins == nullptr) return;
+  s_strip[threadIdx.x] = mine;
+  __syncthreads();
+  for (int off = 1; off < kRouteThreads; off *= 2) {
+    const unsigned long long v = threadIdx.x >= off ? s_strip[threadIdx.x - off] : 0;
+    __syncthreads();
+    s_strip[threadIdx.x] += v;
+    __syncthreads();
+  }
+  unsigned long long run = s_strip[threadIdx.x] - mine;
+  for (uint32_t e = e0; e < e1; ++e) {
+    begins[e] = run;
+    run += at(e);
+  }
+  if (threadIdx.x == kRouteThreads - 1) begins[experts] = s_strip[threadIdx.x];
+}
+
+__global__ void __launch_bounds__(kRouteThreads)
+expert_counts_kernel(Ids ids, const uint8_t* mask, uint64_t rows, uint64_t rows_of_cta, uint32_t experts,
+                     uint64_t* counts, uint64_t* begins, TempHeader* hdr, unsigned long long* sums) {
+  extern __shared__ unsigned s_count[];
+  __shared__ unsigned s_last;
+  for (uint32_t e = threadIdx.x; e < experts; e += kRouteThreads) s_count[e] = 0;
+  __syncthreads();
+  const uint64_t r0 = blockIdx.x * rows_of_cta, r1 = min(r0 + rows_of_cta, rows);
+  if (r0 < r1) count_rows(ids, mask, r0, r1, experts, s_count);
+  __syncthreads();
+  if (gridDim.x == 1) {  // the scratch is not cleared for a single CTA
+    if (threadIdx.x == 0) hdr->status = TB200_OK;
+    write_counts(nullptr, s_count, experts, counts, begins);
+    return;
+  }
+  for (uint32_t e = threadIdx.x; e < experts; e += kRouteThreads)
+    if (s_count[e]) atomicAdd(&sums[e], (unsigned long long)s_count[e]);
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) s_last = atomicAdd(&hdr->ticket, 1u) == gridDim.x - 1;
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  write_counts(sums, nullptr, experts, counts, begins);
+}
+
+// ---- rows of logits over lanes ------------------------------------------------------------------------
+
+// A row over `lanes` (a power of two) lanes: element i of step j is expert (j * lanes + lane) * 8 + i.
+template <typename T, int J>
+struct RowPack {
+  Pack<T, 8> p[J];
+};
+template <typename T>
+__device__ __forceinline__ Pack<T, 8> load8(const char* base, uint64_t element) {
+  Pack<T, 8> p;
+  const uint4* at = reinterpret_cast<const uint4*>(base + element * sizeof(T));
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(p) / 16); ++i) reinterpret_cast<uint4*>(&p)[i] = __ldcs(at + i);
+  return p;
+}
+template <typename T, int J, bool VEC>
+__device__ __forceinline__ void load_row(const RowsOf& z, uint64_t row, uint32_t lanes, uint32_t lane, uint32_t experts,
+                                         RowPack<T, J>& out) {
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    const uint32_t e = (j * lanes + lane) * 8;
+    if constexpr (VEC) {
+      if (e < experts) out.p[j] = load8<T>(z.data, row * z.row + e);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (e + i < experts) out.p[j].v[i] = *reinterpret_cast<const T*>(z.data + (row * z.row + e + i) * sizeof(T));
+    }
+  }
+}
+__device__ __forceinline__ float lanes_max(float v, uint32_t lanes) {
+  for (uint32_t off = 1; off < lanes; off *= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
+  return v;
+}
+__device__ __forceinline__ float lanes_sum(float v, uint32_t lanes) {
+  for (uint32_t off = 1; off < lanes; off *= 2) v += __shfl_xor_sync(0xffffffffu, v, off);
+  return v;
+}
+// Softmax of a row in 32 bits. -inf is a disabled expert; a row of nothing else has no probabilities (zeros).
+template <typename T, int J>
+__device__ __forceinline__ void softmax_row(const RowPack<T, J>& row, uint32_t lanes, uint32_t lane, uint32_t experts,
+                                            float (&p)[J * 8]) {
+  const float none = __int_as_float(0xff800000);
+  float top = none;
+#pragma unroll
+  for (int j = 0; j < J; ++j)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float z = (j * lanes + lane) * 8 + i < experts ? to_f32<T>(row.p[j].v[i]) : none;
+      p[j * 8 + i] = z;
+      top = fmaxf(top, z);
+    }
+  top = lanes_max(top, lanes);
+  float sum = 0.0f;
+  const float base = top == none ? 0.0f : top;
+#pragma unroll
+  for (int i = 0; i < J * 8; ++i) {
+    p[i] = __expf(p[i] - base);
+    sum += p[i];
+  }
+  sum = lanes_sum(sum, lanes);
+  const float scale = top == none && sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+  for (int i = 0; i < J * 8; ++i) p[i] *= scale;
+}
+
+struct Spans {  // packed sequences over the rows, or one sequence
+  const void* offsets;
+  int bytes;
+  uint64_t sequences, rows;
+};
+__device__ __forceinline__ int64_t raw_offset(const Spans& s, uint64_t i) {
+  return s.bytes == 4 ? (int64_t)static_cast<const int32_t*>(s.offsets)[i] : static_cast<const int64_t*>(s.offsets)[i];
+}
+__device__ __forceinline__ uint64_t begin_of(const Spans& s, uint64_t i) {  // of sequence i; i = sequences: the end
+  if (s.bytes == 0) return i == 0 ? 0 : s.rows;
+  const int64_t v = raw_offset(s, i);
+  return v < 0 ? 0 : (uint64_t)v > s.rows ? s.rows : (uint64_t)v;
+}
+__device__ __forceinline__ uint64_t sequence_of(const Spans& s, uint64_t row) {  // last one that begins at or before row
+  if (s.bytes == 0) return 0;
+  uint64_t lo = 0, hi = s.sequences;  // first boundary behind row, less one
+  while (lo < hi) {
+    const uint64_t mid = (lo + hi + 1) / 2;
+    if (begin_of(s, mid) <= row) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+// ---- balance loss -------------------------------------------------------------------------------------
+
+struct BalanceArgs {
+  RowsOf z;
+  Ids ids;
+  const uint8_t* mask;
+  Spans spans;
+  uint64_t rows_of_cta;
+  uint32_t experts, lanes;
+  float scale;  // fixed point: one is `scale`
+  float* loss;
+  uint64_t* counts;
+  float* weights;
+  TempHeader* hdr;
+  unsigned long long* sums;    // [sequences][experts] of probabilities
+  unsigned long long* totals;  // [sequences][experts] of ids
+  unsigned long long* tokens;  // [sequences]
+  unsigned* done;              // [sequences] pieces of a sequence that are in
+  unsigned* poison;            // [sequences] a probability was NaN
+};
+
+template <typename T, int J, bool VEC>
+__global__ void __launch_bounds__(kRouteThreads) balance_kernel(BalanceArgs a) {
+  __shared__ unsigned s_count[kMaxBalanceExperts];
+  __shared__ float s_sum[kRouteWarps][J * 256];
+  __shared__ unsigned s_tokens[kRouteWarps];
+  __shared__ float s_loss[kRouteWarps];
+  __shared__ unsigned s_last;
+  const unsigned lane = lane_id(), warp = threadIdx.x / kWarp;
+  const uint32_t lanes = a.lanes, groups = kWarp / lanes, in_row = lane % lanes, group = lane / lanes;
+  const uint64_t r0 = blockIdx.x * a.rows_of_cta, r1 = min(r0 + a.rows_of_cta, a.spans.rows);
+
+  if (blockIdx.x == 0 && a.spans.bytes) {  // empty sequences belong to no CTA's rows; bad offsets are reported
+    bool bad = threadIdx.x == 0 && raw_offset(a.spans, a.spans.sequences) != (int64_t)begin_of(a.spans, a.spans.sequences);
+    for (uint64_t s = threadIdx.x; s < a.spans.sequences; s += kRouteThreads) {
+      const uint64_t b = begin_of(a.spans, s), e = begin_of(a.spans, s + 1);
+      bad = bad || raw_offset(a.spans, s) != (int64_t)b || (s == 0 && b != 0) || e < b;
+      if (e > b) continue;
+      for (uint32_t i = 0; i < a.experts; ++i) {
+        a.counts[s * a.experts + i] = 0;
+        a.weights[s * a.experts + i] = 0.0f;
+      }
+      a.loss[s] = 0.0f;
+    }
+    if (bad) atomicExch(&a.hdr->status, (int)TB200_ERR_INVALID_ARGUMENT);
+  }
+  if (r0 >= r1) return;
+
+  for (uint64_t s = sequence_of(a.spans, r0); s < a.spans.sequences; ++s) {
+    const uint64_t begin = begin_of(a.spans, s), end = begin_of(a.spans, s + 1);
+    if (begin >= r1) break;
+    const uint64_t from = max(begin, r0), to = min(end, r1);
+    if (from >= to) continue;
+    for (uint32_t e = threadIdx.x; e < a.experts; e += kRouteThreads) s_count[e] = 0;
+    __syncthreads();
+    count_rows(a.ids, a.mask, from, to, a.experts, s_count);
+
+    float acc[J * 8] = {};
+    unsigned kept = 0;
+    for (uint64_t base = from + warp * groups; base < to; base += kRouteWarps * groups) {
+      const uint64_t row = base + group;
+      const bool on = row < to && (a.mask == nullptr || a.mask[row]);
+      RowPack<T, J> pack = {};
+      if (on) load_row<T, J, VEC>(a.z, row, lanes, in_row, a.experts, pack);
+      float p[J * 8];
+      softmax_row<T, J>(pack, lanes, in_row, a.experts, p);
+      if (on) {
+        kept += in_row == 0;
+#pragma unroll
+        for (int i = 0; i < J * 8; ++i) acc[i] += p[i];
+      }
+    }
+    // over the row groups of a warp, then over the warps, in a fixed order
+#pragma unroll
+    for (int i = 0; i < J * 8; ++i)
+      for (uint32_t off = lanes; off < kWarp; off *= 2) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], off);
+    for (int off = 16; off > 0; off /= 2) kept += __shfl_xor_sync(0xffffffffu, kept, off);
+    if (group == 0) {
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s_sum[warp][(j * lanes + in_row) * 8 + i] = acc[j * 8 + i];
+    }
+    if (lane == 0) s_tokens[warp] = kept;
+    __syncthreads();
+    for (uint32_t e = threadIdx.x; e < a.experts; e += kRouteThreads) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kRouteWarps; ++w) sum += s_sum[w][e];
+      if (!(sum == sum)) atomicOr(&a.poison[s], 1u);
+      else if (sum > 0.0f) atomicAdd(&a.sums[s * a.experts + e], __float2ull_rn(sum * a.scale));
+      if (s_count[e]) atomicAdd(&a.totals[s * a.experts + e], (unsigned long long)s_count[e]);
+    }
+    if (threadIdx.x == 0) {
+      unsigned n = 0;
+      for (int w = 0; w < kRouteWarps; ++w) n += s_tokens[w];
+      if (n) atomicAdd(&a.tokens[s], (unsigned long long)n);
+    }
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      const unsigned pieces = (unsigned)((end - 1) / a.rows_of_cta - begin / a.rows_of_cta + 1);
+      s_last = atomicAdd(&a.done[s], 1u) == pieces - 1;
+    }
+    __syncthreads();
+    if (s_last) {
+      __threadfence();
+      const double n = (double)__ldcg(&a.tokens[s]);
+      const double unit = n > 0 ? (double)a.experts / ((double)a.ids.k * n * n) : 0.0;
+      float part = 0.0f;
+      for (uint32_t e = threadIdx.x; e < a.experts; e += kRouteThreads) {
+        const unsigned long long c = __ldcg(&a.totals[s * a.experts + e]);
+        const float w = (float)(unit * (double)c);
+        a.counts[s * a.experts + e] = c;
+        a.weights[s * a.experts + e] = w;
+        part += w * (float)((double)__ldcg(&a.sums[s * a.experts + e]) / (double)a.scale);
+      }
+      part = lanes_sum(part, kWarp);
+      if (lane == 0) s_loss[warp] = part;
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        float loss = 0.0f;
+        for (int w = 0; w < kRouteWarps; ++w) loss += s_loss[w];
+        a.loss[s] = __ldcg(&a.poison[s]) ? __int_as_float(0x7fc00000) : loss;
+      }
+    }
+    __syncthreads();
+  }
+}
+
+struct BalanceBackArgs {
+  RowsOf z, dz;
+  const float* weights;
+  const float* dloss;
+  const uint8_t* mask;
+  Spans spans;
+  uint64_t rows_of_warp;
+  uint32_t experts, lanes;
+};
+
+template <typename T, int J, bool VEC>
+__global__ void __launch_bounds__(kRouteThreads) balance_backward_kernel(BalanceBackArgs a) {
+  const unsigned lane = lane_id();
+  const uint32_t lanes = a.lanes, groups = kWarp / lanes, in_row = lane % lanes, group = lane / lanes;
+  const uint64_t warp = blockIdx.x * (uint64_t)kRouteWarps + threadIdx.x / kWarp;
+  const uint64_t r0 = warp * a.rows_of_warp, r1 = min(r0 + a.rows_of_warp, a.spans.rows);
+  uint64_t s = ~0ull, end = 0;  // the sequence whose weights are held, and its end
+  float w[J * 8] = {};
+  float scale = 0.0f;
+  for (uint64_t base = r0; base < r1; base += groups) {
+    const uint64_t row = base + group;
+    const bool valid = row < r1;
+    if (valid && (s == ~0ull || row >= end)) {
+      if (s == ~0ull) s = sequence_of(a.spans, row);
+      while (s < a.spans.sequences && row >= begin_of(a.spans, s + 1)) ++s;
+      end = s < a.spans.sequences ? begin_of(a.spans, s + 1) : a.spans.rows;
+      const bool some = s < a.spans.sequences && row >= begin_of(a.spans, s);
+      scale = some ? a.dloss[s] : 0.0f;
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t e = (j * lanes + in_row) * 8 + i;
+          w[j * 8 + i] = some && e < a.experts ? a.weights[s * a.experts + e] : 0.0f;
+        }
+    }
+    const bool on = valid && s < a.spans.sequences && (a.mask == nullptr || a.mask[row]);
+    RowPack<T, J> pack = {};
+    if (on) load_row<T, J, VEC>(a.z, row, lanes, in_row, a.experts, pack);
+    float p[J * 8];
+    softmax_row<T, J>(pack, lanes, in_row, a.experts, p);
+    float dot = 0.0f;
+#pragma unroll
+    for (int i = 0; i < J * 8; ++i) dot = fmaf(p[i], w[i], dot);
+    dot = lanes_sum(dot, lanes);
+    if (!valid) continue;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const uint32_t e = (j * lanes + in_row) * 8;
+      Pack<T, 8> out;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) out.v[i] = from_f32<T>(on ? scale * p[j * 8 + i] * (w[j * 8 + i] - dot) : 0.0f);
+      if constexpr (VEC) {
+        if (e < a.experts) {
+          uint4* at = reinterpret_cast<uint4*>(a.dz.data + (row * a.dz.row + e) * sizeof(T));
+#pragma unroll
+          for (int i = 0; i < (int)(sizeof(out) / 16); ++i) at[i] = reinterpret_cast<const uint4*>(&out)[i];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (e + i < a.experts) *reinterpret_cast<T*>(a.dz.data + (row * a.dz.row + e + i) * sizeof(T)) = out.v[i];
+      }
+    }
+  }
+}
+
+uint32_t lanes_of(uint32_t experts) {  // lanes that share a row
+  uint32_t lanes = 1;
+  while (lanes < kWarp && lanes * 8 < experts) lanes *= 2;
+  return lanes;
+}
+// Calls f(type tag, J, VEC) for a row of this type and size.
+template <typename F>
+int by_row(int dtype, uint32_t experts, bool vec, F f) {
+  auto with = [&](auto tag) -> int {
+    using T = decltype(tag);
+    auto sized = [&](auto v) -> int {
+      if (experts <= 256) return f(tag, std::integral_constant<int, 1>{}, v);
+      if (experts <= 512) return f(tag, std::integral_constant<int, 2>{}, v);
+      return f(tag, std::integral_constant<int, 4>{}, v);
+    };
+    (void)sizeof(T);
+    return vec ? sized(std::true_type{}) : sized(std::false_type{});
+  };
+  if (dtype == TB200_F32) return with(float{});
+  if (dtype == TB200_F16) return with(__half{});
+  return with(__nv_bfloat16{});
+}
+
+int check_ids(const void* ids, uint64_t rows, uint32_t k, uint64_t stride, int bytes) {
+  if (bytes != 4 && bytes != 8) return TB200_ERR_INVALID_ARGUMENT;
+  if (k == 0 || (rows > 1 && stride < k) || rows > (1ull << 40) || k > (1u << 20)) return TB200_ERR_INVALID_ARGUMENT;
+  if (rows && (!ids || reinterpret_cast<uintptr_t>(ids) % bytes)) return TB200_ERR_INVALID_ARGUMENT;
+  return TB200_OK;
+}
+
+}  // namespace
+}  // namespace tb200
+
+extern "C" int tb200_expert_counts(void* d_temp, size_t* temp_bytes, const void* d_ids, uint64_t rows, uint32_t k,
+                                   uint64_t id_stride, int id_bytes, const uint8_t* d_mask, uint32_t experts,
+                                   uint64_t* d_counts, uint64_t* d_begins, tb200_stream_t stream) {
+  using namespace tb200;
+  if (temp_bytes == nullptr || experts == 0) return TB200_ERR_INVALID_ARGUMENT;
+  if (experts > kMaxCountExperts) return TB200_ERR_UNSUPPORTED;
+  const size_t need = kHeaderBytes + align_up(experts * sizeof(unsigned long long), 256);
+  if (d_temp == nullptr) {
+    *temp_bytes = need;
+    return TB200_OK;
+  }
+  if (*temp_bytes < need) return TB200_ERR_TEMP_TOO_SMALL;
+  if (reinterpret_cast<uintptr_t>(d_temp) % 256) return TB200_ERR_INVALID_ARGUMENT;
+  int rc = check_ids(d_ids, rows, k, id_stride, id_bytes);
+  if (rc) return rc;
+  if (!d_counts || (reinterpret_cast<uintptr_t>(d_counts) | reinterpret_cast<uintptr_t>(d_begins)) % 8) return TB200_ERR_INVALID_ARGUMENT;
+  int sms = 0;
+  rc = sm_count_of_device(&sms);
+  if (rc) return rc;
+  // a CTA for each 4096 ids, as many as two waves hold
+  uint64_t ctas = (rows * k + 4095) / 4096;
+  if (ctas > 2ull * sms) ctas = 2ull * sms;
+  if (ctas > rows) ctas = rows;
+  if (ctas == 0) ctas = 1;
+  const uint64_t per = rows ? (rows + ctas - 1) / ctas : 1;
+  ctas = rows ? (rows + per - 1) / per : 1;
+  if (ctas > 1) TB200_CUDA_TRY(cudaMemsetAsync(d_temp, 0, need, stream));
+  const Ids ids{d_ids, id_stride, k, id_bytes};
+  expert_counts_kernel<<<(unsigned)ctas, kRouteThreads, experts * sizeof(unsigned), stream>>>(
+      ids, d_mask, rows, per, experts, d_counts, d_begins, static_cast<TempHeader*>(d_temp),
+      reinterpret_cast<unsigned long long*>(static_cast<char*>(d_temp) + kHeaderBytes));
+  trace_mark(stream, kTraceExpertCounts);
+  return (int)cudaGetLastError();
+}
+
+extern "C" int tb200_balance_loss(void* d_temp, size_t* temp_bytes, const tb200_rows* logits, int dtype, const void* d_ids,
+                                  uint32_t k, uint64_t id_stride, int id_bytes, const uint8_t* d_mask,
+                                  const void* d_offsets, int offset_bytes, uint64_t sequences, uint64_t rows,
+                                  uint32_t experts, float* d_loss, uint64_t* d_counts, float* d_weights,
+                                  tb200_stream_t stream) {
+  using namespace tb200;
+  if (temp_bytes == nullptr || experts == 0) return TB200_ERR_INVALID_ARGUMENT;
+  if (model_bytes(dtype) == 0 || experts > kMaxBalanceExperts || sequences > 0x7fffffffull) return TB200_ERR_UNSUPPORTED;
+  if (offset_bytes != 0 && offset_bytes != 4 && offset_bytes != 8) return TB200_ERR_INVALID_ARGUMENT;
+  if (offset_bytes == 0 && sequences != 1) return TB200_ERR_INVALID_ARGUMENT;
+  const uint64_t cells = sequences * experts;
+  const size_t need = kHeaderBytes + align_up(cells * 16 + sequences * 16, 256);
+  if (d_temp == nullptr) {
+    *temp_bytes = need;
+    return TB200_OK;
+  }
+  if (*temp_bytes < need) return TB200_ERR_TEMP_TOO_SMALL;
+  if (reinterpret_cast<uintptr_t>(d_temp) % 256) return TB200_ERR_INVALID_ARGUMENT;
+  int rc = check_ids(d_ids, rows, k, id_stride, id_bytes);
+  if (rc) return rc;
+  const int tb = model_bytes(dtype);
+  if (rows && !good_rows(logits, tb)) return TB200_ERR_INVALID_ARGUMENT;
+  if (offset_bytes && (!d_offsets || reinterpret_cast<uintptr_t>(d_offsets) % offset_bytes)) return TB200_ERR_INVALID_ARGUMENT;
+  if (sequences && (!d_loss || !d_counts || !d_weights)) return TB200_ERR_INVALID_ARGUMENT;
+  if (reinterpret_cast<uintptr_t>(d_counts) % 8 ||
+      (reinterpret_cast<uintptr_t>(d_loss) | reinterpret_cast<uintptr_t>(d_weights)) % 4) return TB200_ERR_INVALID_ARGUMENT;
+  TB200_CUDA_TRY(cudaMemsetAsync(d_temp, 0, need, stream));
+  if (rows == 0 || sequences == 0) {
+    if (sequences == 0) return TB200_OK;
+    TB200_CUDA_TRY(cudaMemsetAsync(d_loss, 0, sequences * sizeof(float), stream));
+    TB200_CUDA_TRY(cudaMemsetAsync(d_counts, 0, cells * sizeof(uint64_t), stream));
+    return (int)cudaMemsetAsync(d_weights, 0, cells * sizeof(float), stream);
+  }
+  int sms = 0;
+  rc = sm_count_of_device(&sms);
+  if (rc) return rc;
+  BalanceArgs a{};
+  a.z = rows_of(logits, true);
+  a.ids = Ids{d_ids, id_stride, k, id_bytes};
+  a.mask = d_mask;
+  a.spans = Spans{d_offsets, offset_bytes, sequences, rows};
+  a.experts = experts;
+  a.lanes = lanes_of(experts);
+  int bits = 62;  // a sum of all rows stays below 2^62
+  while (bits > 1 && (rows >> (62 - bits)) != 0) --bits;
+  a.scale = ldexpf(1.0f, bits);
+  a.loss = d_loss;
+  a.counts = d_counts;
+  a.weights = d_weights;
+  a.hdr = static_cast<TempHeader*>(d_temp);
+  a.sums = reinterpret_cast<unsigned long long*>(static_cast<char*>(d_temp) + kHeaderBytes);
+  a.totals = a.sums + cells;
+  a.tokens = a.totals + cells;
+  a.done = reinterpret_cast<unsigned*>(a.tokens + sequences);
+  a.poison = a.done + sequences;
+  // rows of a CTA: enough to be worth its share of the sums, few enough for two waves of CTAs
+  const uint64_t least = 4ull * kRouteWarps * (kWarp / a.lanes);
+  uint64_t per = (rows + 2ull * sms - 1) / (2ull * sms);
+  if (per < least) per = least;
+  a.rows_of_cta = per;
+  const unsigned grid = (unsigned)((rows + per - 1) / per);
+  const bool vec = experts % 8 == 0 && rows_on(a.z, tb, 16);
+  return by_row(dtype, experts, vec, [&](auto tag, auto j, auto v) -> int {
+    balance_kernel<decltype(tag), decltype(j)::value, decltype(v)::value><<<grid, kRouteThreads, 0, stream>>>(a);
+    trace_mark(stream, kTraceBalanceLoss);
+    return (int)cudaGetLastError();
+  });
+}
+
+extern "C" int tb200_balance_loss_backward(const tb200_rows* logits, int dtype, const float* d_weights,
+                                           const float* d_dloss, const uint8_t* d_mask, const void* d_offsets,
+                                           int offset_bytes, uint64_t sequences, uint64_t rows, uint32_t experts,
+                                           const tb200_rows* dlogits, tb200_stream_t stream) {
+  using namespace tb200;
+  const int tb = model_bytes(dtype);
+  if (experts == 0) return TB200_ERR_INVALID_ARGUMENT;
+  if (tb == 0 || experts > kMaxBalanceExperts || sequences > 0x7fffffffull || rows > (1ull << 40)) return TB200_ERR_UNSUPPORTED;
+  if (offset_bytes != 0 && offset_bytes != 4 && offset_bytes != 8) return TB200_ERR_INVALID_ARGUMENT;
+  if (offset_bytes == 0 && sequences != 1) return TB200_ERR_INVALID_ARGUMENT;
+  if (rows == 0) return TB200_OK;
+  if (!good_rows(logits, tb) || !good_rows(dlogits, tb)) return TB200_ERR_INVALID_ARGUMENT;
+  if (offset_bytes && (!d_offsets || reinterpret_cast<uintptr_t>(d_offsets) % offset_bytes)) return TB200_ERR_INVALID_ARGUMENT;
+  if (sequences && (!d_weights || !d_dloss)) return TB200_ERR_INVALID_ARGUMENT;
+  if ((reinterpret_cast<uintptr_t>(d_weights) | reinterpret_cast<uintptr_t>(d_dloss)) % 4) return TB200_ERR_INVALID_ARGUMENT;
+  BalanceBackArgs a{};
+  a.z = rows_of(logits, true);
+  a.dz = rows_of(dlogits, true);
+  a.weights = d_weights;
+  a.dloss = d_dloss;
+  a.mask = d_mask;
+  a.spans = Spans{d_offsets, offset_bytes, sequences, rows};
+  a.experts = experts;
+  a.lanes = lanes_of(experts);
+  a.rows_of_warp = 4ull * (kWarp / a.lanes);
+  const uint64_t warps = (rows + a.rows_of_warp - 1) / a.rows_of_warp;
+  const uint64_t grid = (warps + kRouteWarps - 1) / kRouteWarps;
+  if (grid > 0x7fffffffull) return TB200_ERR_UNSUPPORTED;
+  const bool vec = experts % 8 == 0 && rows_on(a.z, tb, 16) && rows_on(a.dz, tb, 16);
+  return by_row(dtype, experts, vec, [&](auto tag, auto j, auto v) -> int {
+    balance_backward_kernel<decltype(tag), decltype(j)::value, decltype(v)::value>
+        <<<(unsigned)grid, kRouteThreads, 0, stream>>>(a);
+    trace_mark(stream, kTraceBalanceLoss);
+    return (int)cudaGetLastError();
+  });
+}

@@ -1,4 +1,5 @@
-"""Operators of language models that are scans and histograms: the gated linear recurrence of a recurrent layer.
+"""Operators of language models that are scans and histograms: the gated linear recurrence of a recurrent layer, and the
+statistics of routing its tokens to experts.
 
 Like the rest of this package they take CUDA tensors, enqueue on the current stream of their device and, unless
 ``sync=False``, synchronise and check the device status before returning. Gradients are calls of their own; nothing
@@ -39,7 +40,7 @@ def _float_code(t: torch.Tensor, name: str) -> int:
 def _rows(t: torch.Tensor, name: str) -> capi.Rows:
     """A [rows, channels] or [sequences, rows, channels] tensor whose channels are adjacent, by its strides."""
     stride = t.stride()
-    if stride[-1] != 1 and t.shape[-1] > 1:
+    if stride[-1] != 1 and t.shape[-1] > 1 and t.numel():
         raise ValueError(f"the channels of {name} must be adjacent in memory (its last stride is {stride[-1]})")
     return capi.Rows(t.data_ptr(), stride[-2], stride[0] if t.dim() == 3 else 0)
 
@@ -200,4 +201,134 @@ def linear_recurrence_step(state: torch.Tensor, x: torch.Tensor, gate: torch.Ten
         capi.check(capi.lib.tb200_linear_recurrence_step(
             rs.data, state.shape[0], max(rs.row_stride, channels), sptr, sbytes, C.byref(rg), C.byref(rx), C.byref(ry), rows,
             channels, gate.shape[1], xd, gd, int(bool(log_gate)), _stream(x)), "tb200_linear_recurrence_step")
+    return out
+
+
+def _ids(ids: torch.Tensor) -> Tuple[int, int, int, int]:
+    """(rows, ids of a row, distance of rows, bytes of an id)"""
+    if ids.dtype not in _INDEX_BYTES or ids.dim() not in (1, 2):
+        raise ValueError("ids must be an int32 or int64 tensor [rows, k], or [rows]")
+    if ids.dim() == 1:
+        return ids.shape[0], 1, ids.stride(0) if ids.shape[0] > 1 else 1, _INDEX_BYTES[ids.dtype]
+    rows, k = ids.shape
+    if k == 0 or (rows and k > 1 and ids.stride(1) != 1) or (rows > 1 and ids.stride(0) < k):
+        raise ValueError("the ids of a row must be adjacent in memory, at least one, and rows must not overlap")
+    return rows, k, ids.stride(0) if rows > 1 else k, _INDEX_BYTES[ids.dtype]
+
+
+def _mask(mask: Optional[torch.Tensor], rows: int) -> Optional[int]:
+    if mask is None:
+        return None
+    if mask.dtype not in (torch.bool, torch.uint8) or mask.shape != (rows,) or not mask.is_contiguous():
+        raise ValueError("mask must be a contiguous 1-D tensor of a bool or uint8 for each row")
+    return mask.data_ptr()
+
+
+@lru_cache(maxsize=512)
+def _counts_bytes(experts: int) -> int:
+    need = C.c_size_t(0)
+    capi.check(capi.lib.tb200_expert_counts(None, C.byref(need), None, 0, 1, 1, 8, None, experts, None, None, None),
+               "tb200_expert_counts(size)")
+    return need.value
+
+
+@lru_cache(maxsize=512)
+def _balance_bytes(dtype: int, offset_bytes: int, sequences: int, experts: int) -> int:
+    need = C.c_size_t(0)
+    capi.check(capi.lib.tb200_balance_loss(None, C.byref(need), None, dtype, None, 1, 1, 8, None, None, offset_bytes,
+                                           sequences, 0, experts, None, None, None, None), "tb200_balance_loss(size)")
+    return need.value
+
+
+def expert_counts(ids: torch.Tensor, experts: int, mask: Optional[torch.Tensor] = None, sync: bool = True,
+                  temp: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Tokens per expert: returns (counts [experts], begins [experts + 1]), int64.
+
+    ids: the experts that each row (token) was routed to, int32 or int64, [rows, k] with the ids of a row adjacent, or
+    [rows]. counts[e] is how often e occurs in rows whose mask (bool [rows], None: all) is set; ids outside
+    [0, experts) are not counted. begins is the exclusive prefix sum of the counts: where each expert's tokens begin
+    once (id, token) pairs are sorted with ``sort_by_key``. At most 8192 experts."""
+    _require_cuda(ids.device, ids=ids, mask=mask)
+    rows, k, stride, width = _ids(ids)
+    mptr = _mask(mask, rows)
+    need = _counts_bytes(experts)
+    both = torch.empty(2 * experts + 1, dtype=torch.int64, device=ids.device)
+    counts, begins = both[:experts], both[experts:]
+    with _On(ids.device):
+        stream = _stream(ids)
+        if temp is None or temp.numel() < need:
+            temp = _temp(need, ids.device)
+        have = C.c_size_t(temp.numel())
+        capi.check(capi.lib.tb200_expert_counts(temp.data_ptr(), C.byref(have), ids.data_ptr(), rows, k, stride, width,
+                                                mptr, experts, counts.data_ptr(), begins.data_ptr(), stream),
+                   "tb200_expert_counts")
+        _finish(temp, stream, "tb200_expert_counts", sync)
+    return counts, begins
+
+
+def _logits(logits: torch.Tensor, offsets: Optional[torch.Tensor]):
+    if logits.dim() != 2 or logits.shape[1] == 0:
+        raise ValueError("logits must be [rows, experts]")
+    obytes, optr = _offsets(offsets)
+    return _float_code(logits, "logits"), obytes, optr, 1 if offsets is None else offsets.numel() - 1
+
+
+def balance_loss(logits: torch.Tensor, ids: torch.Tensor, mask: Optional[torch.Tensor] = None,
+                 offsets: Optional[torch.Tensor] = None, sync: bool = True,
+                 temp: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Balance loss of a router: returns (loss [sequences], counts [sequences, experts], weights [sequences, experts]).
+
+    logits: [rows, experts], float32, float16 or bfloat16, at most 1024 experts; ids: the k experts chosen for each
+    row, as in ``expert_counts``; mask: rows to look at. With ``offsets`` (as in ``linear_recurrence``) the loss of
+    every packed sequence, without them one loss over all rows:
+
+        experts / (k * n^2) * sum_e counts[e] * sum_t softmax(logits[t])[e],   n = unmasked rows
+
+    which is 1 when both are balanced, and 0 without any rows. A logit of -inf is a disabled expert; a row of nothing
+    else has no probabilities. weights is the derivative of a sequence's loss by each of its probabilities: what
+    ``balance_loss_backward`` needs besides the logits. Results are reproducible from run to run."""
+    _require_cuda(logits.device, logits=logits, ids=ids, mask=mask, offsets=offsets)
+    dtype, obytes, optr, sequences = _logits(logits, offsets)
+    rows, k, stride, width = _ids(ids)
+    if rows != logits.shape[0]:
+        raise ValueError("logits and ids differ in rows")
+    experts = logits.shape[1]
+    mptr, rz = _mask(mask, rows), _rows(logits, "logits")
+    need = _balance_bytes(dtype, obytes, sequences, experts)
+    loss = torch.empty(sequences, dtype=torch.float32, device=logits.device)
+    counts = torch.empty((sequences, experts), dtype=torch.int64, device=logits.device)
+    weights = torch.empty((sequences, experts), dtype=torch.float32, device=logits.device)
+    with _On(logits.device):
+        stream = _stream(logits)
+        if temp is None or temp.numel() < need:
+            temp = _temp(need, logits.device)
+        have = C.c_size_t(temp.numel())
+        capi.check(capi.lib.tb200_balance_loss(
+            temp.data_ptr(), C.byref(have), C.byref(rz), dtype, ids.data_ptr(), k, stride, width, mptr, optr, obytes,
+            sequences, rows, experts, loss.data_ptr(), counts.data_ptr(), weights.data_ptr(), stream),
+            "tb200_balance_loss")
+        _finish(temp, stream, "tb200_balance_loss", sync)
+    return loss, counts, weights
+
+
+def balance_loss_backward(logits: torch.Tensor, weights: torch.Tensor, dloss: torch.Tensor,
+                          mask: Optional[torch.Tensor] = None, offsets: Optional[torch.Tensor] = None,
+                          out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Gradient of ``balance_loss`` by the logits, in their type, from its weights and dloss (float32 [sequences], the
+    gradient of the losses); mask and offsets as in the forward call. Zero for masked rows and rows of no sequence.
+    ``out`` may be logits. Enqueues one kernel and returns without waiting."""
+    _require_cuda(logits.device, logits=logits, weights=weights, dloss=dloss, mask=mask, offsets=offsets, out=out)
+    dtype, obytes, optr, sequences = _logits(logits, offsets)
+    rows, experts = logits.shape
+    wptr = _states(weights, (sequences, experts), "weights")
+    lptr = _states(dloss, (sequences,), "dloss")
+    if out is None:
+        out = torch.empty((rows, experts), dtype=logits.dtype, device=logits.device)
+    elif out.shape != logits.shape or out.dtype != logits.dtype:
+        raise ValueError("out must have the shape and type of logits")
+    mptr, rz, rd = _mask(mask, rows), _rows(logits, "logits"), _rows(out, "out")
+    with _On(logits.device):
+        capi.check(capi.lib.tb200_balance_loss_backward(C.byref(rz), dtype, wptr, lptr, mptr, optr, obytes, sequences, rows,
+                                                        experts, C.byref(rd), _stream(logits)),
+                   "tb200_balance_loss_backward")
     return out
