@@ -44,6 +44,10 @@ struct RecArgs {
   float* last;                  // forward: final states; backward: gradient of the initial states
   float* partial;               // backward, a head over several blocks: their sums, [rows][heads][parts]
   TempHeader* hdr;
+  uint32_t blocks, chains;      // blocks of channels, chains
+  uint64_t tiles;               // of a chain
+  unsigned long long* maps;     // [tile][chain][block][channel]: what the tile does to a state (0: not there yet)
+  unsigned* states;             // [tile][chain][block][channel]: the state behind the tile (0: not there yet)
 };
 
 // A of a stretch in one word: A - 1 with the lowest bit set where A >= 1/2, else A with it clear. The bit costs at
@@ -54,6 +58,55 @@ __device__ __forceinline__ unsigned word_of(float a, float m) {
 __device__ __forceinline__ float apply(unsigned word, float h, float b) {  // A * h + b
   const float u = fmaf(__uint_as_float(word), h, b);
   return (word & 1u) ? h + u : u;
+}
+
+// Descriptors hold the complement, so that cleared scratch means "not there yet"; the two values whose complement
+// would be zero are NaNs and give way to other NaNs.
+__device__ __forceinline__ unsigned long long map_bits(unsigned word, float b) {
+  if (word == 0xffffffffu) word = 0xfffffffdu;
+  return ~((unsigned long long)word << 32 | __float_as_uint(b));
+}
+__device__ __forceinline__ unsigned state_bits(float h) {
+  const unsigned u = __float_as_uint(h);
+  return ~(u == 0xffffffffu ? 0x7fffffffu : u);
+}
+
+// The state in front of a tile, for one channel: from the nearest known state among the tiles in front, through the maps
+// of the tiles between, in the order of the rows. A known state is itself the one in front of its tile put through that
+// tile's map, so the value is the same wherever the walk begins, to the bit. At most kReach tiles back; where no state is
+// known there, the wait is for one to come closer, which the tile right behind the last known state always brings about.
+constexpr int kReach = 8;
+__device__ float state_in_front(const unsigned long long* maps, const unsigned* states, uint64_t step, uint64_t tile, int* status) {
+  const int n = tile < kReach ? (int)tile : kReach;
+  for (unsigned polls = 0;; ++polls) {
+    unsigned long long m[kReach];
+    unsigned s[kReach];
+#pragma unroll
+    for (int j = 0; j < kReach; ++j) {
+      s[j] = j < n ? ld_relaxed_u32(states - (j + 1) * step) : 0u;
+      m[j] = j < n ? ld_relaxed_u64(maps - (j + 1) * step) : 0ull;
+    }
+    float h = 0.0f;
+    bool known = false;
+#pragma unroll
+    for (int j = kReach - 1; j >= 0; --j) {
+      if (s[j] != 0u) {
+        h = __uint_as_float(~s[j]);
+        known = true;
+      } else if (m[j] != 0ull) {
+        h = apply((unsigned)(~m[j] >> 32), h, __uint_as_float((unsigned)~m[j]));
+      } else {
+        known = false;
+      }
+    }
+    if (known) return h;
+    if ((polls & 63u) == 63u && ld_relaxed_s32(status) != 0) return h;  // someone else gave up
+    if (polls >= kSpinLimit) {
+      note_timeout(status, kSiteLookback, tile, 0);
+      return h;
+    }
+    backoff(polls);
+  }
 }
 
 struct Marks {           // of the rows of a tile; packed sequences fill it in shared memory
@@ -97,7 +150,7 @@ __device__ void mark_rows(const RecArgs& p, uint64_t r0, uint64_t r1, bool at_en
 }
 
 template <typename T, typename G, int V, bool SHARED, bool BACK, int R>
-__global__ void __launch_bounds__(kThreads) recurrence_kernel(RecArgs p) {
+__global__ void __launch_bounds__(kThreads, 2) recurrence_kernel(RecArgs p) {
   constexpr int WIDTH = kWarp * V;
   constexpr int GV = SHARED ? 1 : V;  // gates of a lane in a row
   constexpr int TILE = kWarps * R;
@@ -106,24 +159,39 @@ __global__ void __launch_bounds__(kThreads) recurrence_kernel(RecArgs p) {
   __shared__ unsigned s_word[kWarps][WIDTH];
   __shared__ float s_b[kWarps][WIDTH];
   __shared__ float s_carry[kWarps][WIDTH];
-  __shared__ int s_reset[kWarps];
-  __shared__ float s_state[WIDTH];
+  __shared__ int s_reset[kWarps];  // a sequence begins among the warp's rows
+  __shared__ int s_need[kWarps];   // the warp has rows in front of that
+  __shared__ unsigned s_ticket;
 
   const unsigned lane = lane_id(), warp = threadIdx.x / kWarp;
   const bool logg = p.log_gate != 0;
-  const uint64_t chain = blockIdx.y;
+
+  // Tiles are handed out in the order of the recurrence, all chains and blocks of channels of one stretch of rows before
+  // the next: whatever a tile waits for is worked on by a CTA that runs already.
+  unsigned id = blockIdx.x;
+  if (p.tiles > 1) {
+    if (threadIdx.x == 0) s_ticket = atomicAdd(&p.hdr->ticket, 1u);
+    __syncthreads();
+    id = s_ticket;
+  } else if (id == 0) {  // the scratch is not cleared where no tile waits for another
+    if (threadIdx.x == 0) p.hdr->status = TB200_OK;
+    __syncthreads();
+  }
+  const uint32_t block = id % p.blocks;
+  const uint64_t chain = id / p.blocks % p.chains;
+  const uint64_t tile = id / p.blocks / p.chains;
 
   // the block's channels
   uint32_t c0, count;
   if (!SHARED) {
-    c0 = blockIdx.x * WIDTH;
+    c0 = block * WIDTH;
     count = min((uint32_t)WIDTH, p.channels - c0);
   } else if (p.parts == 1) {
-    const uint32_t h0 = blockIdx.x * p.block_heads;
+    const uint32_t h0 = block * p.block_heads;
     c0 = h0 * p.head_size;
     count = min(p.block_heads, p.heads - h0) * p.head_size;
   } else {
-    const uint32_t h0 = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
+    const uint32_t h0 = block / p.parts, part = block % p.parts;
     c0 = h0 * p.head_size + part * WIDTH;
     count = min((uint32_t)WIDTH, p.head_size - part * WIDTH);
   }
@@ -132,7 +200,7 @@ __global__ void __launch_bounds__(kThreads) recurrence_kernel(RecArgs p) {
   const uint32_t head = SHARED ? ch / p.head_size : 0;
   const uint32_t gate_at = SHARED ? head : ch;
 
-  if (p.offsets != nullptr && blockIdx.x == 0) {  // bad offsets are reported, and cannot lead outside the arrays
+  if (p.offsets != nullptr && id == 0) {  // bad offsets are reported, and cannot lead outside the arrays
     bool bad = false;
     for (uint64_t i = threadIdx.x; i <= p.sequences; i += kThreads) {
       const int64_t v = p.offset_bytes == 4 ? (int64_t)static_cast<const int32_t*>(p.offsets)[i]
@@ -142,12 +210,10 @@ __global__ void __launch_bounds__(kThreads) recurrence_kernel(RecArgs p) {
     if (bad) atomicExch(&p.hdr->status, (int)TB200_ERR_INVALID_ARGUMENT);
   }
 
-  if (threadIdx.x < WIDTH) s_state[threadIdx.x] = 0.0f;
-  const uint64_t tiles = (p.chain_rows + TILE - 1) / TILE;
   const uint64_t used_from = p.offsets ? offset_at(p, 0) : 0;
   const uint64_t used_to = p.offsets ? offset_at(p, p.sequences) : p.chain_rows;
 
-  for (uint64_t tile = 0; tile < tiles; ++tile) {
+  {
     // ---- what the warp's rows are: lane l holds logical row l --------------------------------------
     const uint64_t q = tile * TILE + warp * R + lane;
     const bool valid = lane < R && q < p.chain_rows;
@@ -260,17 +326,50 @@ __global__ void __launch_bounds__(kThreads) recurrence_kernel(RecArgs p) {
       s_word[warp][lane * V + i] = word_of(A[SHARED ? 0 : i], M[SHARED ? 0 : i]);
       s_b[warp][lane * V + i] = B[i];
     }
-    if (lane == 0) s_reset[warp] = (m_begin & m_inside) != 0;
+    if (lane == 0) {
+      s_reset[warp] = m_begin != 0;
+      s_need[warp] = (m_inside & ((m_begin & -m_begin) - 1u)) != 0;  // rows in front of the first begin; all without one
+    }
     __syncthreads();
 
     // ---- the states in front of the warps' stretches -------------------------------------------------------
     if (threadIdx.x < WIDTH) {
-      float h = s_state[threadIdx.x];
+      // the whole tile's map; behind a begin only B counts
+      bool reset = false, need = false;
+      float ta = 1.0f, tm = 0.0f, tb = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const unsigned word = s_word[w][threadIdx.x];
+        const float v = __uint_as_float(word), b = s_b[w][threadIdx.x];
+        const float wa = (word & 1u) ? 1.0f + v : v, wm = (word & 1u) ? v : v - 1.0f;
+        need = need || (!reset && s_need[w]);
+        reset = reset || s_reset[w];
+        tb = s_reset[w] ? b : apply(word, tb, b);
+        ta *= wa;
+        tm = fmaf(tm, wa, wm);
+      }
+      float h = 0.0f;
+      if (p.tiles > 1) {
+        const uint64_t at = (uint64_t)id * WIDTH + threadIdx.x, step = (uint64_t)p.chains * p.blocks * WIDTH;
+        const unsigned word = word_of(ta, tm);
+        const bool last_tile = tile + 1 == p.tiles;
+        if (!last_tile) {
+          if (reset || tile == 0) st_relaxed_u32(p.states + at, state_bits(tb));
+          else st_relaxed_u64(p.maps + at, map_bits(word, tb));
+        }
+        if (need && tile > 0) {
+          h = state_in_front(p.maps + at, p.states + at, step, tile, &p.hdr->status);
+          if (!reset && !last_tile) st_relaxed_u32(p.states + at, state_bits(apply(word, h, tb)));
+        } else if (!need && !reset && tile > 0 && !last_tile) {
+          // no row of the tile belongs to a sequence: nobody behind it needs a state before a sequence begins
+          st_relaxed_u32(p.states + at, state_bits(0.0f));
+        }
+      }
+#pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         s_carry[w][threadIdx.x] = h;
         h = s_reset[w] ? s_b[w][threadIdx.x] : apply(s_word[w][threadIdx.x], h, s_b[w][threadIdx.x]);
       }
-      s_state[threadIdx.x] = h;
     }
     __syncthreads();
 
@@ -342,7 +441,7 @@ __global__ void __launch_bounds__(kThreads) recurrence_kernel(RecArgs p) {
               store_floats<G, 1>(p.dgate.data, rb * p.dgate.seq + rt * p.dgate.row + head, one);
             } else {
               const uint64_t flat = rb * (p.chain_is_sequence || !p.offsets ? p.length : 0) + rt;
-              p.partial[(flat * p.heads + head) * p.parts + blockIdx.x % p.parts] = sum;
+              p.partial[(flat * p.heads + head) * p.parts + block % p.parts] = sum;
             }
           }
         }
@@ -352,7 +451,6 @@ __global__ void __launch_bounds__(kThreads) recurrence_kernel(RecArgs p) {
         for (int i = 0; i < V; ++i) p.last[(uint64_t)s * p.channels + ch + i] = h[i];
       }
     }
-    __syncthreads();
   }
 }
 
@@ -371,31 +469,45 @@ __global__ void __launch_bounds__(kThreads) join_gate_kernel(RecArgs p, uint64_t
   }
 }
 
+// Blocks of channels for V channels a lane.
+void divide_channels(RecArgs& p, uint32_t width) {
+  if (p.heads == p.channels) {
+    p.blocks = (p.channels + width - 1) / width;
+    p.parts = 1;
+  } else if (p.head_size <= width) {
+    p.block_heads = width / p.head_size;
+    p.parts = 1;
+    p.blocks = (p.heads + p.block_heads - 1) / p.block_heads;
+  } else {
+    p.parts = (p.head_size + width - 1) / width;
+    p.blocks = p.heads * p.parts;
+  }
+}
+
+constexpr int kRows = 8;  // rows of a lane
+constexpr uint64_t kTileRows = kWarps * kRows;
+
 struct Call {
   tb200_recurrence_shape shape;
   RecArgs args;
-  uint64_t rows;  // of all sequences
-  uint32_t blocks;
+  uint64_t rows;     // of all sequences
+  char* descriptors;
 };
 
 template <typename T, typename G, int V, bool SHARED, bool BACK>
 int launch_kernel(Call& k, cudaStream_t stream) {
   RecArgs& p = k.args;
   constexpr uint32_t WIDTH = kWarp * V;
-  if (!SHARED) {
-    k.blocks = (p.channels + WIDTH - 1) / WIDTH;
-    p.parts = 1;
-  } else if (p.head_size <= WIDTH) {
-    p.block_heads = WIDTH / p.head_size;
-    p.parts = 1;
-    k.blocks = (p.heads + p.block_heads - 1) / p.block_heads;
-  } else {
-    p.parts = (p.head_size + WIDTH - 1) / WIDTH;
-    k.blocks = p.heads * p.parts;
+  divide_channels(p, WIDTH);
+  const uint64_t ctas = p.tiles * p.chains * p.blocks;
+  if (ctas > 0x7fffffffull) return TB200_ERR_UNSUPPORTED;
+  if (p.tiles > 1) {
+    const size_t states = ctas * WIDTH;
+    p.states = reinterpret_cast<unsigned*>(k.descriptors);
+    p.maps = reinterpret_cast<unsigned long long*>(k.descriptors + states * sizeof(unsigned));
+    TB200_CUDA_TRY(cudaMemsetAsync(p.hdr, 0, kHeaderBytes + states * (sizeof(unsigned) + sizeof(unsigned long long)), stream));
   }
-  const uint64_t chains = p.chain_is_sequence ? p.sequences : 1;
-  if (chains > 65535) return TB200_ERR_UNSUPPORTED;
-  recurrence_kernel<T, G, V, SHARED, BACK, 8><<<dim3(k.blocks, (unsigned)chains), kThreads, 0, stream>>>(p);
+  recurrence_kernel<T, G, V, SHARED, BACK, kRows><<<(unsigned)ctas, kThreads, 0, stream>>>(p);
   trace_mark(stream, kTraceRecurrence);
   TB200_CUDA_TRY(cudaGetLastError());
   if (BACK && SHARED && p.parts > 1) {
@@ -448,16 +560,6 @@ int prepare(void* d_temp, size_t* temp_bytes, const tb200_recurrence_shape* shap
   k.shape = s;
   k.rows = s.offset_bytes ? s.rows : s.sequences * s.rows;
   const uint64_t head_size = s.channels / s.heads;
-  size_t need = kHeaderBytes;
-  // a head over several blocks of channels leaves a sum for each of them; the narrowest blocks have 32 channels
-  if (back && s.heads != s.channels && head_size > kWarp)
-    need += align_up(k.rows * s.heads * ((head_size + kWarp - 1) / kWarp) * sizeof(float), 256);
-  if (d_temp == nullptr) {
-    *temp_bytes = need;
-    return TB200_OK;
-  }
-  if (*temp_bytes < need) return TB200_ERR_TEMP_TOO_SMALL;
-  if (reinterpret_cast<uintptr_t>(d_temp) % 256) return TB200_ERR_INVALID_ARGUMENT;
   RecArgs& p = k.args;
   p = RecArgs{};
   p.offset_bytes = s.offset_bytes;
@@ -465,13 +567,41 @@ int prepare(void* d_temp, size_t* temp_bytes, const tb200_recurrence_shape* shap
   p.fill = s.fill_outside;
   p.sequences = s.sequences;
   p.length = s.rows;
-  p.chain_is_sequence = s.offset_bytes == 0;
-  p.chain_rows = s.rows;
   p.channels = (uint32_t)s.channels;
   p.heads = (uint32_t)s.heads;
-  p.head_size = (uint32_t)head_size;
+  p.head_size = (uint32_t)(s.channels / s.heads);
+  // Sequences of equal length are chains of their own, unless they are so short that their tiles would be mostly empty:
+  // then all of them are one chain, as packed ones are.
+  p.chain_is_sequence = s.offset_bytes == 0 && s.rows > kTileRows / 2;
+  p.chains = p.chain_is_sequence ? (uint32_t)s.sequences : 1;
+  p.chain_rows = p.chain_is_sequence ? s.rows : k.rows;
+  p.tiles = (p.chain_rows + kTileRows - 1) / kTileRows;
+
+  // Descriptors lie directly behind the header, where one clear reaches both; the sums of heads that span several
+  // blocks lie behind them. The pointers' alignment decides on four or one channels a lane: room for either.
+  size_t descriptors = 0, sums = 0;
+  for (uint32_t width = kWarp; width <= 4 * kWarp; width *= 4) {
+    divide_channels(p, width);
+    if (p.tiles > 1) {
+      const size_t d = p.tiles * p.chains * p.blocks * width * (sizeof(unsigned) + sizeof(unsigned long long));
+      if (d > descriptors) descriptors = d;
+    }
+    if (back && p.parts > 1) {
+      const size_t b = k.rows * p.heads * p.parts * sizeof(float);
+      if (b > sums) sums = b;
+    }
+  }
+  descriptors = align_up(descriptors, 256);
+  const size_t need = kHeaderBytes + descriptors + align_up(sums, 256);
+  if (d_temp == nullptr) {
+    *temp_bytes = need;
+    return TB200_OK;
+  }
+  if (*temp_bytes < need) return TB200_ERR_TEMP_TOO_SMALL;
+  if (reinterpret_cast<uintptr_t>(d_temp) % 256) return TB200_ERR_INVALID_ARGUMENT;
   p.hdr = static_cast<TempHeader*>(d_temp);
-  p.partial = reinterpret_cast<float*>(static_cast<char*>(d_temp) + kHeaderBytes);
+  k.descriptors = static_cast<char*>(d_temp) + kHeaderBytes;
+  p.partial = reinterpret_cast<float*>(k.descriptors + descriptors);
   return TB200_OK;
 }
 
@@ -500,8 +630,10 @@ extern "C" int tb200_linear_recurrence(void* d_temp, size_t* temp_bytes, const t
   const int tb = model_bytes(k.shape.dtype);
   if (some && !(good_rows(gate, model_bytes(k.shape.gate_dtype)) && good_rows(x, tb) && good_rows(y, tb)))
     return TB200_ERR_INVALID_ARGUMENT;
-  TB200_CUDA_TRY(cudaMemsetAsync(d_temp, 0, kHeaderBytes, stream));
-  if (!some) return hand_through(k, d_initial, d_final, stream);
+  if (!some) {
+    TB200_CUDA_TRY(cudaMemsetAsync(d_temp, 0, kHeaderBytes, stream));
+    return hand_through(k, d_initial, d_final, stream);
+  }
   RecArgs& p = k.args;
   p.offsets = packed ? d_offsets : nullptr;
   p.gate = rows_of(gate, packed);
@@ -527,8 +659,10 @@ extern "C" int tb200_linear_recurrence_backward(void* d_temp, size_t* temp_bytes
   const int tb = model_bytes(k.shape.dtype), gb = model_bytes(k.shape.gate_dtype);
   if (some && !(good_rows(gate, gb) && good_rows(y, tb) && good_rows(dy, tb) && good_rows(dx, tb) && good_rows(dgate, gb)))
     return TB200_ERR_INVALID_ARGUMENT;
-  TB200_CUDA_TRY(cudaMemsetAsync(d_temp, 0, kHeaderBytes, stream));
-  if (!some) return hand_through(k, d_dfinal, d_dinitial, stream);
+  if (!some) {
+    TB200_CUDA_TRY(cudaMemsetAsync(d_temp, 0, kHeaderBytes, stream));
+    return hand_through(k, d_dfinal, d_dinitial, stream);
+  }
   RecArgs& p = k.args;
   p.offsets = packed ? d_offsets : nullptr;
   p.gate = rows_of(gate, packed);
