@@ -18,6 +18,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <initializer_list>
 
 #include "model_common.cuh"
 
@@ -109,9 +110,10 @@ __device__ float state_in_front(const unsigned long long* maps, const unsigned* 
   }
 }
 
-struct Marks {           // of the rows of a tile; packed sequences fill it in shared memory
-  int seq[kWarps * 16];  // sequence of a first or last row
-  unsigned char kind[kWarps * 16];  // bit 0: first row of its sequence, bit 1: last
+constexpr int kMaxRows = 16;  // rows of a lane, at most
+struct Marks {           // of the rows of a tile of packed sequences
+  int seq[kWarps * kMaxRows];  // sequence of a first or last row
+  unsigned char kind[kWarps * kMaxRows];  // bit 0: first row of its sequence, bit 1: last
 };
 
 __device__ __forceinline__ uint64_t offset_at(const RecArgs& p, uint64_t i) {
@@ -121,16 +123,23 @@ __device__ __forceinline__ uint64_t offset_at(const RecArgs& p, uint64_t i) {
 }
 
 // Marks the first and last rows of sequences among rows [r0, r1), in memory order; hands the states of empty sequences
-// that lie here through for channels [c0, c0 + count).
+// that lie here through for channels [c0, c0 + count). One warp does it; the others wait at the barrier behind.
 __device__ void mark_rows(const RecArgs& p, uint64_t r0, uint64_t r1, bool at_end, uint32_t c0, uint32_t count, Marks& m) {
-  for (int i = threadIdx.x; i < (int)(sizeof(m.kind) / sizeof(m.kind[0])); i += kThreads) m.kind[i] = 0;
-  __syncthreads();
-  uint64_t lo = 0, hi = p.sequences + 1;  // first boundary at or behind r0
+  const unsigned lane = lane_id();
+  for (int i = lane; i < (int)sizeof(m.kind) / 4; i += kWarp) reinterpret_cast<unsigned*>(m.kind)[i] = 0;
+  __syncwarp();
+  // first boundary at or behind r0: every step looks at 32 boundaries at once
+  uint64_t lo = 0, hi = p.sequences + 1;
   while (lo < hi) {
-    const uint64_t mid = (lo + hi) / 2;
-    if (offset_at(p, mid) < r0) lo = mid + 1; else hi = mid;
+    const uint64_t stride = (hi - lo + kWarp - 1) / kWarp;
+    const uint64_t at = lo + (lane + 1) * stride - 1;  // the last of the lane's stretch
+    const unsigned in_front = __ballot_sync(0xffffffffu, at < hi && offset_at(p, at) < r0);
+    const int skip = __popc(in_front);  // stretches that lie wholly in front of r0
+    lo += skip * stride;
+    const uint64_t end = lo + stride - 1;  // the next stretch ends at or behind r0, unless it is cut
+    if (end < hi) hi = end;
   }
-  for (uint64_t j = lo + threadIdx.x; j <= p.sequences; j += kThreads) {
+  for (uint64_t j = lo + lane; j <= p.sequences; j += kWarp) {
     const uint64_t v = offset_at(p, j);
     if (v > r1) break;
     if (j > 0 && v > r0 && offset_at(p, j - 1) < v) {  // sequence j - 1 ends in front of boundary j
@@ -154,7 +163,8 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_kernel(RecArgs p) {
   constexpr int WIDTH = kWarp * V;
   constexpr int GV = SHARED ? 1 : V;  // gates of a lane in a row
   constexpr int TILE = kWarps * R;
-  static_assert(TILE <= kWarps * 16 && R <= kWarp, "marks and row information are sized for this");
+  constexpr unsigned ALL = (unsigned)((1ull << R) - 1);
+  static_assert(R <= kMaxRows, "marks are sized for this");
   __shared__ Marks s_marks;
   __shared__ unsigned s_word[kWarps][WIDTH];
   __shared__ float s_b[kWarps][WIDTH];
@@ -178,7 +188,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_kernel(RecArgs p) {
     __syncthreads();
   }
   const uint32_t block = id % p.blocks;
-  const uint64_t chain = id / p.blocks % p.chains;
+  const uint32_t chain = id / p.blocks % p.chains;
   const uint64_t tile = id / p.blocks / p.chains;
 
   // the block's channels
@@ -200,191 +210,197 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_kernel(RecArgs p) {
   const uint32_t head = SHARED ? ch / p.head_size : 0;
   const uint32_t gate_at = SHARED ? head : ch;
 
-  if (p.offsets != nullptr && id == 0) {  // bad offsets are reported, and cannot lead outside the arrays
-    bool bad = false;
-    for (uint64_t i = threadIdx.x; i <= p.sequences; i += kThreads) {
-      const int64_t v = p.offset_bytes == 4 ? (int64_t)static_cast<const int32_t*>(p.offsets)[i]
-                                            : static_cast<const int64_t*>(p.offsets)[i];
-      bad = bad || v < 0 || (uint64_t)v > p.length || (i == 0 ? v != 0 : (uint64_t)v < offset_at(p, i - 1));
-    }
-    if (bad) atomicExch(&p.hdr->status, (int)TB200_ERR_INVALID_ARGUMENT);
-  }
+  // ---- load: the warp's rows run from `row` with the recurrence, `n` of them exist ----------------------
+  const uint64_t q = tile * TILE + warp * R;
+  const int n = q >= p.chain_rows ? 0 : p.chain_rows - q < R ? (int)(p.chain_rows - q) : R;
+  const int64_t row = BACK ? (int64_t)p.chain_rows - 1 - (int64_t)q : (int64_t)q;  // below zero only where n is 0
+  auto at = [&](const RowsOf& a, uint32_t column) { return (int64_t)(chain * a.seq + column) + row * (int64_t)a.row; };
+  auto next = [](const RowsOf& a) { return BACK ? -(int64_t)a.row : (int64_t)a.row; };
 
-  const uint64_t used_from = p.offsets ? offset_at(p, 0) : 0;
-  const uint64_t used_to = p.offsets ? offset_at(p, p.sequences) : p.chain_rows;
-
+  Pack<G, GV> gate[R];
+  Pack<T, V> x[R];
+  Pack<T, V> before[BACK ? R : 1];  // y of the row in front, in memory
   {
-    // ---- what the warp's rows are: lane l holds logical row l --------------------------------------
-    const uint64_t q = tile * TILE + warp * R + lane;
-    const bool valid = lane < R && q < p.chain_rows;
-    const uint64_t row = valid ? (BACK ? p.chain_rows - 1 - q : q) : 0;  // in the chain
-    uint64_t b = 0, t = row;
-    if (p.chain_is_sequence) {
-      b = chain;
-    } else if (p.offsets == nullptr) {
-      b = row / p.length;
-      t = row - b * p.length;
-    }
-    const unsigned m_valid = __ballot_sync(0xffffffffu, valid);
-
-    // ---- load ---------------------------------------------------------------------------------------
-    float c[R][GV];
-    Pack<T, V> x[R];
-    Pack<T, V> yprev[BACK ? R : 1];
-    float sum_g[GV] = {};
+    int64_t eg = at(p.gate, gate_at), ex = at(p.in, ch), ey = BACK ? at(p.y, ch) - (int64_t)p.y.row : 0;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const uint64_t rb = __shfl_sync(0xffffffffu, b, r), rt = __shfl_sync(0xffffffffu, t, r);
-      const bool on = live && (m_valid >> r & 1);
-      Pack<G, GV> g;
-      if (on) {
-        g = load_pack<G, GV>(p.gate.data, rb * p.gate.seq + rt * p.gate.row + gate_at);
-        x[r] = load_pack<T, V>(p.in.data, rb * p.in.seq + rt * p.in.row + ch);
+      if (live && r < n) {
+        gate[r] = load_pack<G, GV>(p.gate.data, eg);
+        x[r] = load_pack<T, V>(p.in.data, ex);
         if constexpr (BACK)
-          if (rt > 0) yprev[r] = load_pack<T, V>(p.y.data, rb * p.y.seq + (rt - 1) * p.y.row + ch);
+          if (row - r > 0) before[r] = load_pack<T, V>(p.y.data, ey);
       }
-#pragma unroll
-      for (int i = 0; i < GV; ++i) c[r][i] = on ? to_f32<G>(g.v[i]) : 0.0f;
+      eg += next(p.gate);
+      ex += next(p.in);
+      if constexpr (BACK) ey += next(p.y);
     }
+  }
 
-    // ---- first and last rows of sequences -------------------------------------------------------------
-    bool first, last, inside = valid;
-    int seq = (int)b;
-    if (p.offsets != nullptr) {
-      const uint64_t lo = tile * TILE, hi = min(lo + TILE, p.chain_rows);
-      const uint64_t r0 = BACK ? p.chain_rows - hi : lo, r1 = BACK ? p.chain_rows - lo : hi;
-      mark_rows(p, r0, r1, r1 == p.chain_rows, c0, count, s_marks);
-      __syncthreads();
-      const unsigned kind = valid ? s_marks.kind[row - r0] : 0;
-      first = kind & 1;
-      last = kind & 2;
-      if (kind) seq = s_marks.seq[row - r0];
-      inside = valid && row >= used_from && row < used_to;
-    } else {
-      first = valid && t == 0;
-      last = valid && t == p.length - 1;
+  // ---- first and last rows of sequences: bit r of a mask is the warp's row r ------------------------------
+  unsigned m_inside = (unsigned)((1ull << n) - 1), m_first = 0, m_last = 0;
+  int seq = chain;  // of row `lane`, where that is a first or last one
+  if (p.offsets != nullptr) {
+    if (id == 0) {  // bad offsets are reported, and cannot lead outside the arrays
+      bool bad = false;
+      for (uint64_t i = threadIdx.x; i <= p.sequences; i += kThreads) {
+        const int64_t v = p.offset_bytes == 4 ? (int64_t)static_cast<const int32_t*>(p.offsets)[i]
+                                              : static_cast<const int64_t*>(p.offsets)[i];
+        bad = bad || v < 0 || (uint64_t)v > p.length || (i == 0 ? v != 0 : (uint64_t)v < offset_at(p, i - 1));
+      }
+      if (bad) atomicExch(&p.hdr->status, (int)TB200_ERR_INVALID_ARGUMENT);
     }
-    const unsigned m_inside = __ballot_sync(0xffffffffu, inside);
-    const unsigned m_first = __ballot_sync(0xffffffffu, first), m_last = __ballot_sync(0xffffffffu, last);
-    const unsigned m_begin = BACK ? m_last : m_first, m_end = BACK ? m_first : m_last;  // with the recurrence
+    const uint64_t lo = tile * TILE, hi = min(lo + TILE, p.chain_rows);
+    const uint64_t r0 = BACK ? p.chain_rows - hi : lo, r1 = BACK ? p.chain_rows - lo : hi;
+    if (warp == 0) mark_rows(p, r0, r1, r1 == p.chain_rows, c0, count, s_marks);
+    __syncthreads();
+    const uint64_t mine = (uint64_t)(BACK ? row - (int)lane : row + (int)lane);
+    const bool valid = (int)lane < n;
+    const unsigned kind = valid ? s_marks.kind[mine - r0] : 0;
+    if (kind) seq = s_marks.seq[mine - r0];
+    m_first = __ballot_sync(0xffffffffu, kind & 1);
+    m_last = __ballot_sync(0xffffffffu, kind & 2);
+    m_inside = __ballot_sync(0xffffffffu, valid && mine >= offset_at(p, 0) && mine < offset_at(p, p.sequences));
+  } else if (p.chain_is_sequence) {
+    if (n > 0) {
+      const unsigned low = q == 0 ? 1u : 0u, high = q + n == p.chain_rows ? 1u << (n - 1) : 0u;
+      m_first = BACK ? high : low;
+      m_last = BACK ? low : high;
+    }
+  } else if (n > 0) {  // sequences of equal length behind one another
+    const uint64_t mine = (uint64_t)(BACK ? row - (int)min((int)lane, n - 1) : row + (int)min((int)lane, n - 1));
+    const uint64_t s = p.chain_rows >> 32 ? mine / p.length : (uint32_t)mine / (uint32_t)p.length;
+    const uint64_t t = mine - s * p.length;
+    seq = (int)s;
+    m_first = __ballot_sync(0xffffffffu, (int)lane < n && t == 0);
+    m_last = __ballot_sync(0xffffffffu, (int)lane < n && t == p.length - 1);
+  }
+  const unsigned m_begin = BACK ? m_last : m_first, m_end = BACK ? m_first : m_last;  // with the recurrence
+  const bool plain_rows = m_inside == ALL && (m_begin | m_end) == 0;  // nothing but rows of one sequence
 
-    // the state that a sequence begins with
-    auto first_state = [&](int r, float (&h)[V]) {
-      const int s = __shfl_sync(0xffffffffu, seq, r);
-      const float* at = p.first + (uint64_t)s * p.channels + ch;
+  // the state that a sequence begins with
+  auto first_state = [&](int r, float (&h)[V]) {
+    const int s = __shfl_sync(0xffffffffu, seq, r);
+    const float* from = p.first + (uint64_t)s * p.channels + ch;
 #pragma unroll
-      for (int i = 0; i < V; ++i) h[i] = live ? at[i] : 0.0f;
-    };
+    for (int i = 0; i < V; ++i) h[i] = live ? from[i] : 0.0f;
+  };
 
-    // ---- first pass: the stretch's A and B --------------------------------------------------------------
-    float A[GV], M[GV], B[V];
+  // ---- first pass: the stretch's A and B --------------------------------------------------------------------
+  float a[R][GV];  // the gates themselves from here on
+  float A[GV], M[GV], B[V];
+  {
+    float sum[GV];
 #pragma unroll
-    for (int i = 0; i < GV; ++i) A[i] = 1.0f, M[i] = 0.0f;
+    for (int i = 0; i < GV; ++i) A[i] = 1.0f, M[i] = 0.0f, sum[i] = 0.0f;
 #pragma unroll
     for (int i = 0; i < V; ++i) B[i] = 0.0f;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      if (!(m_inside >> r & 1)) continue;
-      const bool begin = m_begin >> r & 1;
-      float h[V];
-      if (begin && p.first) first_state(r, h);
+      if (!plain_rows && !(m_inside >> r & 1)) continue;
+      const bool begin = !plain_rows && (m_begin >> r & 1);
+      if (begin) {
+        if (p.first) {
+          first_state(r, B);
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; ++i) B[i] = 0.0f;
+        }
+      }
 #pragma unroll
       for (int i = 0; i < GV; ++i) {
-        const float g = c[r][i];
+        const float g = to_f32<G>(gate[r].v[i]);
         if (logg) {
-          sum_g[i] += g;
+          sum[i] += g;
+          a[r][i] = __expf(g);
         } else {
           A[i] *= g;
           M[i] = fmaf(M[i], g, g - 1.0f);
+          a[r][i] = g;
         }
-        c[r][i] = hold_gate(g, logg);
       }
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float cc = c[r][SHARED ? 0 : i];
-        const bool near = held_near(cc, logg);
-        const float xv = to_f32<T>(x[r].v[i]);
-        if (begin) B[i] = p.first ? h[i] : 0.0f;
+        const float ai = a[r][SHARED ? 0 : i], xv = to_f32<T>(x[r].v[i]);
         if constexpr (BACK) {
-          B[i] = advance(cc, near, xv + B[i], 0.0f);
+          B[i] = ai * (xv + B[i]);
         } else {
-          B[i] = begin && !p.first ? xv : advance(cc, near, B[i], xv);
+          B[i] = begin && !p.first ? xv : fmaf(ai, B[i], xv);
         }
       }
     }
     if (logg) {
 #pragma unroll
       for (int i = 0; i < GV; ++i) {
-        const float cc = hold_gate(sum_g[i], true);
-        const bool near = held_near(cc, true);
-        A[i] = near ? 1.0f + cc : cc;
-        M[i] = near ? cc : cc - 1.0f;
+        const float c = hold_gate(sum[i], true);
+        const bool near = held_near(c, true);
+        A[i] = near ? 1.0f + c : c;
+        M[i] = near ? c : c - 1.0f;
       }
     }
+  }
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      s_word[warp][lane * V + i] = word_of(A[SHARED ? 0 : i], M[SHARED ? 0 : i]);
-      s_b[warp][lane * V + i] = B[i];
-    }
-    if (lane == 0) {
-      s_reset[warp] = m_begin != 0;
-      s_need[warp] = (m_inside & ((m_begin & -m_begin) - 1u)) != 0;  // rows in front of the first begin; all without one
-    }
-    __syncthreads();
+  for (int i = 0; i < V; ++i) {
+    s_word[warp][lane * V + i] = word_of(A[SHARED ? 0 : i], M[SHARED ? 0 : i]);
+    s_b[warp][lane * V + i] = B[i];
+  }
+  if (lane == 0) {
+    s_reset[warp] = m_begin != 0;
+    s_need[warp] = (m_inside & ((m_begin & -m_begin) - 1u)) != 0;  // rows in front of the first begin; all without one
+  }
+  __syncthreads();
 
-    // ---- the states in front of the warps' stretches -------------------------------------------------------
-    if (threadIdx.x < WIDTH) {
-      // the whole tile's map; behind a begin only B counts
-      bool reset = false, need = false;
-      float ta = 1.0f, tm = 0.0f, tb = 0.0f;
+  // ---- the states in front of the warps' stretches --------------------------------------------------------------
+  if (threadIdx.x < WIDTH) {
+    // the whole tile's map; behind a begin only B counts
+    bool reset = false, need = false;
+    float ta = 1.0f, tm = 0.0f, tb = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const unsigned word = s_word[w][threadIdx.x];
-        const float v = __uint_as_float(word), b = s_b[w][threadIdx.x];
-        const float wa = (word & 1u) ? 1.0f + v : v, wm = (word & 1u) ? v : v - 1.0f;
-        need = need || (!reset && s_need[w]);
-        reset = reset || s_reset[w];
-        tb = s_reset[w] ? b : apply(word, tb, b);
-        ta *= wa;
-        tm = fmaf(tm, wa, wm);
+    for (int w = 0; w < kWarps; ++w) {
+      const unsigned word = s_word[w][threadIdx.x];
+      const float v = __uint_as_float(word), b = s_b[w][threadIdx.x];
+      const float wa = (word & 1u) ? 1.0f + v : v, wm = (word & 1u) ? v : v - 1.0f;
+      need = need || (!reset && s_need[w]);
+      reset = reset || s_reset[w];
+      tb = s_reset[w] ? b : apply(word, tb, b);
+      ta *= wa;
+      tm = fmaf(tm, wa, wm);
+    }
+    float h = 0.0f;
+    if (p.tiles > 1) {
+      const uint64_t to = (uint64_t)id * WIDTH + threadIdx.x, step = (uint64_t)p.chains * p.blocks * WIDTH;
+      const unsigned word = word_of(ta, tm);
+      const bool last_tile = tile + 1 == p.tiles;
+      if (!last_tile) {
+        if (reset || tile == 0) st_relaxed_u32(p.states + to, state_bits(tb));
+        else st_relaxed_u64(p.maps + to, map_bits(word, tb));
       }
-      float h = 0.0f;
-      if (p.tiles > 1) {
-        const uint64_t at = (uint64_t)id * WIDTH + threadIdx.x, step = (uint64_t)p.chains * p.blocks * WIDTH;
-        const unsigned word = word_of(ta, tm);
-        const bool last_tile = tile + 1 == p.tiles;
-        if (!last_tile) {
-          if (reset || tile == 0) st_relaxed_u32(p.states + at, state_bits(tb));
-          else st_relaxed_u64(p.maps + at, map_bits(word, tb));
-        }
-        if (need && tile > 0) {
-          h = state_in_front(p.maps + at, p.states + at, step, tile, &p.hdr->status);
-          if (!reset && !last_tile) st_relaxed_u32(p.states + at, state_bits(apply(word, h, tb)));
-        } else if (!need && !reset && tile > 0 && !last_tile) {
-          // no row of the tile belongs to a sequence: nobody behind it needs a state before a sequence begins
-          st_relaxed_u32(p.states + at, state_bits(0.0f));
-        }
-      }
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        s_carry[w][threadIdx.x] = h;
-        h = s_reset[w] ? s_b[w][threadIdx.x] : apply(s_word[w][threadIdx.x], h, s_b[w][threadIdx.x]);
+      if (need && tile > 0) {
+        h = state_in_front(p.maps + to, p.states + to, step, tile, &p.hdr->status);
+        if (!reset && !last_tile) st_relaxed_u32(p.states + to, state_bits(apply(word, h, tb)));
+      } else if (!need && !reset && tile > 0 && !last_tile) {
+        // no row of the tile belongs to a sequence: nobody behind it needs a state before a sequence begins
+        st_relaxed_u32(p.states + to, state_bits(0.0f));
       }
     }
-    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      s_carry[w][threadIdx.x] = h;
+      h = s_reset[w] ? s_b[w][threadIdx.x] : apply(s_word[w][threadIdx.x], h, s_b[w][threadIdx.x]);
+    }
+  }
+  __syncthreads();
 
-    // ---- second pass: outputs ----------------------------------------------------------------------------
-    float h[V];
+  // ---- second pass: outputs ----------------------------------------------------------------------------------
+  float h[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) h[i] = s_carry[warp][lane * V + i];
+  for (int i = 0; i < V; ++i) h[i] = s_carry[warp][lane * V + i];
+  int64_t eo = at(p.out, ch), ed = BACK ? at(p.dgate, gate_at) : 0;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      if (!(m_valid >> r & 1)) continue;
-      const uint64_t rb = __shfl_sync(0xffffffffu, b, r), rt = __shfl_sync(0xffffffffu, t, r);
-      const bool in = m_inside >> r & 1;
-      if (!in && !p.fill) continue;
-      const bool begin = m_begin >> r & 1;
-      const int s = __shfl_sync(0xffffffffu, seq, r);
+  for (int r = 0; r < R; ++r) {
+    const bool in = plain_rows || (m_inside >> r & 1);
+    if (in || (p.fill && r < n)) {
+      const bool begin = !plain_rows && (m_begin >> r & 1);
+      const bool end = !plain_rows && (m_end >> r & 1);
       if (begin) {
         if (p.first) {
           first_state(r, h);
@@ -393,25 +409,19 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_kernel(RecArgs p) {
           for (int i = 0; i < V; ++i) h[i] = 0.0f;
         }
       }
+      const int s = plain_rows ? 0 : __shfl_sync(0xffffffffu, seq, r);
       float out[V], dg[V];
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float cc = c[r][SHARED ? 0 : i];
-        const bool near = held_near(cc, logg);
-        const float xv = to_f32<T>(x[r].v[i]);
+        const float xv = to_f32<T>(x[r].v[i]), ai = a[r][SHARED ? 0 : i];
         if constexpr (BACK) {
-          const float g = xv + h[i];
-          h[i] = advance(cc, near, g, 0.0f);
-          out[i] = g;
-          float prev = 0.0f;
-          if (m_first >> r & 1) {
-            if (p.initial && live) prev = p.initial[(uint64_t)s * p.channels + ch + i];
-          } else if (rt > 0) {
-            prev = to_f32<T>(yprev[r].v[i]);
-          }
-          dg[i] = (logg ? h[i] : g) * prev;
+          float prev = to_f32<T>(before[r].v[i]);
+          if (end) prev = p.initial && live ? p.initial[(uint64_t)s * p.channels + ch + i] : 0.0f;
+          out[i] = xv + h[i];
+          h[i] = ai * out[i];
+          dg[i] = (logg ? h[i] : out[i]) * prev;
         } else {
-          h[i] = begin && !p.first ? xv : advance(cc, near, h[i], xv);
+          h[i] = begin && !p.first ? xv : fmaf(ai, h[i], xv);
           out[i] = h[i];
         }
       }
@@ -419,10 +429,10 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_kernel(RecArgs p) {
 #pragma unroll
         for (int i = 0; i < V; ++i) out[i] = dg[i] = 0.0f;
       }
-      if (live) store_floats<T, V>(p.out.data, rb * p.out.seq + rt * p.out.row + ch, out);
+      if (live) store_floats<T, V>(p.out.data, eo, out);
       if constexpr (BACK) {
         if constexpr (!SHARED) {
-          if (live) store_floats<G, V>(p.dgate.data, rb * p.dgate.seq + rt * p.dgate.row + ch, dg);
+          if (live) store_floats<G, V>(p.dgate.data, ed, dg);
         } else {
           // the head's lanes are neighbours; the first of them gathers the sum
           float sum = 0.0f;
@@ -430,27 +440,29 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_kernel(RecArgs p) {
           for (int i = 0; i < V; ++i) sum += dg[i];
           if (!live) sum = 0.0f;
           const uint32_t per = p.parts == 1 ? p.head_size / V : kWarp;
-          const uint32_t at = lane % per;
+          const uint32_t place = lane % per;
           for (uint32_t off = 1; off < per; off *= 2) {
             const float other = __shfl_down_sync(0xffffffffu, sum, off);
-            if (at + off < per) sum += other;
+            if (place + off < per) sum += other;
           }
-          if (live && at == 0) {
+          if (live && place == 0) {
             if (p.parts == 1) {
               const float one[1] = {sum};
-              store_floats<G, 1>(p.dgate.data, rb * p.dgate.seq + rt * p.dgate.row + head, one);
+              store_floats<G, 1>(p.dgate.data, ed, one);
             } else {
-              const uint64_t flat = rb * (p.chain_is_sequence || !p.offsets ? p.length : 0) + rt;
+              const uint64_t flat = chain * p.chain_rows + (uint64_t)(row - r);
               p.partial[(flat * p.heads + head) * p.parts + block % p.parts] = sum;
             }
           }
         }
       }
-      if (in && (m_end >> r & 1) && p.last && live) {
+      if (in && end && p.last && live) {
 #pragma unroll
         for (int i = 0; i < V; ++i) p.last[(uint64_t)s * p.channels + ch + i] = h[i];
       }
     }
+    eo += next(p.out);
+    if constexpr (BACK) ed += next(p.dgate);
   }
 }
 
@@ -549,8 +561,16 @@ int launch(Call& k, cudaStream_t stream) {
   return g == TB200_F32 ? launch_typed<__half, float, BACK>(k, stream) : launch_typed<__half, __half, BACK>(k, stream);
 }
 
-// The checks that both directions share. *go is set where there are rows to work on.
-int prepare(void* d_temp, size_t* temp_bytes, const tb200_recurrence_shape* shape, bool back, Call& k) {
+// Whether the sequences of all arrays lie directly behind one another. A size query names no arrays: it has to be
+// answered for those that need the most scratch.
+bool dense(const tb200_recurrence_shape* s, std::initializer_list<const tb200_rows*> arrays) {
+  for (const tb200_rows* r : arrays)
+    if (s && r && s->sequences > 1 && r->sequence_stride != s->rows * r->row_stride) return false;
+  return true;
+}
+
+// The checks that both directions share.
+int prepare(void* d_temp, size_t* temp_bytes, const tb200_recurrence_shape* shape, bool back, bool dense, Call& k) {
   if (temp_bytes == nullptr || shape == nullptr) return TB200_ERR_INVALID_ARGUMENT;
   const tb200_recurrence_shape& s = *shape;
   if (model_bytes(s.dtype) == 0 || (s.gate_dtype != s.dtype && s.gate_dtype != TB200_F32)) return TB200_ERR_UNSUPPORTED;
@@ -559,7 +579,6 @@ int prepare(void* d_temp, size_t* temp_bytes, const tb200_recurrence_shape* shap
   if (s.channels > (1u << 24) || s.sequences > 0x7fffffffull || s.rows > (1ull << 40)) return TB200_ERR_UNSUPPORTED;
   k.shape = s;
   k.rows = s.offset_bytes ? s.rows : s.sequences * s.rows;
-  const uint64_t head_size = s.channels / s.heads;
   RecArgs& p = k.args;
   p = RecArgs{};
   p.offset_bytes = s.offset_bytes;
@@ -570,9 +589,10 @@ int prepare(void* d_temp, size_t* temp_bytes, const tb200_recurrence_shape* shap
   p.channels = (uint32_t)s.channels;
   p.heads = (uint32_t)s.heads;
   p.head_size = (uint32_t)(s.channels / s.heads);
-  // Sequences of equal length are chains of their own, unless they are so short that their tiles would be mostly empty:
-  // then all of them are one chain, as packed ones are.
-  p.chain_is_sequence = s.offset_bytes == 0 && s.rows > kTileRows / 2;
+  // Sequences of equal length are chains of their own, unless they are so short that their tiles would be mostly empty
+  // and lie behind one another (strides, which a size query does not see): then all of them are one chain, as packed
+  // ones are.
+  p.chain_is_sequence = s.offset_bytes == 0 && (s.rows > kTileRows / 2 || !dense);
   p.chains = p.chain_is_sequence ? (uint32_t)s.sequences : 1;
   p.chain_rows = p.chain_is_sequence ? s.rows : k.rows;
   p.tiles = (p.chain_rows + kTileRows - 1) / kTileRows;
@@ -622,7 +642,7 @@ extern "C" int tb200_linear_recurrence(void* d_temp, size_t* temp_bytes, const t
                                        tb200_stream_t stream) {
   using namespace tb200;
   Call k{};
-  const int rc = prepare(d_temp, temp_bytes, shape, false, k);
+  const int rc = prepare(d_temp, temp_bytes, shape, false, dense(shape, {gate, x, y}), k);
   if (rc || d_temp == nullptr) return rc;
   const bool packed = k.shape.offset_bytes != 0;
   if (packed && (!d_offsets || reinterpret_cast<uintptr_t>(d_offsets) % k.shape.offset_bytes)) return TB200_ERR_INVALID_ARGUMENT;
@@ -651,7 +671,7 @@ extern "C" int tb200_linear_recurrence_backward(void* d_temp, size_t* temp_bytes
                                                 tb200_stream_t stream) {
   using namespace tb200;
   Call k{};
-  const int rc = prepare(d_temp, temp_bytes, shape, true, k);
+  const int rc = prepare(d_temp, temp_bytes, shape, true, dense(shape, {gate, y, dy, dx, dgate}), k);
   if (rc || d_temp == nullptr) return rc;
   const bool packed = k.shape.offset_bytes != 0;
   if (packed && (!d_offsets || reinterpret_cast<uintptr_t>(d_offsets) % k.shape.offset_bytes)) return TB200_ERR_INVALID_ARGUMENT;
