@@ -19,6 +19,7 @@
 
 #include <cstdint>
 #include <initializer_list>
+#include <type_traits>
 
 #include "model_common.cuh"
 
@@ -27,6 +28,16 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * kWarp;
+
+struct Divisor {  // n / d for n below 2^31, by a multiplication
+  uint32_t factor, shift;
+  __device__ __forceinline__ uint32_t of(uint32_t n) const { return (__umulhi(factor, n) + n) >> shift; }
+};
+Divisor divisor(uint32_t d) {
+  uint32_t shift = 0;
+  while ((1ull << shift) < d) ++shift;
+  return Divisor{(uint32_t)(((1ull << 32) * ((1ull << shift) - d)) / d + 1), shift};
+}
 
 struct RecArgs {
   const void* offsets;
@@ -46,10 +57,19 @@ struct RecArgs {
   float* partial;               // backward, a head over several blocks: their sums, [rows][heads][parts]
   TempHeader* hdr;
   uint32_t blocks, chains;      // blocks of channels, chains
+  Divisor by_blocks, by_chains, by_head_size;
   uint64_t tiles;               // of a chain
   unsigned long long* maps;     // [tile][chain][block][channel]: what the tile does to a state (0: not there yet)
   unsigned* states;             // [tile][chain][block][channel]: the state behind the tile (0: not there yet)
 };
+
+// The gate of a row from its logarithm. Errors of it stay within a stretch of a warp's rows, so the fast exponential
+// will do (2^-22 of the value); denormal gates count as zero.
+__device__ __forceinline__ float exp_of(float g) {
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * 1.4426950408889634f));
+  return e;
+}
 
 // A of a stretch in one word: A - 1 with the lowest bit set where A >= 1/2, else A with it clear. The bit costs at
 // most one unit of the last place, of A - 1 where that is what matters.
@@ -110,10 +130,11 @@ __device__ float state_in_front(const unsigned long long* maps, const unsigned* 
   }
 }
 
-constexpr int kMaxRows = 16;  // rows of a lane, at most
-struct Marks {           // of the rows of a tile of packed sequences
-  int seq[kWarps * kMaxRows];  // sequence of a first or last row
-  unsigned char kind[kWarps * kMaxRows];  // bit 0: first row of its sequence, bit 1: last
+template <int TILE>
+struct Marks {  // of the rows of a tile of packed sequences
+  int seq[TILE];             // sequence of a first or last row
+  unsigned char kind[TILE];  // bit 0: first row of its sequence, bit 1: last
+  uint64_t from, to;         // the rows of all sequences
 };
 
 __device__ __forceinline__ uint64_t offset_at(const RecArgs& p, uint64_t i) {
@@ -123,8 +144,9 @@ __device__ __forceinline__ uint64_t offset_at(const RecArgs& p, uint64_t i) {
 }
 
 // Marks the first and last rows of sequences among rows [r0, r1), in memory order; hands the states of empty sequences
-// that lie here through for channels [c0, c0 + count). One warp does it; the others wait at the barrier behind.
-__device__ void mark_rows(const RecArgs& p, uint64_t r0, uint64_t r1, bool at_end, uint32_t c0, uint32_t count, Marks& m) {
+// that lie here through for channels [c0, c0 + count). For one warp.
+template <int TILE>
+__device__ void mark_rows(const RecArgs& p, uint64_t r0, uint64_t r1, bool at_end, uint32_t c0, uint32_t count, Marks<TILE>& m) {
   const unsigned lane = lane_id();
   for (int i = lane; i < (int)sizeof(m.kind) / 4; i += kWarp) reinterpret_cast<unsigned*>(m.kind)[i] = 0;
   __syncwarp();
@@ -158,311 +180,516 @@ __device__ void mark_rows(const RecArgs& p, uint64_t r0, uint64_t r1, bool at_en
   }
 }
 
-template <typename T, typename G, int V, bool SHARED, bool BACK, int R>
-__global__ void __launch_bounds__(kThreads, 2) recurrence_kernel(RecArgs p) {
-  constexpr int WIDTH = kWarp * V;
-  constexpr int GV = SHARED ? 1 : V;  // gates of a lane in a row
-  constexpr int TILE = kWarps * R;
-  constexpr unsigned ALL = (unsigned)((1ull << R) - 1);
-  static_assert(R <= kMaxRows, "marks are sized for this");
-  __shared__ Marks s_marks;
-  __shared__ unsigned s_word[kWarps][WIDTH];
-  __shared__ float s_b[kWarps][WIDTH];
-  __shared__ float s_carry[kWarps][WIDTH];
-  __shared__ int s_reset[kWarps];  // a sequence begins among the warp's rows
-  __shared__ int s_need[kWarps];   // the warp has rows in front of that
-  __shared__ unsigned s_ticket;
+// Asynchronous copies of a lane's own channels into its own place in shared memory: no barrier, only the lane's wait.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(to)), "l"(from), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 
+// What a thread works on in one tile.
+struct Place {
+  uint32_t block, chain, c0, count;  // the block's channels
+  uint32_t ch, head;                 // the lane's first channel, its head
+  bool live;
+  uint32_t tile;
+  int n;        // how many of the warp's rows exist
+  int64_t row;  // the first of them in memory; the others follow with the recurrence (below zero only where n is 0)
+};
+template <int V, bool SHARED, bool BACK, int R>
+__device__ __forceinline__ Place place_of(const RecArgs& p, unsigned id) {
+  constexpr uint32_t WIDTH = kWarp * V;
+  Place w;
+  const unsigned rest = p.by_blocks.of(id);
+  w.block = id - rest * p.blocks;
+  w.tile = p.by_chains.of(rest);
+  w.chain = rest - w.tile * p.chains;
+  if (!SHARED) {
+    w.c0 = w.block * WIDTH;
+    w.count = min(WIDTH, p.channels - w.c0);
+  } else if (p.parts == 1) {
+    const uint32_t h0 = w.block * p.block_heads;
+    w.c0 = h0 * p.head_size;
+    w.count = min(p.block_heads, p.heads - h0) * p.head_size;
+  } else {
+    const uint32_t h0 = w.block / p.parts, part = w.block % p.parts;
+    w.c0 = h0 * p.head_size + part * WIDTH;
+    w.count = min(WIDTH, p.head_size - part * WIDTH);
+  }
+  const unsigned lane = lane_id();
+  w.ch = w.c0 + lane * V;
+  w.live = lane * V < w.count;
+  w.head = SHARED ? p.by_head_size.of(w.ch) : 0;
+  const uint64_t q = (uint64_t)w.tile * (kWarps * R) + threadIdx.x / kWarp * R;
+  w.n = q >= p.chain_rows ? 0 : p.chain_rows - q < R ? (int)(p.chain_rows - q) : R;
+  w.row = BACK ? (int64_t)p.chain_rows - 1 - (int64_t)q : (int64_t)q;
+  return w;
+}
+// Which of the warp's rows are what: bit r of a mask is row r.
+struct RowKinds {
+  unsigned inside, begin, end;  // rows of a sequence; its first and last one with the recurrence
+  int seq;                      // lane r: the sequence of row r, where that is a first or last one
+  // nothing but rows of one sequence
+  __device__ __forceinline__ bool plain(unsigned all) const { return inside == all && (begin | end) == 0; }
+};
+template <int TILE, int V, bool SHARED, bool BACK, int R>
+__device__ void marks_of_tile(const RecArgs& p, unsigned id, bool mine, Marks<TILE>& m) {
+  if (!mine) return;  // one warp
+  const Place w = place_of<V, SHARED, BACK, R>(p, id);
+  const uint64_t lo = (uint64_t)w.tile * TILE, hi = min(lo + TILE, p.chain_rows);
+  const uint64_t r0 = BACK ? p.chain_rows - hi : lo, r1 = BACK ? p.chain_rows - lo : hi;
+  mark_rows(p, r0, r1, r1 == p.chain_rows, w.c0, w.count, m);
+  if (lane_id() == 0) {
+    m.from = offset_at(p, 0);
+    m.to = offset_at(p, p.sequences);
+  }
+}
+
+// Bytes of shared memory that tiles may take, beside the joins and marks.
+constexpr int kStageBudget = 200 << 10;
+// Rows of a lane: eight, or four where eight rows of everything would leave room for less than three tiles.
+constexpr int rows_of_lane(int bytes_of_row) { return 3 * 8 * bytes_of_row * kThreads <= kStageBudget ? 8 : 4; }
+
+template <typename T, typename G, int V, bool SHARED, bool BACK>
+struct Shape {
+  static constexpr int GV = SHARED ? 1 : V;  // gates of a lane in a row
+  static constexpr int ROW = (int)(sizeof(Pack<T, V>) * (BACK ? 2 : 1) + sizeof(Pack<G, GV>));
+  static constexpr int R = rows_of_lane(ROW);
+  // what takes 4 bytes and more is copied asynchronously, the rest goes through registers
+  static constexpr bool X_ASYNC = sizeof(Pack<T, V>) >= 4, G_ASYNC = sizeof(Pack<G, GV>) >= 4;
+  static constexpr int kX = R * kThreads * (int)sizeof(Pack<T, V>);
+  static constexpr int kStage = R * kThreads * ROW;
+  static constexpr int STAGES = kStageBudget / kStage >= 4 ? 4 : 3;
+  static constexpr int kJoin = kWarps * kWarp * V * 4;
+  static constexpr size_t kBytes = (size_t)STAGES * kStage + 4 * kJoin;
+  static_assert(STAGES * kStage <= kStageBudget, "a tile on its way, a landed one and a parked one");
+};
+
+// Barriers between the warps that compute and the warps that join, by the parity of the tile.
+enum : int { kMapsReady = 1, kStatesReady = 3, kJoined = 5 };
+__device__ __forceinline__ void barrier_arrive(int id, int count) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(count) : "memory");
+}
+
+// One CTA on an SM, which takes tile after tile. Eight warps compute: the first pass over a tile as soon as its rows
+// have landed, the second pass over the tile in front, whose rows wait in shared memory, once the state in front of it is
+// known. One thread for each channel joins: it puts the warps' stretches together, publishes the tile's map, and finds
+// the state in front of the tile before, all while the others compute. Every thread copies the rows that it computes
+// itself, so their arrival needs no barrier.
+template <typename T, typename G, int V, bool SHARED, bool BACK>
+__global__ void __launch_bounds__(kThreads + kWarp * V, 1) recurrence_kernel(RecArgs p) {
+  using S = Shape<T, G, V, SHARED, BACK>;
+  constexpr int WIDTH = kWarp * V, GV = S::GV, R = S::R, TILE = kWarps * R, STAGES = S::STAGES;
+  constexpr int CTA = kThreads + WIDTH;
+  constexpr unsigned ALL = (1u << R) - 1;
+  extern __shared__ __align__(16) char s_dynamic[];
+  __shared__ Marks<TILE> s_marks[2];
+  __shared__ int s_reset[2][kWarps];  // a sequence begins among the warp's rows
+  __shared__ int s_need[2][kWarps];   // the warp has rows in front of that
+  __shared__ unsigned s_ids[8];       // of the CTA's tiles, a ring
+  auto* s_word = reinterpret_cast<unsigned(*)[kWarps][WIDTH]>(s_dynamic + STAGES * S::kStage);
+  auto* s_b = reinterpret_cast<float(*)[kWarps][WIDTH]>(s_dynamic + STAGES * S::kStage + 2 * S::kJoin);
+
+  // Tiles are handed out in the order of the recurrence, all chains and blocks of channels of one stretch of rows before
+  // the next: whatever a tile waits for is worked on by a CTA that runs already, and a tile's map never waits for more
+  // than the tiles in front of it in its own CTA.
+  const bool chained = p.tiles > 1;
+  const unsigned total = (unsigned)p.tiles * p.chains * p.blocks;
+  auto draw = [&](unsigned behind) { return chained ? atomicAdd(&p.hdr->ticket, 1u) : behind + gridDim.x; };
+
+
+  const bool joins = threadIdx.x >= kThreads;
   const unsigned lane = lane_id(), warp = threadIdx.x / kWarp;
   const bool logg = p.log_gate != 0;
 
-  // Tiles are handed out in the order of the recurrence, all chains and blocks of channels of one stretch of rows before
-  // the next: whatever a tile waits for is worked on by a CTA that runs already.
-  unsigned id = blockIdx.x;
-  if (p.tiles > 1) {
-    if (threadIdx.x == 0) s_ticket = atomicAdd(&p.hdr->ticket, 1u);
-    __syncthreads();
-    id = s_ticket;
-  } else if (id == 0) {  // the scratch is not cleared where no tile waits for another
-    if (threadIdx.x == 0) p.hdr->status = TB200_OK;
-    __syncthreads();
-  }
-  const uint32_t block = id % p.blocks;
-  const uint32_t chain = id / p.blocks % p.chains;
-  const uint64_t tile = id / p.blocks / p.chains;
-
-  // the block's channels
-  uint32_t c0, count;
-  if (!SHARED) {
-    c0 = block * WIDTH;
-    count = min((uint32_t)WIDTH, p.channels - c0);
-  } else if (p.parts == 1) {
-    const uint32_t h0 = block * p.block_heads;
-    c0 = h0 * p.head_size;
-    count = min(p.block_heads, p.heads - h0) * p.head_size;
-  } else {
-    const uint32_t h0 = block / p.parts, part = block % p.parts;
-    c0 = h0 * p.head_size + part * WIDTH;
-    count = min((uint32_t)WIDTH, p.head_size - part * WIDTH);
-  }
-  const uint32_t ch = c0 + lane * V;
-  const bool live = lane * V < count;
-  const uint32_t head = SHARED ? ch / p.head_size : 0;
-  const uint32_t gate_at = SHARED ? head : ch;
-
-  // ---- load: the warp's rows run from `row` with the recurrence, `n` of them exist ----------------------
-  const uint64_t q = tile * TILE + warp * R;
-  const int n = q >= p.chain_rows ? 0 : p.chain_rows - q < R ? (int)(p.chain_rows - q) : R;
-  const int64_t row = BACK ? (int64_t)p.chain_rows - 1 - (int64_t)q : (int64_t)q;  // below zero only where n is 0
-  auto at = [&](const RowsOf& a, uint32_t column) { return (int64_t)(chain * a.seq + column) + row * (int64_t)a.row; };
+  // the thread's place for row r of a stage: [r * kThreads]
+  auto stage_x = [&](int k) { return reinterpret_cast<Pack<T, V>*>(s_dynamic + k * S::kStage) + threadIdx.x; };
+  auto stage_y = [&](int k) { return reinterpret_cast<Pack<T, V>*>(s_dynamic + k * S::kStage + S::kX) + threadIdx.x; };
+  auto stage_g = [&](int k) {
+    return reinterpret_cast<Pack<G, GV>*>(s_dynamic + k * S::kStage + S::kX * (BACK ? 2 : 1)) + threadIdx.x;
+  };
+  auto at = [&](const Place& w, const RowsOf& a, uint32_t column) {
+    return (int64_t)(w.chain * a.seq + column) + w.row * (int64_t)a.row;
+  };
   auto next = [](const RowsOf& a) { return BACK ? -(int64_t)a.row : (int64_t)a.row; };
 
-  Pack<G, GV> gate[R];
-  Pack<T, V> x[R];
-  Pack<T, V> before[BACK ? R : 1];  // y of the row in front, in memory
-  {
-    int64_t eg = at(p.gate, gate_at), ex = at(p.in, ch), ey = BACK ? at(p.y, ch) - (int64_t)p.y.row : 0;
+  // Brings a tile's rows on their way to a stage. What is copied through registers gets there with `settle`.
+  struct Late {
+    Pack<G, GV> gate[S::G_ASYNC ? 1 : R];
+    Pack<T, V> x[S::X_ASYNC ? 1 : R];
+    Pack<T, V> before[S::X_ASYNC || !BACK ? 1 : R];
+  } late;
+  auto fetch = [&](unsigned id, int k) {
+    const Place w = place_of<V, SHARED, BACK, R>(p, id);
+    if (!w.live) return;
+    const char* g = p.gate.data + at(w, p.gate, SHARED ? w.head : w.ch) * (int64_t)sizeof(G);
+    const char* x = p.in.data + at(w, p.in, w.ch) * (int64_t)sizeof(T);
+    const char* y = BACK ? p.y.data + (at(w, p.y, w.ch) - (int64_t)p.y.row) * (int64_t)sizeof(T) : nullptr;
+    const int64_t dg = next(p.gate) * (int64_t)sizeof(G), dx = next(p.in) * (int64_t)sizeof(T);
+    const int64_t dy = BACK ? next(p.y) * (int64_t)sizeof(T) : 0;
+    auto rows = [&](auto all) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        if (all || r < w.n) {
+          if constexpr (S::G_ASYNC) copy_async<sizeof(Pack<G, GV>)>(stage_g(k) + r * kThreads, g);
+          else late.gate[r] = load_pack<G, GV>(g, 0);
+          if constexpr (S::X_ASYNC) copy_async<sizeof(Pack<T, V>)>(stage_x(k) + r * kThreads, x);
+          else late.x[r] = load_pack<T, V>(x, 0);
+          if constexpr (BACK) {
+            if (all || w.row - r > 0) {
+              if constexpr (S::X_ASYNC) copy_async<sizeof(Pack<T, V>)>(stage_y(k) + r * kThreads, y);
+              else late.before[r] = load_pack<T, V>(y, 0);
+            }
+          }
+        }
+        g += dg;
+        x += dx;
+        if constexpr (BACK) y += dy;
+      }
+    };
+    if (w.n == R && (!BACK || w.row >= R)) rows(std::true_type{}); else rows(std::false_type{});
+  };
+  auto settle = [&](int k) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      if (live && r < n) {
-        gate[r] = load_pack<G, GV>(p.gate.data, eg);
-        x[r] = load_pack<T, V>(p.in.data, ex);
-        if constexpr (BACK)
-          if (row - r > 0) before[r] = load_pack<T, V>(p.y.data, ey);
+      if constexpr (!S::G_ASYNC) stage_g(k)[r * kThreads] = late.gate[r];
+      if constexpr (!S::X_ASYNC) {
+        stage_x(k)[r * kThreads] = late.x[r];
+        if constexpr (BACK) stage_y(k)[r * kThreads] = late.before[r];
       }
-      eg += next(p.gate);
-      ex += next(p.in);
-      if constexpr (BACK) ey += next(p.y);
     }
-  }
+  };
 
-  // ---- first and last rows of sequences: bit r of a mask is the warp's row r ------------------------------
-  unsigned m_inside = (unsigned)((1ull << n) - 1), m_first = 0, m_last = 0;
-  int seq = chain;  // of row `lane`, where that is a first or last one
-  if (p.offsets != nullptr) {
-    if (id == 0) {  // bad offsets are reported, and cannot lead outside the arrays
+  // two tiles to begin with, drawn one by one: a burst would hand neighbouring tiles to one CTA
+  if (threadIdx.x == kThreads) s_ids[0] = chained ? draw(0) : blockIdx.x;
+  __syncthreads();
+  const unsigned id0 = s_ids[0];
+  if (id0 >= total) return;
+  if (!joins) {
+    fetch(id0, 0);
+    copies_issued();
+    settle(0);
+  } else {
+    if (threadIdx.x == kThreads) {
+      s_ids[1] = draw(id0);
+      if (!chained && blockIdx.x == 0) p.hdr->status = TB200_OK;  // scratch that no tile waits in is not cleared
+    }
+    if (p.offsets) marks_of_tile<TILE, V, SHARED, BACK, R>(p, id0, threadIdx.x - kThreads < kWarp, s_marks[0]);
+  }
+  __syncthreads();
+
+  if (joins) {
+    // ================================ the threads that join: one for each channel ==============================
+    const unsigned c = threadIdx.x - kThreads;
+    const uint64_t step = (uint64_t)p.chains * p.blocks * WIDTH;
+    if (p.offsets != nullptr && id0 == 0) {  // bad offsets are reported, and cannot lead outside the arrays
       bool bad = false;
-      for (uint64_t i = threadIdx.x; i <= p.sequences; i += kThreads) {
+      for (uint64_t i = c; i <= p.sequences; i += WIDTH) {
         const int64_t v = p.offset_bytes == 4 ? (int64_t)static_cast<const int32_t*>(p.offsets)[i]
                                               : static_cast<const int64_t*>(p.offsets)[i];
         bad = bad || v < 0 || (uint64_t)v > p.length || (i == 0 ? v != 0 : (uint64_t)v < offset_at(p, i - 1));
       }
       if (bad) atomicExch(&p.hdr->status, (int)TB200_ERR_INVALID_ARGUMENT);
     }
-    const uint64_t lo = tile * TILE, hi = min(lo + TILE, p.chain_rows);
-    const uint64_t r0 = BACK ? p.chain_rows - hi : lo, r1 = BACK ? p.chain_rows - lo : hi;
-    if (warp == 0) mark_rows(p, r0, r1, r1 == p.chain_rows, c0, count, s_marks);
-    __syncthreads();
-    const uint64_t mine = (uint64_t)(BACK ? row - (int)lane : row + (int)lane);
-    const bool valid = (int)lane < n;
-    const unsigned kind = valid ? s_marks.kind[mine - r0] : 0;
-    if (kind) seq = s_marks.seq[mine - r0];
-    m_first = __ballot_sync(0xffffffffu, kind & 1);
-    m_last = __ballot_sync(0xffffffffu, kind & 2);
-    m_inside = __ballot_sync(0xffffffffu, valid && mine >= offset_at(p, 0) && mine < offset_at(p, p.sequences));
-  } else if (p.chain_is_sequence) {
-    if (n > 0) {
-      const unsigned low = q == 0 ? 1u : 0u, high = q + n == p.chain_rows ? 1u << (n - 1) : 0u;
-      m_first = BACK ? high : low;
-      m_last = BACK ? low : high;
-    }
-  } else if (n > 0) {  // sequences of equal length behind one another
-    const uint64_t mine = (uint64_t)(BACK ? row - (int)min((int)lane, n - 1) : row + (int)min((int)lane, n - 1));
-    const uint64_t s = p.chain_rows >> 32 ? mine / p.length : (uint32_t)mine / (uint32_t)p.length;
-    const uint64_t t = mine - s * p.length;
-    seq = (int)s;
-    m_first = __ballot_sync(0xffffffffu, (int)lane < n && t == 0);
-    m_last = __ballot_sync(0xffffffffu, (int)lane < n && t == p.length - 1);
-  }
-  const unsigned m_begin = BACK ? m_last : m_first, m_end = BACK ? m_first : m_last;  // with the recurrence
-  const bool plain_rows = m_inside == ALL && (m_begin | m_end) == 0;  // nothing but rows of one sequence
+    // of the tile in front: its own map, whether its state is to be published, whether it needs the one in front
+    unsigned p_id = 0, p_tile = 0, p_word = 0;
+    float p_b = 0.0f;
+    bool p_state = false, p_wait = false;
+    for (unsigned i = 0;; ++i) {
+      const int k = i & 1;
+      const unsigned id = s_ids[i & 7];
+      const bool some = id < total;
+      const unsigned behind = s_ids[(i + 1) & 7];
+      if (c == 0) s_ids[(i + 2) & 7] = behind < total ? draw(behind) : total;
+      if (p.offsets && behind < total) marks_of_tile<TILE, V, SHARED, BACK, R>(p, behind, c < kWarp, s_marks[k ^ 1]);
 
-  // the state that a sequence begins with
-  auto first_state = [&](int r, float (&h)[V]) {
-    const int s = __shfl_sync(0xffffffffu, seq, r);
-    const float* from = p.first + (uint64_t)s * p.channels + ch;
+      // ---- this tile's map; behind a begin only B counts --------------------------------------------------
+      bool reset = false, need = false;
+      unsigned word = 0, tile = 0;
+      float tb = 0.0f;
+      if (some) {
+        tile = p.by_chains.of(p.by_blocks.of(id));
+        named_barrier(kMapsReady + k, CTA);
+        if (chained) {
+          float ta = 1.0f, tm = 0.0f;
 #pragma unroll
-    for (int i = 0; i < V; ++i) h[i] = live ? from[i] : 0.0f;
-  };
-
-  // ---- first pass: the stretch's A and B --------------------------------------------------------------------
-  float a[R][GV];  // the gates themselves from here on
-  float A[GV], M[GV], B[V];
-  {
-    float sum[GV];
-#pragma unroll
-    for (int i = 0; i < GV; ++i) A[i] = 1.0f, M[i] = 0.0f, sum[i] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < V; ++i) B[i] = 0.0f;
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      if (!plain_rows && !(m_inside >> r & 1)) continue;
-      const bool begin = !plain_rows && (m_begin >> r & 1);
-      if (begin) {
-        if (p.first) {
-          first_state(r, B);
-        } else {
-#pragma unroll
-          for (int i = 0; i < V; ++i) B[i] = 0.0f;
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < GV; ++i) {
-        const float g = to_f32<G>(gate[r].v[i]);
-        if (logg) {
-          sum[i] += g;
-          a[r][i] = __expf(g);
-        } else {
-          A[i] *= g;
-          M[i] = fmaf(M[i], g, g - 1.0f);
-          a[r][i] = g;
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float ai = a[r][SHARED ? 0 : i], xv = to_f32<T>(x[r].v[i]);
-        if constexpr (BACK) {
-          B[i] = ai * (xv + B[i]);
-        } else {
-          B[i] = begin && !p.first ? xv : fmaf(ai, B[i], xv);
-        }
-      }
-    }
-    if (logg) {
-#pragma unroll
-      for (int i = 0; i < GV; ++i) {
-        const float c = hold_gate(sum[i], true);
-        const bool near = held_near(c, true);
-        A[i] = near ? 1.0f + c : c;
-        M[i] = near ? c : c - 1.0f;
-      }
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    s_word[warp][lane * V + i] = word_of(A[SHARED ? 0 : i], M[SHARED ? 0 : i]);
-    s_b[warp][lane * V + i] = B[i];
-  }
-  if (lane == 0) {
-    s_reset[warp] = m_begin != 0;
-    s_need[warp] = (m_inside & ((m_begin & -m_begin) - 1u)) != 0;  // rows in front of the first begin; all without one
-  }
-  __syncthreads();
-
-  // ---- the states in front of the warps' stretches --------------------------------------------------------------
-  if (threadIdx.x < WIDTH) {
-    // the whole tile's map; behind a begin only B counts
-    bool reset = false, need = false;
-    float ta = 1.0f, tm = 0.0f, tb = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const unsigned word = s_word[w][threadIdx.x];
-      const float v = __uint_as_float(word), b = s_b[w][threadIdx.x];
-      const float wa = (word & 1u) ? 1.0f + v : v, wm = (word & 1u) ? v : v - 1.0f;
-      need = need || (!reset && s_need[w]);
-      reset = reset || s_reset[w];
-      tb = s_reset[w] ? b : apply(word, tb, b);
-      ta *= wa;
-      tm = fmaf(tm, wa, wm);
-    }
-    float h = 0.0f;
-    if (p.tiles > 1) {
-      const uint64_t to = (uint64_t)id * WIDTH + threadIdx.x, step = (uint64_t)p.chains * p.blocks * WIDTH;
-      const unsigned word = word_of(ta, tm);
-      const bool last_tile = tile + 1 == p.tiles;
-      if (!last_tile) {
-        if (reset || tile == 0) st_relaxed_u32(p.states + to, state_bits(tb));
-        else st_relaxed_u64(p.maps + to, map_bits(word, tb));
-      }
-      if (need && tile > 0) {
-        h = state_in_front(p.maps + to, p.states + to, step, tile, &p.hdr->status);
-        if (!reset && !last_tile) st_relaxed_u32(p.states + to, state_bits(apply(word, h, tb)));
-      } else if (!need && !reset && tile > 0 && !last_tile) {
-        // no row of the tile belongs to a sequence: nobody behind it needs a state before a sequence begins
-        st_relaxed_u32(p.states + to, state_bits(0.0f));
-      }
-    }
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      s_carry[w][threadIdx.x] = h;
-      h = s_reset[w] ? s_b[w][threadIdx.x] : apply(s_word[w][threadIdx.x], h, s_b[w][threadIdx.x]);
-    }
-  }
-  __syncthreads();
-
-  // ---- second pass: outputs ----------------------------------------------------------------------------------
-  float h[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) h[i] = s_carry[warp][lane * V + i];
-  int64_t eo = at(p.out, ch), ed = BACK ? at(p.dgate, gate_at) : 0;
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const bool in = plain_rows || (m_inside >> r & 1);
-    if (in || (p.fill && r < n)) {
-      const bool begin = !plain_rows && (m_begin >> r & 1);
-      const bool end = !plain_rows && (m_end >> r & 1);
-      if (begin) {
-        if (p.first) {
-          first_state(r, h);
-        } else {
-#pragma unroll
-          for (int i = 0; i < V; ++i) h[i] = 0.0f;
-        }
-      }
-      const int s = plain_rows ? 0 : __shfl_sync(0xffffffffu, seq, r);
-      float out[V], dg[V];
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float xv = to_f32<T>(x[r].v[i]), ai = a[r][SHARED ? 0 : i];
-        if constexpr (BACK) {
-          float prev = to_f32<T>(before[r].v[i]);
-          if (end) prev = p.initial && live ? p.initial[(uint64_t)s * p.channels + ch + i] : 0.0f;
-          out[i] = xv + h[i];
-          h[i] = ai * out[i];
-          dg[i] = (logg ? h[i] : out[i]) * prev;
-        } else {
-          h[i] = begin && !p.first ? xv : fmaf(ai, h[i], xv);
-          out[i] = h[i];
-        }
-      }
-      if (!in) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) out[i] = dg[i] = 0.0f;
-      }
-      if (live) store_floats<T, V>(p.out.data, eo, out);
-      if constexpr (BACK) {
-        if constexpr (!SHARED) {
-          if (live) store_floats<G, V>(p.dgate.data, ed, dg);
-        } else {
-          // the head's lanes are neighbours; the first of them gathers the sum
-          float sum = 0.0f;
-#pragma unroll
-          for (int i = 0; i < V; ++i) sum += dg[i];
-          if (!live) sum = 0.0f;
-          const uint32_t per = p.parts == 1 ? p.head_size / V : kWarp;
-          const uint32_t place = lane % per;
-          for (uint32_t off = 1; off < per; off *= 2) {
-            const float other = __shfl_down_sync(0xffffffffu, sum, off);
-            if (place + off < per) sum += other;
+          for (int v = 0; v < kWarps; ++v) {
+            const unsigned wd = s_word[k][v][c];
+            const float m = __uint_as_float(wd), b = s_b[k][v][c];
+            const float wa = (wd & 1u) ? 1.0f + m : m, wm = (wd & 1u) ? m : m - 1.0f;
+            need = need || (!reset && s_need[k][v]);
+            reset = reset || s_reset[k][v];
+            tb = s_reset[k][v] ? b : apply(wd, tb, b);
+            ta *= wa;
+            tm = fmaf(tm, wa, wm);
           }
-          if (live && place == 0) {
-            if (p.parts == 1) {
-              const float one[1] = {sum};
-              store_floats<G, 1>(p.dgate.data, ed, one);
+          word = word_of(ta, tm);
+          if (tile + 1 < p.tiles) {
+            const uint64_t to = (uint64_t)id * WIDTH + c;
+            // no row of any sequence: nobody behind needs a state before a sequence begins, so any will do
+            if (reset || tile == 0 || !need) st_relaxed_u32(p.states + to, state_bits(tb));
+            else st_relaxed_u64(p.maps + to, map_bits(word, tb));
+          }
+        }
+      }
+      // ---- the states in front of the stretches of the tile before -----------------------------------------
+      if (i > 0) {
+        float h = 0.0f;
+        if (p_wait) {
+          const uint64_t to = (uint64_t)p_id * WIDTH + c;
+          h = state_in_front(p.maps + to, p.states + to, step, p_tile, &p.hdr->status);
+          if (p_state) st_relaxed_u32(p.states + to, state_bits(apply(p_word, h, p_b)));
+        }
+#pragma unroll
+        for (int v = 0; v < kWarps; ++v) {
+          const float b = s_b[k ^ 1][v][c];
+          s_b[k ^ 1][v][c] = h;
+          h = s_reset[k ^ 1][v] ? b : apply(s_word[k ^ 1][v][c], h, b);
+        }
+      }
+      barrier_arrive(kStatesReady + (k ^ 1), CTA);
+      if (!some) return;
+      p_id = id;
+      p_tile = tile;
+      p_word = word;
+      p_b = tb;
+      p_wait = need && tile > 0;
+      p_state = p_wait && !reset && tile + 1 < p.tiles;
+      __syncwarp();
+      if constexpr (WIDTH > kWarp) named_barrier(kJoined, WIDTH);  // s_ids and marks of one warp, read by all
+    }
+  }
+
+  // ==================================== the warps that compute ================================================
+  Place pw{};
+  RowKinds pk{};
+  bool parked = false, unsettled = false;
+  int stage = 0, p_stage = 0;  // of tile i, of the tile in front
+  for (unsigned i = 0;; ++i) {
+    const int k = i & 1;
+    const unsigned id = s_ids[i & 7];
+    const bool some = id < total;
+    const int s1 = stage + 1 == STAGES ? 0 : stage + 1, s2 = s1 + 1 == STAGES ? 0 : s1 + 1;
+    if (i == 0) {
+      const unsigned id1 = s_ids[1];
+      if (id1 < total) {
+        fetch(id1, s1);
+        unsettled = true;
+      }
+      copies_issued();
+    }
+    Place w{};
+    RowKinds kinds{};
+    if (some) {
+      w = place_of<V, SHARED, BACK, R>(p, id);
+      // ---- first and last rows of sequences ---------------------------------------------------------------
+      const uint64_t mine = (uint64_t)(BACK ? w.row - (int)lane : w.row + (int)lane);  // lane r: row r, if it exists
+      const bool valid = (int)lane < w.n;
+      unsigned m_first = 0, m_last = 0;
+      kinds.inside = (1u << w.n) - 1;
+      kinds.seq = w.chain;
+      if (p.offsets != nullptr) {
+        const uint64_t lo = (uint64_t)w.tile * TILE, hi = min(lo + TILE, p.chain_rows);
+        const uint64_t r0 = BACK ? p.chain_rows - hi : lo;
+        const unsigned kind = valid ? s_marks[k].kind[mine - r0] : 0;
+        if (kind & 3) kinds.seq = s_marks[k].seq[mine - r0];
+        m_first = __ballot_sync(0xffffffffu, kind & 1);
+        m_last = __ballot_sync(0xffffffffu, kind & 2);
+        kinds.inside = __ballot_sync(0xffffffffu, valid && mine >= s_marks[k].from && mine < s_marks[k].to);
+      } else if (p.chain_is_sequence) {
+        m_first = __ballot_sync(0xffffffffu, valid && mine == 0);
+        m_last = __ballot_sync(0xffffffffu, valid && mine == p.chain_rows - 1);
+      } else {  // sequences of equal length behind one another
+        const uint64_t m = valid ? mine : 0;
+        const uint64_t s = p.chain_rows >> 32 ? m / p.length : (uint32_t)m / (uint32_t)p.length;
+        const uint64_t t = m - s * p.length;
+        kinds.seq = (int)s;
+        m_first = __ballot_sync(0xffffffffu, valid && t == 0);
+        m_last = __ballot_sync(0xffffffffu, valid && t == p.length - 1);
+      }
+      kinds.begin = BACK ? m_last : m_first;
+      kinds.end = BACK ? m_first : m_last;
+
+      // ---- first pass: the stretch's A and B ----------------------------------------------------------------
+      asm volatile("cp.async.wait_group 1;" ::: "memory");  // all but the copies of the tile behind
+      float A[GV], M[GV], B[V], sum[GV];
+#pragma unroll
+      for (int e = 0; e < GV; ++e) A[e] = 1.0f, M[e] = 0.0f, sum[e] = 0.0f;
+#pragma unroll
+      for (int e = 0; e < V; ++e) B[e] = 0.0f;
+      auto first_pass = [&](auto plain, auto log_gate) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          if (!plain && !(kinds.inside >> r & 1)) continue;
+          const bool begin = !plain && (kinds.begin >> r & 1);
+          if (begin) {
+            const int s = __shfl_sync(0xffffffffu, kinds.seq, r);
+#pragma unroll
+            for (int e = 0; e < V; ++e) B[e] = p.first && w.live ? p.first[(uint64_t)s * p.channels + w.ch + e] : 0.0f;
+          }
+          const Pack<G, GV> gate = stage_g(stage)[r * kThreads];
+          const Pack<T, V> x = stage_x(stage)[r * kThreads];
+          float a[GV];
+#pragma unroll
+          for (int e = 0; e < GV; ++e) {
+            const float g = to_f32<G>(gate.v[e]);
+            if (log_gate) {
+              sum[e] += g;
+              a[e] = exp_of(g);
             } else {
-              const uint64_t flat = chain * p.chain_rows + (uint64_t)(row - r);
-              p.partial[(flat * p.heads + head) * p.parts + block % p.parts] = sum;
+              A[e] *= g;
+              M[e] = fmaf(M[e], g, g - 1.0f);
+              a[e] = g;
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float ai = a[SHARED ? 0 : e], xv = to_f32<T>(x.v[e]);
+            if constexpr (BACK) {
+              B[e] = ai * (xv + B[e]);
+            } else {
+              B[e] = begin && !p.first ? xv : fmaf(ai, B[e], xv);
             }
           }
         }
+      };
+      if (kinds.plain(ALL)) {
+        if (logg) first_pass(std::true_type{}, std::true_type{}); else first_pass(std::true_type{}, std::false_type{});
+      } else {
+        first_pass(std::false_type{}, logg);
       }
-      if (in && end && p.last && live) {
+      if (logg) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) p.last[(uint64_t)s * p.channels + ch + i] = h[i];
+        for (int e = 0; e < GV; ++e) {
+          const float c = hold_gate(sum[e], true);
+          const bool near = held_near(c, true);
+          A[e] = near ? 1.0f + c : c;
+          M[e] = near ? c : c - 1.0f;
+        }
+      }
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        s_word[k][warp][lane * V + v] = word_of(A[SHARED ? 0 : v], M[SHARED ? 0 : v]);
+        s_b[k][warp][lane * V + v] = B[v];
+      }
+      if (lane == 0) {
+        s_reset[k][warp] = kinds.begin != 0;
+        // rows in front of the first begin; all of them without one
+        s_need[k][warp] = (kinds.inside & ((kinds.begin & -kinds.begin) - 1u)) != 0;
+      }
+      barrier_arrive(kMapsReady + k, CTA);
+    }
+    if (unsettled) settle(s1);  // what was fetched a step ago, for the tile behind this one
+    unsettled = false;
+
+    named_barrier(kStatesReady + (k ^ 1), CTA);
+    auto fetch_two_ahead = [&] {
+      const unsigned id2 = s_ids[(i + 2) & 7];
+      if (id2 < total) {
+        fetch(id2, s2);
+        unsettled = true;
+      }
+      copies_issued();
+    };
+    if constexpr (STAGES > 3) fetch_two_ahead();  // into the stage that the tile before the parked one has left
+
+    // ---- second pass: the parked tile's outputs ---------------------------------------------------------------
+    if (parked) {
+      float h[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) h[e] = s_b[k ^ 1][warp][lane * V + e];
+      char* to = p.out.data + at(pw, p.out, pw.ch) * (int64_t)sizeof(T);
+      char* to_g = BACK ? p.dgate.data + at(pw, p.dgate, SHARED ? pw.head : pw.ch) * (int64_t)sizeof(G) : nullptr;
+      const int64_t d_out = next(p.out) * (int64_t)sizeof(T), d_g = BACK ? next(p.dgate) * (int64_t)sizeof(G) : 0;
+      auto second_pass = [&](auto plain, auto log_gate) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const bool in = plain || (pk.inside >> r & 1);
+          if (in || (p.fill && r < pw.n)) {
+            const bool begin = !plain && (pk.begin >> r & 1);
+            const bool end = !plain && (pk.end >> r & 1);
+            const int s = plain ? 0 : __shfl_sync(0xffffffffu, pk.seq, r);
+            if (begin) {
+#pragma unroll
+              for (int e = 0; e < V; ++e) h[e] = p.first && pw.live ? p.first[(uint64_t)s * p.channels + pw.ch + e] : 0.0f;
+            }
+            const Pack<G, GV> gate = stage_g(p_stage)[r * kThreads];
+            const Pack<T, V> x = stage_x(p_stage)[r * kThreads];
+            Pack<T, V> before;
+            if constexpr (BACK) before = stage_y(p_stage)[r * kThreads];
+            float a[GV], out[V], dg[V];
+#pragma unroll
+            for (int e = 0; e < GV; ++e) {
+              const float g = to_f32<G>(gate.v[e]);
+              a[e] = log_gate ? exp_of(g) : g;
+            }
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+              const float xv = to_f32<T>(x.v[e]), ai = a[SHARED ? 0 : e];
+              if constexpr (BACK) {
+                float prev = to_f32<T>(before.v[e]);
+                if (end) prev = p.initial && pw.live ? p.initial[(uint64_t)s * p.channels + pw.ch + e] : 0.0f;
+                out[e] = xv + h[e];
+                h[e] = ai * out[e];
+                dg[e] = (log_gate ? h[e] : out[e]) * prev;
+              } else {
+                h[e] = begin && !p.first ? xv : fmaf(ai, h[e], xv);
+                out[e] = h[e];
+              }
+            }
+            if (!in) {
+#pragma unroll
+              for (int e = 0; e < V; ++e) out[e] = dg[e] = 0.0f;
+            }
+            if (pw.live) store_floats<T, V>(to, 0, out);
+            if constexpr (BACK) {
+              if constexpr (!SHARED) {
+                if (pw.live) store_floats<G, V>(to_g, 0, dg);
+              } else {
+                // the head's lanes are neighbours; the first of them gathers the sum
+                float sum = 0.0f;
+#pragma unroll
+                for (int e = 0; e < V; ++e) sum += dg[e];
+                if (!pw.live) sum = 0.0f;
+                const uint32_t per = p.parts == 1 ? p.head_size / V : kWarp;
+                const uint32_t place = lane % per;
+                for (uint32_t off = 1; off < per; off *= 2) {
+                  const float other = __shfl_down_sync(0xffffffffu, sum, off);
+                  if (place + off < per) sum += other;
+                }
+                if (pw.live && place == 0) {
+                  if (p.parts == 1) {
+                    const float one[1] = {sum};
+                    store_floats<G, 1>(to_g, 0, one);
+                  } else {
+                    const uint64_t flat = pw.chain * p.chain_rows + (uint64_t)(pw.row - r);
+                    p.partial[(flat * p.heads + pw.head) * p.parts + pw.block % p.parts] = sum;
+                  }
+                }
+              }
+            }
+            if (in && end && p.last && pw.live) {
+#pragma unroll
+              for (int e = 0; e < V; ++e) p.last[(uint64_t)s * p.channels + pw.ch + e] = h[e];
+            }
+          }
+          to += d_out;
+          if constexpr (BACK) to_g += d_g;
+        }
+      };
+      if (pk.plain(ALL)) {
+        if (logg) second_pass(std::true_type{}, std::true_type{}); else second_pass(std::true_type{}, std::false_type{});
+      } else {
+        second_pass(std::false_type{}, logg);
       }
     }
-    eo += next(p.out);
-    if constexpr (BACK) ed += next(p.dgate);
+    if constexpr (STAGES == 3) fetch_two_ahead();  // into the parked tile's stage
+    if (!some) return;
+    parked = true;
+    pw = w;
+    pk = kinds;
+    p_stage = stage;
+    stage = s1;
   }
 }
 
@@ -481,8 +708,10 @@ __global__ void __launch_bounds__(kThreads) join_gate_kernel(RecArgs p, uint64_t
   }
 }
 
-// Blocks of channels for V channels a lane.
-void divide_channels(RecArgs& p, uint32_t width) {
+// Blocks of channels and tiles for a CTA that is `width` channels wide.
+void divide(RecArgs& p, uint32_t width, int bytes_of_row) {
+  const uint64_t tile_rows = (uint64_t)kWarps * rows_of_lane(bytes_of_row);
+  p.tiles = (p.chain_rows + tile_rows - 1) / tile_rows;
   if (p.heads == p.channels) {
     p.blocks = (p.channels + width - 1) / width;
     p.parts = 1;
@@ -496,8 +725,7 @@ void divide_channels(RecArgs& p, uint32_t width) {
   }
 }
 
-constexpr int kRows = 8;  // rows of a lane
-constexpr uint64_t kTileRows = kWarps * kRows;
+constexpr uint64_t kShortRows = 32;  // sequences up to this length fill at most half a tile
 
 struct Call {
   tb200_recurrence_shape shape;
@@ -507,10 +735,12 @@ struct Call {
 };
 
 template <typename T, typename G, int V, bool SHARED, bool BACK>
+struct Tag {};
+template <typename T, typename G, int V, bool SHARED, bool BACK>
 int launch_kernel(Call& k, cudaStream_t stream) {
   RecArgs& p = k.args;
   constexpr uint32_t WIDTH = kWarp * V;
-  divide_channels(p, WIDTH);
+  divide(p, WIDTH, Shape<T, G, V, SHARED, BACK>::ROW);
   const uint64_t ctas = p.tiles * p.chains * p.blocks;
   if (ctas > 0x7fffffffull) return TB200_ERR_UNSUPPORTED;
   if (p.tiles > 1) {
@@ -519,7 +749,18 @@ int launch_kernel(Call& k, cudaStream_t stream) {
     p.maps = reinterpret_cast<unsigned long long*>(k.descriptors + states * sizeof(unsigned));
     TB200_CUDA_TRY(cudaMemsetAsync(p.hdr, 0, kHeaderBytes + states * (sizeof(unsigned) + sizeof(unsigned long long)), stream));
   }
-  recurrence_kernel<T, G, V, SHARED, BACK, kRows><<<(unsigned)ctas, kThreads, 0, stream>>>(p);
+  p.by_blocks = divisor(p.blocks);
+  p.by_chains = divisor(p.chains);
+  p.by_head_size = divisor(p.head_size);
+  constexpr size_t smem = Shape<T, G, V, SHARED, BACK>::kBytes;
+  constexpr int threads = kThreads + kWarp * V;
+  auto kernel = recurrence_kernel<T, G, V, SHARED, BACK>;
+  int per_sm = 0, sms = 0;
+  int rc = resident_ctas<Tag<T, G, V, SHARED, BACK>>(kernel, threads, smem, &per_sm);
+  if (rc == TB200_OK) rc = sm_count_of_device(&sms);
+  if (rc) return rc;
+  const uint64_t slots = (uint64_t)per_sm * sms;
+  kernel<<<(unsigned)(ctas < slots ? ctas : slots), threads, smem, stream>>>(p);
   trace_mark(stream, kTraceRecurrence);
   TB200_CUDA_TRY(cudaGetLastError());
   if (BACK && SHARED && p.parts > 1) {
@@ -592,16 +833,17 @@ int prepare(void* d_temp, size_t* temp_bytes, const tb200_recurrence_shape* shap
   // Sequences of equal length are chains of their own, unless they are so short that their tiles would be mostly empty
   // and lie behind one another (strides, which a size query does not see): then all of them are one chain, as packed
   // ones are.
-  p.chain_is_sequence = s.offset_bytes == 0 && (s.rows > kTileRows / 2 || !dense);
+  p.chain_is_sequence = s.offset_bytes == 0 && (s.rows > kShortRows || !dense);
   p.chains = p.chain_is_sequence ? (uint32_t)s.sequences : 1;
   p.chain_rows = p.chain_is_sequence ? s.rows : k.rows;
-  p.tiles = (p.chain_rows + kTileRows - 1) / kTileRows;
 
   // Descriptors lie directly behind the header, where one clear reaches both; the sums of heads that span several
   // blocks lie behind them. The pointers' alignment decides on four or one channels a lane: room for either.
   size_t descriptors = 0, sums = 0;
-  for (uint32_t width = kWarp; width <= 4 * kWarp; width *= 4) {
-    divide_channels(p, width);
+  const int tb = model_bytes(s.dtype), gb = model_bytes(s.gate_dtype);
+  for (int v = 1; v <= 4; v *= 4) {
+    const uint32_t width = kWarp * v;
+    divide(p, width, v * tb * (back ? 2 : 1) + (s.heads == s.channels ? v : 1) * gb);
     if (p.tiles > 1) {
       const size_t d = p.tiles * p.chains * p.blocks * width * (sizeof(unsigned) + sizeof(unsigned long long));
       if (d > descriptors) descriptors = d;
