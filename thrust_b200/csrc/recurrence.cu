@@ -97,37 +97,41 @@ __device__ __forceinline__ unsigned state_bits(float h) {
 // tile's map, so the value is the same wherever the walk begins, to the bit. At most kReach tiles back; where no state is
 // known there, the wait is for one to come closer, which the tile right behind the last known state always brings about.
 constexpr int kReach = 8;
-__device__ float state_in_front(const unsigned long long* maps, const unsigned* states, uint64_t step, uint64_t tile, int* status) {
-  const int n = tile < kReach ? (int)tile : kReach;
-  for (unsigned polls = 0;; ++polls) {
-    unsigned long long m[kReach];
-    unsigned s[kReach];
+struct InFront {  // what is known of the tiles in front, nearest first
+  unsigned long long maps[kReach];
+  unsigned states[kReach];
+  __device__ __forceinline__ void look(const unsigned long long* m, const unsigned* s, uint64_t step, unsigned tile) {
 #pragma unroll
     for (int j = 0; j < kReach; ++j) {
-      s[j] = j < n ? ld_relaxed_u32(states - (j + 1) * step) : 0u;
-      m[j] = j < n ? ld_relaxed_u64(maps - (j + 1) * step) : 0ull;
+      states[j] = j < tile ? ld_relaxed_u32(s - (j + 1) * step) : 0u;
+      maps[j] = j < tile ? ld_relaxed_u64(m - (j + 1) * step) : 0ull;
     }
-    float h = 0.0f;
+  }
+  __device__ __forceinline__ bool state(float& h) const {
     bool known = false;
+    h = 0.0f;
 #pragma unroll
     for (int j = kReach - 1; j >= 0; --j) {
-      if (s[j] != 0u) {
-        h = __uint_as_float(~s[j]);
-        known = true;
-      } else if (m[j] != 0ull) {
-        h = apply((unsigned)(~m[j] >> 32), h, __uint_as_float((unsigned)~m[j]));
-      } else {
-        known = false;
-      }
+      const float through = apply((unsigned)(~maps[j] >> 32), h, __uint_as_float((unsigned)~maps[j]));
+      h = states[j] != 0u ? __uint_as_float(~states[j]) : through;
+      known = states[j] != 0u || (known && maps[j] != 0ull);
     }
-    if (known) return h;
-    if ((polls & 63u) == 63u && ld_relaxed_s32(status) != 0) return h;  // someone else gave up
+    return known;
+  }
+};
+__device__ __forceinline__ float state_in_front(InFront& f, const unsigned long long* maps, const unsigned* states,
+                                                uint64_t step, unsigned tile, int* status) {
+  float h;
+  for (unsigned polls = 0; !f.state(h); ++polls) {
+    if ((polls & 63u) == 63u && ld_relaxed_s32(status) != 0) break;  // someone else gave up
     if (polls >= kSpinLimit) {
       note_timeout(status, kSiteLookback, tile, 0);
-      return h;
+      break;
     }
     backoff(polls);
+    f.look(maps, states, step, tile);
   }
+  return h;
 }
 
 template <int TILE>
@@ -284,8 +288,8 @@ __global__ void __launch_bounds__(kThreads + kWarp * V, 1) recurrence_kernel(Rec
   constexpr unsigned ALL = (1u << R) - 1;
   extern __shared__ __align__(16) char s_dynamic[];
   __shared__ Marks<TILE> s_marks[2];
-  __shared__ int s_reset[2][kWarps];  // a sequence begins among the warp's rows
-  __shared__ int s_need[2][kWarps];   // the warp has rows in front of that
+  // of the stretches: bit 0, a sequence begins among the rows; bit 1, there are rows in front of that
+  __shared__ __align__(8) unsigned char s_kinds[2][kWarps];
   __shared__ unsigned s_ids[8];       // of the CTA's tiles, a ring
   auto* s_word = reinterpret_cast<unsigned(*)[kWarps][WIDTH]>(s_dynamic + STAGES * S::kStage);
   auto* s_b = reinterpret_cast<float(*)[kWarps][WIDTH]>(s_dynamic + STAGES * S::kStage + 2 * S::kJoin);
@@ -391,35 +395,47 @@ __global__ void __launch_bounds__(kThreads + kWarp * V, 1) recurrence_kernel(Rec
       }
       if (bad) atomicExch(&p.hdr->status, (int)TB200_ERR_INVALID_ARGUMENT);
     }
-    // of the tile in front: its own map, whether its state is to be published, whether it needs the one in front
-    unsigned p_id = 0, p_tile = 0, p_word = 0;
-    float p_b = 0.0f;
+    // of the tile before: its own map and its warps', whether its state is to be published, whether it needs the one in front
+    unsigned p_id = 0, p_tile = 0, p_word = 0, p_words[kWarps] = {};
+    float p_b = 0.0f, p_bs[kWarps] = {};
+    unsigned long long p_begins = 0;
     bool p_state = false, p_wait = false;
     for (unsigned i = 0;; ++i) {
       const int k = i & 1;
       const unsigned id = s_ids[i & 7];
       const bool some = id < total;
       const unsigned behind = s_ids[(i + 1) & 7];
-      if (c == 0) s_ids[(i + 2) & 7] = behind < total ? draw(behind) : total;
+      unsigned drawn = total;  // the answer is looked at much later
+      if (c == 0 && behind < total) drawn = draw(behind);
+      const uint64_t p_at = (uint64_t)p_id * WIDTH + c;
+      InFront front;
+      if (p_wait) front.look(p.maps + p_at, p.states + p_at, step, p_tile);
       if (p.offsets && behind < total) marks_of_tile<TILE, V, SHARED, BACK, R>(p, behind, c < kWarp, s_marks[k ^ 1]);
 
       // ---- this tile's map; behind a begin only B counts --------------------------------------------------
-      bool reset = false, need = false;
-      unsigned word = 0, tile = 0;
-      float tb = 0.0f;
+      unsigned word = 0, tile = 0, words[kWarps] = {};
+      float tb = 0.0f, bs[kWarps] = {};
+      unsigned long long begins = 0;
+      bool need = false;
       if (some) {
         tile = p.by_chains.of(p.by_blocks.of(id));
         named_barrier(kMapsReady + k, CTA);
+        const unsigned long long kinds = *reinterpret_cast<const unsigned long long*>(s_kinds[k]);
+        begins = kinds & 0x0101010101010101ull;
+        need = (kinds >> 1 & 0x0101010101010101ull & (((begins & -begins) << 1) - 1)) != 0;
+#pragma unroll
+        for (int v = 0; v < kWarps; ++v) {
+          words[v] = s_word[k][v][c];
+          bs[v] = s_b[k][v][c];
+        }
         if (chained) {
           float ta = 1.0f, tm = 0.0f;
 #pragma unroll
           for (int v = 0; v < kWarps; ++v) {
-            const unsigned wd = s_word[k][v][c];
-            const float m = __uint_as_float(wd), b = s_b[k][v][c];
-            const float wa = (wd & 1u) ? 1.0f + m : m, wm = (wd & 1u) ? m : m - 1.0f;
-            need = need || (!reset && s_need[k][v]);
-            reset = reset || s_reset[k][v];
-            tb = s_reset[k][v] ? b : apply(wd, tb, b);
+            const float m = __uint_as_float(words[v]);
+            const float wa = (words[v] & 1u) ? 1.0f + m : m, wm = (words[v] & 1u) ? m : m - 1.0f;
+            const float on = apply(words[v], tb, bs[v]);
+            tb = begins >> (8 * v) & 1 ? bs[v] : on;
             ta *= wa;
             tm = fmaf(tm, wa, wm);
           }
@@ -427,7 +443,7 @@ __global__ void __launch_bounds__(kThreads + kWarp * V, 1) recurrence_kernel(Rec
           if (tile + 1 < p.tiles) {
             const uint64_t to = (uint64_t)id * WIDTH + c;
             // no row of any sequence: nobody behind needs a state before a sequence begins, so any will do
-            if (reset || tile == 0 || !need) st_relaxed_u32(p.states + to, state_bits(tb));
+            if (begins || tile == 0 || !need) st_relaxed_u32(p.states + to, state_bits(tb));
             else st_relaxed_u64(p.maps + to, map_bits(word, tb));
           }
         }
@@ -436,27 +452,29 @@ __global__ void __launch_bounds__(kThreads + kWarp * V, 1) recurrence_kernel(Rec
       if (i > 0) {
         float h = 0.0f;
         if (p_wait) {
-          const uint64_t to = (uint64_t)p_id * WIDTH + c;
-          h = state_in_front(p.maps + to, p.states + to, step, p_tile, &p.hdr->status);
-          if (p_state) st_relaxed_u32(p.states + to, state_bits(apply(p_word, h, p_b)));
+          h = state_in_front(front, p.maps + p_at, p.states + p_at, step, p_tile, &p.hdr->status);
+          if (p_state) st_relaxed_u32(p.states + p_at, state_bits(apply(p_word, h, p_b)));
         }
 #pragma unroll
         for (int v = 0; v < kWarps; ++v) {
-          const float b = s_b[k ^ 1][v][c];
           s_b[k ^ 1][v][c] = h;
-          h = s_reset[k ^ 1][v] ? b : apply(s_word[k ^ 1][v][c], h, b);
+          const float on = apply(p_words[v], h, p_bs[v]);
+          h = p_begins >> (8 * v) & 1 ? p_bs[v] : on;
         }
       }
+      if (c == 0) s_ids[(i + 2) & 7] = drawn;
       barrier_arrive(kStatesReady + (k ^ 1), CTA);
       if (!some) return;
       p_id = id;
       p_tile = tile;
       p_word = word;
       p_b = tb;
+      p_begins = begins;
+#pragma unroll
+      for (int v = 0; v < kWarps; ++v) p_words[v] = words[v], p_bs[v] = bs[v];
       p_wait = need && tile > 0;
-      p_state = p_wait && !reset && tile + 1 < p.tiles;
-      __syncwarp();
-      if constexpr (WIDTH > kWarp) named_barrier(kJoined, WIDTH);  // s_ids and marks of one warp, read by all
+      p_state = p_wait && !begins && tile + 1 < p.tiles;
+      if constexpr (WIDTH > kWarp) named_barrier(kJoined, WIDTH); else __syncwarp();  // s_ids, written by one thread
     }
   }
 
@@ -573,9 +591,8 @@ __global__ void __launch_bounds__(kThreads + kWarp * V, 1) recurrence_kernel(Rec
         s_b[k][warp][lane * V + v] = B[v];
       }
       if (lane == 0) {
-        s_reset[k][warp] = kinds.begin != 0;
-        // rows in front of the first begin; all of them without one
-        s_need[k][warp] = (kinds.inside & ((kinds.begin & -kinds.begin) - 1u)) != 0;
+        const bool in_front = (kinds.inside & ((kinds.begin & -kinds.begin) - 1u)) != 0;
+        s_kinds[k][warp] = (unsigned char)((kinds.begin != 0) | in_front << 1);
       }
       barrier_arrive(kMapsReady + k, CTA);
     }
