@@ -47,11 +47,28 @@ __device__ __forceinline__ Pack<T, V> load_pack(const char* base, uint64_t eleme
   return p;
 }
 template <typename T, int V>
-__device__ __forceinline__ void store_floats(char* base, uint64_t element, const float (&f)[V]) {
+__device__ __forceinline__ Pack<T, V> pack_of(const float (&f)[V]) {
   Pack<T, V> p;
 #pragma unroll
   for (int i = 0; i < V; ++i) p.v[i] = from_f32<T>(f[i]);
-  *reinterpret_cast<Pack<T, V>*>(base + element * sizeof(T)) = p;
+  return p;
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void store_floats(char* base, uint64_t element, const float (&f)[V]) {
+  const Pack<T, V> p = pack_of<T, V>(f);
+  const uint64_t at = __cvta_generic_to_global(base + element * sizeof(T));
+  if constexpr (sizeof(p) == 16) {
+    const uint4 w = *reinterpret_cast<const uint4*>(&p);
+    asm volatile("st.global.v4.b32 [%0], {%1, %2, %3, %4};" ::"l"(at), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
+  } else if constexpr (sizeof(p) == 8) {
+    const uint2 w = *reinterpret_cast<const uint2*>(&p);
+    asm volatile("st.global.v2.b32 [%0], {%1, %2};" ::"l"(at), "r"(w.x), "r"(w.y) : "memory");
+  } else if constexpr (sizeof(p) == 4) {
+    asm volatile("st.global.b32 [%0], %1;" ::"l"(at), "r"(*reinterpret_cast<const unsigned*>(&p)) : "memory");
+  } else {
+    asm volatile("st.global.b16 [%0], %1;" ::"l"(at), "h"(*reinterpret_cast<const unsigned short*>(&p)) : "memory");
+  }
 }
 
 // exp(g) - 1 for g in [-0.3, 0]: its power series up to g^7 (the next term is 5e-9 of the value).

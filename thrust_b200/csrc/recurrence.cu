@@ -57,18 +57,73 @@ struct RecArgs {
   float* partial;               // backward, a head over several blocks: their sums, [rows][heads][parts]
   TempHeader* hdr;
   uint32_t blocks, chains;      // blocks of channels, chains
-  Divisor by_blocks, by_chains, by_head_size;
+  Divisor by_blocks, by_chains;
+  // bytes from a row to the next one with the recurrence
+  int next_gate, next_in, next_out, next_y, next_dgate;
   uint64_t tiles;               // of a chain
   unsigned long long* maps;     // [tile][chain][block][channel]: what the tile does to a state (0: not there yet)
   unsigned* states;             // [tile][chain][block][channel]: the state behind the tile (0: not there yet)
 };
 
-// The gate of a row from its logarithm. Errors of it stay within a stretch of a warp's rows, so the fast exponential
-// will do (2^-22 of the value); denormal gates count as zero.
-__device__ __forceinline__ float exp_of(float g) {
+// 2^x. The gate of a row comes from its logarithm this way: errors of it stay within a stretch of a warp's rows, so the
+// fast exponential will do (2^-22 of the value); denormal gates count as zero.
+__device__ __forceinline__ float exp2_fast(float x) {
   float e;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * 1.4426950408889634f));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x));
   return e;
+}
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Two channels at once: the packed 32-bit instructions of this architecture do two in the issue slot of one.
+__device__ __forceinline__ void fma2(float& d0, float& d1, float a0, float a1, float b0, float b1, float c0, float c1) {
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d0), "=f"(d1) : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
+}
+__device__ __forceinline__ void mul2(float& d0, float& d1, float a0, float a1, float b0, float b1) {
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d0), "=f"(d1) : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+__device__ __forceinline__ void add2(float& d0, float& d1, float a0, float a1, float b0, float b1) {
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d0), "=f"(d1) : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+template <int N>
+__device__ __forceinline__ void fma_n(float (&d)[N], const float (&a)[N], const float (&b)[N], const float (&c)[N]) {
+  if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) fma2(d[i], d[i + 1], a[i], a[i + 1], b[i], b[i + 1], c[i], c[i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) d[i] = fmaf(a[i], b[i], c[i]);
+  }
+}
+template <int N>
+__device__ __forceinline__ void mul_n(float (&d)[N], const float (&a)[N], const float (&b)[N]) {
+  if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) mul2(d[i], d[i + 1], a[i], a[i + 1], b[i], b[i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) d[i] = a[i] * b[i];
+  }
+}
+template <int N>
+__device__ __forceinline__ void add_n(float (&d)[N], const float (&a)[N], const float (&b)[N]) {
+  if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) add2(d[i], d[i + 1], a[i], a[i + 1], b[i], b[i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) d[i] = a[i] + b[i];
+  }
+}
+template <int N>
+__device__ __forceinline__ void fill_n(float (&d)[N], float v) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) d[i] = v;
 }
 
 // A of a stretch in one word: A - 1 with the lowest bit set where A >= 1/2, else A with it clear. The bit costs at
@@ -103,8 +158,10 @@ struct InFront {  // what is known of the tiles in front, nearest first
   __device__ __forceinline__ void look(const unsigned long long* m, const unsigned* s, uint64_t step, unsigned tile) {
 #pragma unroll
     for (int j = 0; j < kReach; ++j) {
-      states[j] = j < tile ? ld_relaxed_u32(s - (j + 1) * step) : 0u;
-      maps[j] = j < tile ? ld_relaxed_u64(m - (j + 1) * step) : 0ull;
+      s -= step;
+      m -= step;
+      states[j] = j < tile ? ld_relaxed_u32(s) : 0u;
+      maps[j] = j < tile ? ld_relaxed_u64(m) : 0ull;
     }
   }
   __device__ __forceinline__ bool state(float& h) const {
@@ -139,6 +196,7 @@ struct Marks {  // of the rows of a tile of packed sequences
   int seq[TILE];             // sequence of a first or last row
   unsigned char kind[TILE];  // bit 0: first row of its sequence, bit 1: last
   uint64_t from, to;         // the rows of all sequences
+  bool plain;                // the tile is full, and all its rows are inner ones of one sequence
 };
 
 __device__ __forceinline__ uint64_t offset_at(const RecArgs& p, uint64_t i) {
@@ -148,9 +206,9 @@ __device__ __forceinline__ uint64_t offset_at(const RecArgs& p, uint64_t i) {
 }
 
 // Marks the first and last rows of sequences among rows [r0, r1), in memory order; hands the states of empty sequences
-// that lie here through for channels [c0, c0 + count). For one warp.
+// that lie here through for channels [c0, c0 + count). True where the rows are inner ones of one sequence. For one warp.
 template <int TILE>
-__device__ void mark_rows(const RecArgs& p, uint64_t r0, uint64_t r1, bool at_end, uint32_t c0, uint32_t count, Marks<TILE>& m) {
+__device__ bool mark_rows(const RecArgs& p, uint64_t r0, uint64_t r1, bool at_end, uint32_t c0, uint32_t count, Marks<TILE>& m) {
   const unsigned lane = lane_id();
   for (int i = lane; i < (int)sizeof(m.kind) / 4; i += kWarp) reinterpret_cast<unsigned*>(m.kind)[i] = 0;
   __syncwarp();
@@ -165,6 +223,7 @@ __device__ void mark_rows(const RecArgs& p, uint64_t r0, uint64_t r1, bool at_en
     const uint64_t end = lo + stride - 1;  // the next stretch ends at or behind r0, unless it is cut
     if (end < hi) hi = end;
   }
+  if (lo > 0 && lo <= p.sequences && offset_at(p, lo) > r1) return true;  // inner rows of one sequence
   for (uint64_t j = lo + lane; j <= p.sequences; j += kWarp) {
     const uint64_t v = offset_at(p, j);
     if (v > r1) break;
@@ -182,6 +241,7 @@ __device__ void mark_rows(const RecArgs& p, uint64_t r0, uint64_t r1, bool at_en
       }
     }
   }
+  return false;
 }
 
 // Asynchronous copies of a lane's own channels into its own place in shared memory: no barrier, only the lane's wait.
@@ -191,61 +251,71 @@ __device__ __forceinline__ void copy_async(void* to, const void* from) {
 }
 __device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 
-// What a thread works on in one tile.
-struct Place {
-  uint32_t block, chain, c0, count;  // the block's channels
-  uint32_t ch, head;                 // the lane's first channel, its head
-  bool live;
-  uint32_t tile;
-  int n;        // how many of the warp's rows exist
-  int64_t row;  // the first of them in memory; the others follow with the recurrence (below zero only where n is 0)
+// A tile, as one thread works it out for all: where its first row (with the recurrence) begins in every array, at the
+// block's first channel. The others follow at RecArgs::next_* bytes.
+struct TileInfo {
+  const char *gate, *in, *y;  // y: the row in front in memory, which may not exist
+  char *out, *dgate;
+  int64_t row;          // the first row's place in the chain, in memory order
+  uint32_t id, tile;    // id >= the number of tiles: there is none
+  uint32_t chain, block;
+  uint32_t c0, count;   // the block's channels
+  uint32_t head;        // its first head
+  int rows;             // how many of the tile's rows exist
+  bool plain;           // all, and none is a first or last one; what packed sequences add to that stands in their marks
 };
-template <int V, bool SHARED, bool BACK, int R>
-__device__ __forceinline__ Place place_of(const RecArgs& p, unsigned id) {
-  constexpr uint32_t WIDTH = kWarp * V;
-  Place w;
-  const unsigned rest = p.by_blocks.of(id);
-  w.block = id - rest * p.blocks;
-  w.tile = p.by_chains.of(rest);
-  w.chain = rest - w.tile * p.chains;
-  if (!SHARED) {
-    w.c0 = w.block * WIDTH;
-    w.count = min(WIDTH, p.channels - w.c0);
-  } else if (p.parts == 1) {
-    const uint32_t h0 = w.block * p.block_heads;
-    w.c0 = h0 * p.head_size;
-    w.count = min(p.block_heads, p.heads - h0) * p.head_size;
-  } else {
-    const uint32_t h0 = w.block / p.parts, part = w.block % p.parts;
-    w.c0 = h0 * p.head_size + part * WIDTH;
-    w.count = min(WIDTH, p.head_size - part * WIDTH);
+template <typename T, typename G, int WIDTH, int TILE, bool SHARED, bool BACK>
+__device__ __forceinline__ void describe(const RecArgs& p, unsigned id, unsigned total, TileInfo& o) {
+  o.id = id;
+  if (id >= total) return;
+  const unsigned rest = p.by_blocks.of(id), block = id - rest * p.blocks;
+  const unsigned tile = p.by_chains.of(rest), chain = rest - tile * p.chains;
+  o.tile = tile;
+  o.chain = chain;
+  o.block = block;
+  uint32_t head = 0, c0 = block * WIDTH, count = min((uint32_t)WIDTH, p.channels - c0);
+  if (SHARED && p.parts == 1) {
+    head = block * p.block_heads;
+    c0 = head * p.head_size;
+    count = min(p.block_heads, p.heads - head) * p.head_size;
+  } else if (SHARED) {
+    head = block / p.parts;
+    const uint32_t part = block - head * p.parts;
+    c0 = head * p.head_size + part * WIDTH;
+    count = min((uint32_t)WIDTH, p.head_size - part * WIDTH);
   }
-  const unsigned lane = lane_id();
-  w.ch = w.c0 + lane * V;
-  w.live = lane * V < w.count;
-  w.head = SHARED ? p.by_head_size.of(w.ch) : 0;
-  const uint64_t q = (uint64_t)w.tile * (kWarps * R) + threadIdx.x / kWarp * R;
-  w.n = q >= p.chain_rows ? 0 : p.chain_rows - q < R ? (int)(p.chain_rows - q) : R;
-  w.row = BACK ? (int64_t)p.chain_rows - 1 - (int64_t)q : (int64_t)q;
-  return w;
+  o.c0 = c0;
+  o.count = count;
+  o.head = head;
+  const uint64_t first = (uint64_t)tile * TILE, left = p.chain_rows - first;
+  o.rows = left < TILE ? (int)left : TILE;
+  const int64_t row = BACK ? (int64_t)(p.chain_rows - 1 - first) : (int64_t)first;
+  o.row = row;
+  o.plain = left > TILE && first != 0 && p.chain_is_sequence;
+  auto place = [&](const RowsOf& a, uint32_t column) { return (int64_t)(chain * a.seq + column) + row * (int64_t)a.row; };
+  const uint32_t gate = SHARED ? head : c0;
+  o.gate = p.gate.data + place(p.gate, gate) * (int64_t)sizeof(G);
+  o.in = p.in.data + place(p.in, c0) * (int64_t)sizeof(T);
+  o.out = p.out.data + place(p.out, c0) * (int64_t)sizeof(T);
+  if constexpr (BACK) {
+    o.y = p.y.data + (place(p.y, c0) - (int64_t)p.y.row) * (int64_t)sizeof(T);
+    o.dgate = p.dgate.data + place(p.dgate, gate) * (int64_t)sizeof(G);
+  }
 }
 // Which of the warp's rows are what: bit r of a mask is row r.
 struct RowKinds {
   unsigned inside, begin, end;  // rows of a sequence; its first and last one with the recurrence
   int seq;                      // lane r: the sequence of row r, where that is a first or last one
-  // nothing but rows of one sequence
-  __device__ __forceinline__ bool plain(unsigned all) const { return inside == all && (begin | end) == 0; }
 };
-template <int TILE, int V, bool SHARED, bool BACK, int R>
-__device__ void marks_of_tile(const RecArgs& p, unsigned id, bool mine, Marks<TILE>& m) {
-  if (!mine) return;  // one warp
-  const Place w = place_of<V, SHARED, BACK, R>(p, id);
+template <int TILE, bool BACK>
+__device__ void marks_of_tile(const RecArgs& p, const TileInfo& w, Marks<TILE>& m) {  // for one warp
   const uint64_t lo = (uint64_t)w.tile * TILE, hi = min(lo + TILE, p.chain_rows);
   const uint64_t r0 = BACK ? p.chain_rows - hi : lo, r1 = BACK ? p.chain_rows - lo : hi;
-  mark_rows(p, r0, r1, r1 == p.chain_rows, w.c0, w.count, m);
+  const bool none = mark_rows(p, r0, r1, r1 == p.chain_rows, w.c0, w.count, m);
   if (lane_id() == 0) {
     m.from = offset_at(p, 0);
     m.to = offset_at(p, p.sequences);
+    m.plain = none && w.rows == TILE;
   }
 }
 
@@ -261,6 +331,8 @@ struct Shape {
   static constexpr int R = rows_of_lane(ROW);
   // what takes 4 bytes and more is copied asynchronously, the rest goes through registers
   static constexpr bool X_ASYNC = sizeof(Pack<T, V>) >= 4, G_ASYNC = sizeof(Pack<G, GV>) >= 4;
+  // the exponentials of log gates take the place of gates of 32 bits
+  static constexpr bool KEEPS_EXP = sizeof(G) == 4;
   static constexpr int kX = R * kThreads * (int)sizeof(Pack<T, V>);
   static constexpr int kStage = R * kThreads * ROW;
   static constexpr int STAGES = kStageBudget / kStage >= 4 ? 4 : 3;
@@ -287,10 +359,10 @@ __global__ void __launch_bounds__(kThreads + kWarp * V, 1) recurrence_kernel(Rec
   constexpr int CTA = kThreads + WIDTH;
   constexpr unsigned ALL = (1u << R) - 1;
   extern __shared__ __align__(16) char s_dynamic[];
-  __shared__ Marks<TILE> s_marks[2];
+  __shared__ Marks<TILE> s_marks[4];  // a ring
   // of the stretches: bit 0, a sequence begins among the rows; bit 1, there are rows in front of that
   __shared__ __align__(8) unsigned char s_kinds[2][kWarps];
-  __shared__ unsigned s_ids[8];       // of the CTA's tiles, a ring
+  __shared__ TileInfo s_tiles[8];     // of the CTA, a ring
   auto* s_word = reinterpret_cast<unsigned(*)[kWarps][WIDTH]>(s_dynamic + STAGES * S::kStage);
   auto* s_b = reinterpret_cast<float(*)[kWarps][WIDTH]>(s_dynamic + STAGES * S::kStage + 2 * S::kJoin);
 
@@ -300,11 +372,14 @@ __global__ void __launch_bounds__(kThreads + kWarp * V, 1) recurrence_kernel(Rec
   const bool chained = p.tiles > 1;
   const unsigned total = (unsigned)p.tiles * p.chains * p.blocks;
   auto draw = [&](unsigned behind) { return chained ? atomicAdd(&p.hdr->ticket, 1u) : behind + gridDim.x; };
-
+  auto describe_tile = [&](unsigned id, unsigned i) { describe<T, G, WIDTH, TILE, SHARED, BACK>(p, id, total, s_tiles[i & 7]); };
 
   const bool joins = threadIdx.x >= kThreads;
-  const unsigned lane = lane_id(), warp = threadIdx.x / kWarp;
+  const int lane = (int)lane_id(), warp = (int)(threadIdx.x / kWarp);
   const bool logg = p.log_gate != 0;
+  // the lane's place in a row, in bytes
+  const int lane_x = lane * V * (int)sizeof(T);
+  const int lane_g = SHARED ? (p.parts == 1 ? lane * V / (int)p.head_size : 0) * (int)sizeof(G) : lane * V * (int)sizeof(G);
 
   // the thread's place for row r of a stage: [r * kThreads]
   auto stage_x = [&](int k) { return reinterpret_cast<Pack<T, V>*>(s_dynamic + k * S::kStage) + threadIdx.x; };
@@ -312,10 +387,7 @@ __global__ void __launch_bounds__(kThreads + kWarp * V, 1) recurrence_kernel(Rec
   auto stage_g = [&](int k) {
     return reinterpret_cast<Pack<G, GV>*>(s_dynamic + k * S::kStage + S::kX * (BACK ? 2 : 1)) + threadIdx.x;
   };
-  auto at = [&](const Place& w, const RowsOf& a, uint32_t column) {
-    return (int64_t)(w.chain * a.seq + column) + w.row * (int64_t)a.row;
-  };
-  auto next = [](const RowsOf& a) { return BACK ? -(int64_t)a.row : (int64_t)a.row; };
+  auto row_of = [&](auto* base, int next, int r) { return base + (int64_t)(warp * R + r) * next; };
 
   // Brings a tile's rows on their way to a stage. What is copied through registers gets there with `settle`.
   struct Late {
@@ -323,35 +395,30 @@ __global__ void __launch_bounds__(kThreads + kWarp * V, 1) recurrence_kernel(Rec
     Pack<T, V> x[S::X_ASYNC ? 1 : R];
     Pack<T, V> before[S::X_ASYNC || !BACK ? 1 : R];
   } late;
-  auto fetch = [&](unsigned id, int k) {
-    const Place w = place_of<V, SHARED, BACK, R>(p, id);
-    if (!w.live) return;
-    const char* g = p.gate.data + at(w, p.gate, SHARED ? w.head : w.ch) * (int64_t)sizeof(G);
-    const char* x = p.in.data + at(w, p.in, w.ch) * (int64_t)sizeof(T);
-    const char* y = BACK ? p.y.data + (at(w, p.y, w.ch) - (int64_t)p.y.row) * (int64_t)sizeof(T) : nullptr;
-    const int64_t dg = next(p.gate) * (int64_t)sizeof(G), dx = next(p.in) * (int64_t)sizeof(T);
-    const int64_t dy = BACK ? next(p.y) * (int64_t)sizeof(T) : 0;
+  auto fetch = [&](const TileInfo& w, int k) {
+    if (lane * V >= (int)w.count) return;
+    const char* g = w.gate + lane_g;
+    const char* x = w.in + lane_x;
+    const char* y = BACK ? w.y + lane_x : nullptr;
+    const int n = w.rows - warp * R;  // rows of this warp
     auto rows = [&](auto all) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        if (all || r < w.n) {
-          if constexpr (S::G_ASYNC) copy_async<sizeof(Pack<G, GV>)>(stage_g(k) + r * kThreads, g);
-          else late.gate[r] = load_pack<G, GV>(g, 0);
-          if constexpr (S::X_ASYNC) copy_async<sizeof(Pack<T, V>)>(stage_x(k) + r * kThreads, x);
-          else late.x[r] = load_pack<T, V>(x, 0);
+        if (all || r < n) {
+          if constexpr (S::G_ASYNC) copy_async<sizeof(Pack<G, GV>)>(stage_g(k) + r * kThreads, row_of(g, p.next_gate, r));
+          else late.gate[r] = load_pack<G, GV>(row_of(g, p.next_gate, r), 0);
+          if constexpr (S::X_ASYNC) copy_async<sizeof(Pack<T, V>)>(stage_x(k) + r * kThreads, row_of(x, p.next_in, r));
+          else late.x[r] = load_pack<T, V>(row_of(x, p.next_in, r), 0);
           if constexpr (BACK) {
-            if (all || w.row - r > 0) {
-              if constexpr (S::X_ASYNC) copy_async<sizeof(Pack<T, V>)>(stage_y(k) + r * kThreads, y);
-              else late.before[r] = load_pack<T, V>(y, 0);
+            if (all || w.row - warp * R - r > 0) {
+              if constexpr (S::X_ASYNC) copy_async<sizeof(Pack<T, V>)>(stage_y(k) + r * kThreads, row_of(y, p.next_y, r));
+              else late.before[r] = load_pack<T, V>(row_of(y, p.next_y, r), 0);
             }
           }
         }
-        g += dg;
-        x += dx;
-        if constexpr (BACK) y += dy;
       }
     };
-    if (w.n == R && (!BACK || w.row >= R)) rows(std::true_type{}); else rows(std::false_type{});
+    if (n >= R && (!BACK || w.row >= TILE)) rows(std::true_type{}); else rows(std::false_type{});
   };
   auto settle = [&](int k) {
 #pragma unroll
@@ -364,21 +431,23 @@ __global__ void __launch_bounds__(kThreads + kWarp * V, 1) recurrence_kernel(Rec
     }
   };
 
-  // two tiles to begin with, drawn one by one: a burst would hand neighbouring tiles to one CTA
-  if (threadIdx.x == kThreads) s_ids[0] = chained ? draw(0) : blockIdx.x;
+  if (threadIdx.x == kThreads) describe_tile(chained ? draw(0) : blockIdx.x, 0);
   __syncthreads();
-  const unsigned id0 = s_ids[0];
-  if (id0 >= total) return;
+  if (s_tiles[0].id >= total) return;
   if (!joins) {
-    fetch(id0, 0);
+    fetch(s_tiles[0], 0);
     copies_issued();
     settle(0);
   } else {
     if (threadIdx.x == kThreads) {
-      s_ids[1] = draw(id0);
+      const unsigned id1 = draw(s_tiles[0].id), id2 = draw(id1);
+      describe_tile(id1, 1);
+      describe_tile(id2, 2);
       if (!chained && blockIdx.x == 0) p.hdr->status = TB200_OK;  // scratch that no tile waits in is not cleared
     }
-    if (p.offsets) marks_of_tile<TILE, V, SHARED, BACK, R>(p, id0, threadIdx.x - kThreads < kWarp, s_marks[0]);
+    __syncwarp();
+    if (p.offsets && warp == kWarps)
+      for (int i = 0; i < 2 && s_tiles[i].id < total; ++i) marks_of_tile<TILE, BACK>(p, s_tiles[i], s_marks[i]);
   }
   __syncthreads();
 
@@ -386,7 +455,7 @@ __global__ void __launch_bounds__(kThreads + kWarp * V, 1) recurrence_kernel(Rec
     // ================================ the threads that join: one for each channel ==============================
     const unsigned c = threadIdx.x - kThreads;
     const uint64_t step = (uint64_t)p.chains * p.blocks * WIDTH;
-    if (p.offsets != nullptr && id0 == 0) {  // bad offsets are reported, and cannot lead outside the arrays
+    if (p.offsets != nullptr && s_tiles[0].id == 0) {  // bad offsets are reported, and cannot lead outside the arrays
       bool bad = false;
       for (uint64_t i = c; i <= p.sequences; i += WIDTH) {
         const int64_t v = p.offset_bytes == 4 ? (int64_t)static_cast<const int32_t*>(p.offsets)[i]
@@ -402,15 +471,38 @@ __global__ void __launch_bounds__(kThreads + kWarp * V, 1) recurrence_kernel(Rec
     bool p_state = false, p_wait = false;
     for (unsigned i = 0;; ++i) {
       const int k = i & 1;
-      const unsigned id = s_ids[i & 7];
+      const unsigned id = s_tiles[i & 7].id;
       const bool some = id < total;
-      const unsigned behind = s_ids[(i + 1) & 7];
       unsigned drawn = total;  // the answer is looked at much later
-      if (c == 0 && behind < total) drawn = draw(behind);
+      if (c == 0) {
+        const unsigned newest = s_tiles[(i + 2) & 7].id;
+        if (newest < total) drawn = draw(newest);
+      }
       const uint64_t p_at = (uint64_t)p_id * WIDTH + c;
+      // ---- the states in front of the stretches of the tile before: at once where they are known by now, ---------
+      // ---- else after this tile's map is out -----------------------------------------------------------------------
       InFront front;
-      if (p_wait) front.look(p.maps + p_at, p.states + p_at, step, p_tile);
-      if (p.offsets && behind < total) marks_of_tile<TILE, V, SHARED, BACK, R>(p, behind, c < kWarp, s_marks[k ^ 1]);
+      float in_front = 0.0f;
+      bool known = true;
+      if (p_wait) {
+        front.look(p.maps + p_at, p.states + p_at, step, p_tile);
+        known = front.state(in_front);
+      }
+      auto hand_on = [&] {
+        if (i > 0) {
+          if (p_state) st_relaxed_u32(p.states + p_at, state_bits(apply(p_word, in_front, p_b)));
+          float h = in_front;
+#pragma unroll
+          for (int v = 0; v < kWarps; ++v) {
+            s_b[k ^ 1][v][c] = h;
+            const float on = apply(p_words[v], h, p_bs[v]);
+            h = p_begins >> (8 * v) & 1 ? p_bs[v] : on;
+          }
+        }
+        barrier_arrive(kStatesReady + (k ^ 1), CTA);
+      };
+      const bool at_once = __all_sync(0xffffffffu, known);
+      if (at_once) hand_on();
 
       // ---- this tile's map; behind a begin only B counts --------------------------------------------------
       unsigned word = 0, tile = 0, words[kWarps] = {};
@@ -418,7 +510,7 @@ __global__ void __launch_bounds__(kThreads + kWarp * V, 1) recurrence_kernel(Rec
       unsigned long long begins = 0;
       bool need = false;
       if (some) {
-        tile = p.by_chains.of(p.by_blocks.of(id));
+        tile = s_tiles[i & 7].tile;
         named_barrier(kMapsReady + k, CTA);
         const unsigned long long kinds = *reinterpret_cast<const unsigned long long*>(s_kinds[k]);
         begins = kinds & 0x0101010101010101ull;
@@ -448,23 +540,14 @@ __global__ void __launch_bounds__(kThreads + kWarp * V, 1) recurrence_kernel(Rec
           }
         }
       }
-      // ---- the states in front of the stretches of the tile before -----------------------------------------
-      if (i > 0) {
-        float h = 0.0f;
-        if (p_wait) {
-          h = state_in_front(front, p.maps + p_at, p.states + p_at, step, p_tile, &p.hdr->status);
-          if (p_state) st_relaxed_u32(p.states + p_at, state_bits(apply(p_word, h, p_b)));
-        }
-#pragma unroll
-        for (int v = 0; v < kWarps; ++v) {
-          s_b[k ^ 1][v][c] = h;
-          const float on = apply(p_words[v], h, p_bs[v]);
-          h = p_begins >> (8 * v) & 1 ? p_bs[v] : on;
-        }
+      if (!at_once) {
+        if (!known) in_front = state_in_front(front, p.maps + p_at, p.states + p_at, step, p_tile, &p.hdr->status);
+        hand_on();
       }
-      if (c == 0) s_ids[(i + 2) & 7] = drawn;
-      barrier_arrive(kStatesReady + (k ^ 1), CTA);
       if (!some) return;
+      if (c == 0) describe_tile(drawn, i + 3);
+      if (p.offsets && warp == kWarps && s_tiles[(i + 2) & 7].id < total)
+        marks_of_tile<TILE, BACK>(p, s_tiles[(i + 2) & 7], s_marks[(i + 2) & 3]);
       p_id = id;
       p_tile = tile;
       p_word = word;
@@ -474,104 +557,114 @@ __global__ void __launch_bounds__(kThreads + kWarp * V, 1) recurrence_kernel(Rec
       for (int v = 0; v < kWarps; ++v) p_words[v] = words[v], p_bs[v] = bs[v];
       p_wait = need && tile > 0;
       p_state = p_wait && !begins && tile + 1 < p.tiles;
-      if constexpr (WIDTH > kWarp) named_barrier(kJoined, WIDTH); else __syncwarp();  // s_ids, written by one thread
+      // what one thread has described, and no thread far ahead of the others
+      if constexpr (WIDTH > kWarp) named_barrier(kJoined, WIDTH); else __syncwarp();
     }
   }
 
   // ==================================== the warps that compute ================================================
-  Place pw{};
   RowKinds pk{};
-  bool parked = false, unsettled = false;
+  bool parked = false, unsettled = false, p_plain = false;
   int stage = 0, p_stage = 0;  // of tile i, of the tile in front
   for (unsigned i = 0;; ++i) {
     const int k = i & 1;
-    const unsigned id = s_ids[i & 7];
-    const bool some = id < total;
+    const TileInfo& w = s_tiles[i & 7];
+    const bool some = w.id < total;
     const int s1 = stage + 1 == STAGES ? 0 : stage + 1, s2 = s1 + 1 == STAGES ? 0 : s1 + 1;
     if (i == 0) {
-      const unsigned id1 = s_ids[1];
-      if (id1 < total) {
-        fetch(id1, s1);
+      if (s_tiles[1].id < total) {
+        fetch(s_tiles[1], s1);
         unsettled = true;
       }
       copies_issued();
     }
-    Place w{};
-    RowKinds kinds{};
+    const bool plain = p.offsets ? s_marks[i & 3].plain : w.plain;
+    RowKinds kinds{ALL, 0, 0, 0};
     if (some) {
-      w = place_of<V, SHARED, BACK, R>(p, id);
       // ---- first and last rows of sequences ---------------------------------------------------------------
-      const uint64_t mine = (uint64_t)(BACK ? w.row - (int)lane : w.row + (int)lane);  // lane r: row r, if it exists
-      const bool valid = (int)lane < w.n;
-      unsigned m_first = 0, m_last = 0;
-      kinds.inside = (1u << w.n) - 1;
-      kinds.seq = w.chain;
-      if (p.offsets != nullptr) {
-        const uint64_t lo = (uint64_t)w.tile * TILE, hi = min(lo + TILE, p.chain_rows);
-        const uint64_t r0 = BACK ? p.chain_rows - hi : lo;
-        const unsigned kind = valid ? s_marks[k].kind[mine - r0] : 0;
-        if (kind & 3) kinds.seq = s_marks[k].seq[mine - r0];
-        m_first = __ballot_sync(0xffffffffu, kind & 1);
-        m_last = __ballot_sync(0xffffffffu, kind & 2);
-        kinds.inside = __ballot_sync(0xffffffffu, valid && mine >= s_marks[k].from && mine < s_marks[k].to);
-      } else if (p.chain_is_sequence) {
-        m_first = __ballot_sync(0xffffffffu, valid && mine == 0);
-        m_last = __ballot_sync(0xffffffffu, valid && mine == p.chain_rows - 1);
-      } else {  // sequences of equal length behind one another
-        const uint64_t m = valid ? mine : 0;
-        const uint64_t s = p.chain_rows >> 32 ? m / p.length : (uint32_t)m / (uint32_t)p.length;
-        const uint64_t t = m - s * p.length;
-        kinds.seq = (int)s;
-        m_first = __ballot_sync(0xffffffffu, valid && t == 0);
-        m_last = __ballot_sync(0xffffffffu, valid && t == p.length - 1);
+      if (!plain) {
+        const int n = max(0, min(R, w.rows - warp * R));
+        const bool valid = lane < n;
+        const int64_t mine = valid ? (BACK ? w.row - warp * R - lane : w.row + warp * R + lane) : 0;  // lane r: row r
+        unsigned m_first = 0, m_last = 0;
+        kinds.inside = (1u << n) - 1;
+        kinds.seq = w.chain;
+        if (p.offsets != nullptr) {
+          const uint64_t lo = (uint64_t)w.tile * TILE, hi = min(lo + TILE, p.chain_rows);
+          const int64_t r0 = BACK ? p.chain_rows - hi : lo;
+          const unsigned kind = valid ? s_marks[i & 3].kind[mine - r0] : 0;
+          if (kind) kinds.seq = s_marks[i & 3].seq[mine - r0];
+          m_first = __ballot_sync(0xffffffffu, kind & 1);
+          m_last = __ballot_sync(0xffffffffu, kind & 2);
+          kinds.inside = __ballot_sync(0xffffffffu, valid && (uint64_t)mine >= s_marks[i & 3].from && (uint64_t)mine < s_marks[i & 3].to);
+        } else if (p.chain_is_sequence) {
+          m_first = __ballot_sync(0xffffffffu, valid && mine == 0);
+          m_last = __ballot_sync(0xffffffffu, valid && (uint64_t)mine == p.chain_rows - 1);
+        } else {  // sequences of equal length behind one another
+          const uint64_t s = p.chain_rows >> 32 ? (uint64_t)mine / p.length : (uint32_t)mine / (uint32_t)p.length;
+          const uint64_t t = (uint64_t)mine - s * p.length;
+          kinds.seq = (int)s;
+          m_first = __ballot_sync(0xffffffffu, valid && t == 0);
+          m_last = __ballot_sync(0xffffffffu, valid && t == p.length - 1);
+        }
+        kinds.begin = BACK ? m_last : m_first;
+        kinds.end = BACK ? m_first : m_last;
       }
-      kinds.begin = BACK ? m_last : m_first;
-      kinds.end = BACK ? m_first : m_last;
 
       // ---- first pass: the stretch's A and B ----------------------------------------------------------------
       asm volatile("cp.async.wait_group 1;" ::: "memory");  // all but the copies of the tile behind
       float A[GV], M[GV], B[V], sum[GV];
-#pragma unroll
-      for (int e = 0; e < GV; ++e) A[e] = 1.0f, M[e] = 0.0f, sum[e] = 0.0f;
-#pragma unroll
-      for (int e = 0; e < V; ++e) B[e] = 0.0f;
-      auto first_pass = [&](auto plain, auto log_gate) {
+      fill_n(A, 1.0f);
+      fill_n(M, 0.0f);
+      fill_n(sum, 0.0f);
+      fill_n(B, 0.0f);
+      auto first_pass = [&](auto inner, auto log_gate) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          if (!plain && !(kinds.inside >> r & 1)) continue;
-          const bool begin = !plain && (kinds.begin >> r & 1);
+          if (!inner && !(kinds.inside >> r & 1)) continue;
+          const bool begin = !inner && (kinds.begin >> r & 1);
           if (begin) {
             const int s = __shfl_sync(0xffffffffu, kinds.seq, r);
 #pragma unroll
-            for (int e = 0; e < V; ++e) B[e] = p.first && w.live ? p.first[(uint64_t)s * p.channels + w.ch + e] : 0.0f;
+            for (int e = 0; e < V; ++e)
+              B[e] = p.first && lane * V < (int)w.count ? p.first[(uint64_t)s * p.channels + w.c0 + lane * V + e] : 0.0f;
           }
           const Pack<G, GV> gate = stage_g(stage)[r * kThreads];
           const Pack<T, V> x = stage_x(stage)[r * kThreads];
-          float a[GV];
+          float a[GV], av[V], xv[V];
 #pragma unroll
-          for (int e = 0; e < GV; ++e) {
-            const float g = to_f32<G>(gate.v[e]);
-            if (log_gate) {
-              sum[e] += g;
-              a[e] = exp_of(g);
-            } else {
-              A[e] *= g;
-              M[e] = fmaf(M[e], g, g - 1.0f);
-              a[e] = g;
-            }
+          for (int e = 0; e < GV; ++e) a[e] = to_f32<G>(gate.v[e]);
+#pragma unroll
+          for (int e = 0; e < V; ++e) xv[e] = to_f32<T>(x.v[e]);
+          if (log_gate) {
+            float unit[GV];
+            fill_n(unit, kLog2e);
+            add_n(sum, sum, a);
+            mul_n(a, a, unit);
+#pragma unroll
+            for (int e = 0; e < GV; ++e) a[e] = exp2_fast(a[e]);
+            if constexpr (S::KEEPS_EXP) stage_g(stage)[r * kThreads] = pack_of<G, GV>(a);  // for the second pass
+          } else {
+            float less[GV], one[GV];
+            fill_n(one, -1.0f);
+            add_n(less, a, one);
+            mul_n(A, A, a);
+            fma_n(M, M, a, less);
           }
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const float ai = a[SHARED ? 0 : e], xv = to_f32<T>(x.v[e]);
-            if constexpr (BACK) {
-              B[e] = ai * (xv + B[e]);
-            } else {
-              B[e] = begin && !p.first ? xv : fmaf(ai, B[e], xv);
-            }
+          for (int e = 0; e < V; ++e) av[e] = a[SHARED ? 0 : e];
+          if constexpr (BACK) {
+            add_n(B, xv, B);
+            mul_n(B, av, B);
+          } else if (begin && !p.first) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) B[e] = xv[e];
+          } else {
+            fma_n(B, av, B, xv);
           }
         }
       };
-      if (kinds.plain(ALL)) {
+      if (plain) {
         if (logg) first_pass(std::true_type{}, std::true_type{}); else first_pass(std::true_type{}, std::false_type{});
       } else {
         first_pass(std::false_type{}, logg);
@@ -585,11 +678,11 @@ __global__ void __launch_bounds__(kThreads + kWarp * V, 1) recurrence_kernel(Rec
           M[e] = near ? c : c - 1.0f;
         }
       }
+      Pack<unsigned, V> words;
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        s_word[k][warp][lane * V + v] = word_of(A[SHARED ? 0 : v], M[SHARED ? 0 : v]);
-        s_b[k][warp][lane * V + v] = B[v];
-      }
+      for (int e = 0; e < V; ++e) words.v[e] = word_of(A[SHARED ? 0 : e], M[SHARED ? 0 : e]);
+      *reinterpret_cast<Pack<unsigned, V>*>(&s_word[k][warp][lane * V]) = words;
+      *reinterpret_cast<Pack<float, V>*>(&s_b[k][warp][lane * V]) = pack_of<float, V>(B);
       if (lane == 0) {
         const bool in_front = (kinds.inside & ((kinds.begin & -kinds.begin) - 1u)) != 0;
         s_kinds[k][warp] = (unsigned char)((kinds.begin != 0) | in_front << 1);
@@ -601,9 +694,9 @@ __global__ void __launch_bounds__(kThreads + kWarp * V, 1) recurrence_kernel(Rec
 
     named_barrier(kStatesReady + (k ^ 1), CTA);
     auto fetch_two_ahead = [&] {
-      const unsigned id2 = s_ids[(i + 2) & 7];
-      if (id2 < total) {
-        fetch(id2, s2);
+      const TileInfo& ahead = s_tiles[(i + 2) & 7];
+      if (some && ahead.id < total) {
+        fetch(ahead, s2);
         unsettled = true;
       }
       copies_issued();
@@ -612,89 +705,101 @@ __global__ void __launch_bounds__(kThreads + kWarp * V, 1) recurrence_kernel(Rec
 
     // ---- second pass: the parked tile's outputs ---------------------------------------------------------------
     if (parked) {
+      const TileInfo& pw = s_tiles[(i - 1) & 7];
+      const bool live = lane * V < (int)pw.count;
+      const uint32_t ch = pw.c0 + lane * V;
+      const Pack<float, V> in_front = *reinterpret_cast<const Pack<float, V>*>(&s_b[k ^ 1][warp][lane * V]);
       float h[V];
 #pragma unroll
-      for (int e = 0; e < V; ++e) h[e] = s_b[k ^ 1][warp][lane * V + e];
-      char* to = p.out.data + at(pw, p.out, pw.ch) * (int64_t)sizeof(T);
-      char* to_g = BACK ? p.dgate.data + at(pw, p.dgate, SHARED ? pw.head : pw.ch) * (int64_t)sizeof(G) : nullptr;
-      const int64_t d_out = next(p.out) * (int64_t)sizeof(T), d_g = BACK ? next(p.dgate) * (int64_t)sizeof(G) : 0;
-      auto second_pass = [&](auto plain, auto log_gate) {
+      for (int e = 0; e < V; ++e) h[e] = in_front.v[e];
+      char* to = pw.out + lane_x;
+      char* to_g = BACK ? pw.dgate + lane_g : nullptr;
+      auto second_pass = [&](auto inner, auto log_gate) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          const bool in = plain || (pk.inside >> r & 1);
-          if (in || (p.fill && r < pw.n)) {
-            const bool begin = !plain && (pk.begin >> r & 1);
-            const bool end = !plain && (pk.end >> r & 1);
-            const int s = plain ? 0 : __shfl_sync(0xffffffffu, pk.seq, r);
-            if (begin) {
+          const bool in = inner || (pk.inside >> r & 1);
+          if (!in && !(p.fill && warp * R + r < pw.rows)) continue;
+          const bool begin = !inner && (pk.begin >> r & 1);
+          const bool end = !inner && (pk.end >> r & 1);
+          const int s = inner ? 0 : __shfl_sync(0xffffffffu, pk.seq, r);
+          if (begin) {
 #pragma unroll
-              for (int e = 0; e < V; ++e) h[e] = p.first && pw.live ? p.first[(uint64_t)s * p.channels + pw.ch + e] : 0.0f;
+            for (int e = 0; e < V; ++e) h[e] = p.first && live ? p.first[(uint64_t)s * p.channels + ch + e] : 0.0f;
+          }
+          const Pack<G, GV> gate = stage_g(p_stage)[r * kThreads];
+          const Pack<T, V> x = stage_x(p_stage)[r * kThreads];
+          float a[GV], av[V], xv[V], out[V], dg[V];
+#pragma unroll
+          for (int e = 0; e < GV; ++e) a[e] = to_f32<G>(gate.v[e]);
+          if (!S::KEEPS_EXP && log_gate) {
+            float unit[GV];
+            fill_n(unit, kLog2e);
+            mul_n(a, a, unit);
+#pragma unroll
+            for (int e = 0; e < GV; ++e) a[e] = exp2_fast(a[e]);
+          }
+#pragma unroll
+          for (int e = 0; e < V; ++e) av[e] = a[SHARED ? 0 : e], xv[e] = to_f32<T>(x.v[e]);
+          if constexpr (BACK) {
+            const Pack<T, V> before = stage_y(p_stage)[r * kThreads];
+            float prev[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) prev[e] = to_f32<T>(before.v[e]);
+            if (end) {
+#pragma unroll
+              for (int e = 0; e < V; ++e) prev[e] = p.initial && live ? p.initial[(uint64_t)s * p.channels + ch + e] : 0.0f;
             }
-            const Pack<G, GV> gate = stage_g(p_stage)[r * kThreads];
-            const Pack<T, V> x = stage_x(p_stage)[r * kThreads];
-            Pack<T, V> before;
-            if constexpr (BACK) before = stage_y(p_stage)[r * kThreads];
-            float a[GV], out[V], dg[V];
+            add_n(out, xv, h);
+            mul_n(h, av, out);
+            if (log_gate) mul_n(dg, h, prev); else mul_n(dg, out, prev);
+          } else {
+            if (begin && !p.first) {
 #pragma unroll
-            for (int e = 0; e < GV; ++e) {
-              const float g = to_f32<G>(gate.v[e]);
-              a[e] = log_gate ? exp_of(g) : g;
+              for (int e = 0; e < V; ++e) h[e] = xv[e];
+            } else {
+              fma_n(h, av, h, xv);
             }
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-              const float xv = to_f32<T>(x.v[e]), ai = a[SHARED ? 0 : e];
-              if constexpr (BACK) {
-                float prev = to_f32<T>(before.v[e]);
-                if (end) prev = p.initial && pw.live ? p.initial[(uint64_t)s * p.channels + pw.ch + e] : 0.0f;
-                out[e] = xv + h[e];
-                h[e] = ai * out[e];
-                dg[e] = (log_gate ? h[e] : out[e]) * prev;
-              } else {
-                h[e] = begin && !p.first ? xv : fmaf(ai, h[e], xv);
-                out[e] = h[e];
+            for (int e = 0; e < V; ++e) out[e] = h[e];
+          }
+          if (!in) {
+            fill_n(out, 0.0f);
+            fill_n(dg, 0.0f);
+          }
+          if (live) store_floats<T, V>(row_of(to, p.next_out, r), 0, out);
+          if constexpr (BACK) {
+            if constexpr (!SHARED) {
+              if (live) store_floats<G, V>(row_of(to_g, p.next_dgate, r), 0, dg);
+            } else {
+              // the head's lanes are neighbours; the first of them gathers the sum
+              float sum = 0.0f;
+#pragma unroll
+              for (int e = 0; e < V; ++e) sum += dg[e];
+              if (!live) sum = 0.0f;
+              const int per = p.parts == 1 ? (int)p.head_size / V : kWarp;
+              const int place = lane % per;
+              for (int off = 1; off < per; off *= 2) {
+                const float other = __shfl_down_sync(0xffffffffu, sum, off);
+                if (place + off < per) sum += other;
               }
-            }
-            if (!in) {
-#pragma unroll
-              for (int e = 0; e < V; ++e) out[e] = dg[e] = 0.0f;
-            }
-            if (pw.live) store_floats<T, V>(to, 0, out);
-            if constexpr (BACK) {
-              if constexpr (!SHARED) {
-                if (pw.live) store_floats<G, V>(to_g, 0, dg);
-              } else {
-                // the head's lanes are neighbours; the first of them gathers the sum
-                float sum = 0.0f;
-#pragma unroll
-                for (int e = 0; e < V; ++e) sum += dg[e];
-                if (!pw.live) sum = 0.0f;
-                const uint32_t per = p.parts == 1 ? p.head_size / V : kWarp;
-                const uint32_t place = lane % per;
-                for (uint32_t off = 1; off < per; off *= 2) {
-                  const float other = __shfl_down_sync(0xffffffffu, sum, off);
-                  if (place + off < per) sum += other;
-                }
-                if (pw.live && place == 0) {
-                  if (p.parts == 1) {
-                    const float one[1] = {sum};
-                    store_floats<G, 1>(to_g, 0, one);
-                  } else {
-                    const uint64_t flat = pw.chain * p.chain_rows + (uint64_t)(pw.row - r);
-                    p.partial[(flat * p.heads + pw.head) * p.parts + pw.block % p.parts] = sum;
-                  }
+              if (live && place == 0) {
+                if (p.parts == 1) {
+                  const float one[1] = {sum};
+                  store_floats<G, 1>(row_of(to_g, p.next_dgate, r), 0, one);
+                } else {
+                  const uint64_t flat = pw.chain * p.chain_rows + (uint64_t)(pw.row - warp * R - r);
+                  p.partial[(flat * p.heads + pw.head) * p.parts + pw.block % p.parts] = sum;
                 }
               }
-            }
-            if (in && end && p.last && pw.live) {
-#pragma unroll
-              for (int e = 0; e < V; ++e) p.last[(uint64_t)s * p.channels + pw.ch + e] = h[e];
             }
           }
-          to += d_out;
-          if constexpr (BACK) to_g += d_g;
+          if (in && end && p.last && live) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) p.last[(uint64_t)s * p.channels + ch + e] = h[e];
+          }
         }
       };
-      if (pk.plain(ALL)) {
+      if (p_plain) {
         if (logg) second_pass(std::true_type{}, std::true_type{}); else second_pass(std::true_type{}, std::false_type{});
       } else {
         second_pass(std::false_type{}, logg);
@@ -703,7 +808,7 @@ __global__ void __launch_bounds__(kThreads + kWarp * V, 1) recurrence_kernel(Rec
     if constexpr (STAGES == 3) fetch_two_ahead();  // into the parked tile's stage
     if (!some) return;
     parked = true;
-    pw = w;
+    p_plain = plain;
     pk = kinds;
     p_stage = stage;
     stage = s1;
@@ -768,7 +873,14 @@ int launch_kernel(Call& k, cudaStream_t stream) {
   }
   p.by_blocks = divisor(p.blocks);
   p.by_chains = divisor(p.chains);
-  p.by_head_size = divisor(p.head_size);
+  const auto next = [](const RowsOf& a, int elem) { return (int)(a.row * elem) * (BACK ? -1 : 1); };
+  for (const RowsOf* a : {&p.gate, &p.in, &p.out, &p.y, &p.dgate})
+    if (a->row > (1u << 28)) return TB200_ERR_UNSUPPORTED;  // a tile's rows are reached by 32-bit steps
+  p.next_gate = next(p.gate, sizeof(G));
+  p.next_in = next(p.in, sizeof(T));
+  p.next_out = next(p.out, sizeof(T));
+  p.next_y = next(p.y, sizeof(T));
+  p.next_dgate = next(p.dgate, sizeof(G));
   constexpr size_t smem = Shape<T, G, V, SHARED, BACK>::kBytes;
   constexpr int threads = kThreads + kWarp * V;
   auto kernel = recurrence_kernel<T, G, V, SHARED, BACK>;
