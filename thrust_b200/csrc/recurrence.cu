@@ -15,6 +15,7 @@
 // memory. With log gates in [-0.3, 0] the state therefore advances by its change, h + ((a - 1) * h + x), with a - 1
 // from its own series, and A is the exponential of the SUM of the gates, in the same two forms; with plain gates
 // A - 1 is carried beside A. States, products and sums are held in 32 bits; outputs are rounded once.
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -321,25 +322,36 @@ __device__ void marks_of_tile(const RecArgs& p, const TileInfo& w, Marks<TILE>& 
 
 // Bytes of shared memory that tiles may take, beside the joins and marks.
 constexpr int kStageBudget = 200 << 10;
-// Rows of a lane: eight, or four where eight rows of everything would leave room for less than three tiles.
-constexpr int rows_of_lane(int bytes_of_row) { return 3 * 8 * bytes_of_row * kThreads <= kStageBudget ? 8 : 4; }
+constexpr int kStages = 4;  // a tile in each: parked, landed, and two on their way
+// Rows of a lane: eight, or four where four tiles of eight rows a lane would not fit.
+constexpr int rows_of_lane(int bytes_of_row) { return kStages * 8 * bytes_of_row * kThreads <= kStageBudget ? 8 : 4; }
 
 template <typename T, typename G, int V, bool SHARED, bool BACK>
 struct Shape {
   static constexpr int GV = SHARED ? 1 : V;  // gates of a lane in a row
   static constexpr int ROW = (int)(sizeof(Pack<T, V>) * (BACK ? 2 : 1) + sizeof(Pack<G, GV>));
   static constexpr int R = rows_of_lane(ROW);
-  // what takes 4 bytes and more is copied asynchronously, the rest goes through registers
-  static constexpr bool X_ASYNC = sizeof(Pack<T, V>) >= 4, G_ASYNC = sizeof(Pack<G, GV>) >= 4;
+  // Four channels a lane: tiles come as boxes of a tensor map. One: every thread copies its own channels, 4 bytes and
+  // more asynchronously, less through registers. Shared gates always take the latter way.
+  static constexpr bool BOXES = V == 4;
+  static constexpr bool X_ASYNC = sizeof(T) >= 4, G_ASYNC = !SHARED && sizeof(G) >= 4;
   // the exponentials of log gates take the place of gates of 32 bits
-  static constexpr bool KEEPS_EXP = sizeof(G) == 4;
+  static constexpr bool KEEPS_EXP = sizeof(G) == 4 && !SHARED;
   static constexpr int kX = R * kThreads * (int)sizeof(Pack<T, V>);
-  static constexpr int kStage = R * kThreads * ROW;
-  static constexpr int STAGES = kStageBudget / kStage >= 4 ? 4 : 3;
+  static constexpr int kGate = R * kThreads * (int)sizeof(Pack<G, GV>);
+  static constexpr int kStage = kX * (BACK ? 2 : 1) + kGate;
+  [[maybe_unused]] static constexpr int kBoxes = kX * (BACK ? 2 : 1) + (SHARED ? 0 : kGate);
   static constexpr int kJoin = kWarps * kWarp * V * 4;
-  static constexpr size_t kBytes = (size_t)STAGES * kStage + 4 * kJoin;
-  static_assert(STAGES * kStage <= kStageBudget, "a tile on its way, a landed one and a parked one");
+  static constexpr size_t kBytes = (size_t)kStages * kStage + 4 * kJoin;
+  static_assert(kStages * kStage <= kStageBudget && kStage % 128 == 0 && kX % 128 == 0, "room and alignment of the stages");
 };
+
+// A box of rows and channels of one sequence into shared memory. x is a multiple of 16 bytes; rows and channels outside the
+// array come as zeros. Never used with multicast.
+__device__ __forceinline__ void box_load(void* to, const CUtensorMap* map, int x, int y, int z, unsigned long long* bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+               ::"r"(smem_u32(to)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar)) : "memory");
+}
 
 // Barriers between the warps that compute and the warps that join, by the parity of the tile.
 enum : int { kMapsReady = 1, kStatesReady = 3, kJoined = 5 };
@@ -350,21 +362,23 @@ __device__ __forceinline__ void barrier_arrive(int id, int count) {
 // One CTA on an SM, which takes tile after tile. Eight warps compute: the first pass over a tile as soon as its rows
 // have landed, the second pass over the tile in front, whose rows wait in shared memory, once the state in front of it is
 // known. One thread for each channel joins: it puts the warps' stretches together, publishes the tile's map, and finds
-// the state in front of the tile before, all while the others compute. Every thread copies the rows that it computes
-// itself, so their arrival needs no barrier.
+// the state in front of the tile before, all while the others compute.
 template <typename T, typename G, int V, bool SHARED, bool BACK>
-__global__ void __launch_bounds__(kThreads + kWarp * V, 1) recurrence_kernel(RecArgs p) {
+__global__ void __launch_bounds__(kThreads + kWarp * V, 1)
+recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUtensorMap map_gate,
+                  const __grid_constant__ CUtensorMap map_in, const __grid_constant__ CUtensorMap map_y) {
   using S = Shape<T, G, V, SHARED, BACK>;
-  constexpr int WIDTH = kWarp * V, GV = S::GV, R = S::R, TILE = kWarps * R, STAGES = S::STAGES;
+  constexpr int WIDTH = kWarp * V, GV = S::GV, R = S::R, TILE = kWarps * R;
   constexpr int CTA = kThreads + WIDTH;
   constexpr unsigned ALL = (1u << R) - 1;
-  extern __shared__ __align__(16) char s_dynamic[];
+  extern __shared__ __align__(128) char s_dynamic[];
   __shared__ Marks<TILE> s_marks[4];  // a ring
   // of the stretches: bit 0, a sequence begins among the rows; bit 1, there are rows in front of that
   __shared__ __align__(8) unsigned char s_kinds[2][kWarps];
-  __shared__ TileInfo s_tiles[8];     // of the CTA, a ring
-  auto* s_word = reinterpret_cast<unsigned(*)[kWarps][WIDTH]>(s_dynamic + STAGES * S::kStage);
-  auto* s_b = reinterpret_cast<float(*)[kWarps][WIDTH]>(s_dynamic + STAGES * S::kStage + 2 * S::kJoin);
+  __shared__ TileInfo s_tiles[8];  // of the CTA, a ring
+  __shared__ unsigned long long s_landed[kStages];
+  auto* s_word = reinterpret_cast<unsigned(*)[kWarps][WIDTH]>(s_dynamic + kStages * S::kStage);
+  auto* s_b = reinterpret_cast<float(*)[kWarps][WIDTH]>(s_dynamic + kStages * S::kStage + 2 * S::kJoin);
 
   // Tiles are handed out in the order of the recurrence, all chains and blocks of channels of one stretch of rows before
   // the next: whatever a tile waits for is worked on by a CTA that runs already, and a tile's map never waits for more
@@ -377,60 +391,97 @@ __global__ void __launch_bounds__(kThreads + kWarp * V, 1) recurrence_kernel(Rec
   const bool joins = threadIdx.x >= kThreads;
   const int lane = (int)lane_id(), warp = (int)(threadIdx.x / kWarp);
   const bool logg = p.log_gate != 0;
-  // the lane's place in a row, in bytes
+  // the lane's place in a row, in bytes; shared gates: its head's place among the block's
   const int lane_x = lane * V * (int)sizeof(T);
-  const int lane_g = SHARED ? (p.parts == 1 ? lane * V / (int)p.head_size : 0) * (int)sizeof(G) : lane * V * (int)sizeof(G);
+  const int lane_head = SHARED && p.parts == 1 ? lane * V / (int)p.head_size : 0;
+  const int lane_g = SHARED ? lane_head * (int)sizeof(G) : lane * V * (int)sizeof(G);
+  constexpr int GATES = SHARED ? kWarp : WIDTH;  // places for gates in a row of a stage
 
-  // the thread's place for row r of a stage: [r * kThreads]
-  auto stage_x = [&](int k) { return reinterpret_cast<Pack<T, V>*>(s_dynamic + k * S::kStage) + threadIdx.x; };
-  auto stage_y = [&](int k) { return reinterpret_cast<Pack<T, V>*>(s_dynamic + k * S::kStage + S::kX) + threadIdx.x; };
-  auto stage_g = [&](int k) {
-    return reinterpret_cast<Pack<G, GV>*>(s_dynamic + k * S::kStage + S::kX * (BACK ? 2 : 1)) + threadIdx.x;
-  };
+  // row r of the warp in a stage; rows lie in the order of memory
+  auto place = [&](int r) { return BACK ? TILE - 1 - (warp * R + r) : warp * R + r; };
+  auto stage_x = [&](int k, int r) { return reinterpret_cast<Pack<T, V>*>(s_dynamic + k * S::kStage + place(r) * WIDTH * (int)sizeof(T) + lane_x); };
+  auto stage_y = [&](int k, int r) { return reinterpret_cast<Pack<T, V>*>(s_dynamic + k * S::kStage + S::kX + place(r) * WIDTH * (int)sizeof(T) + lane_x); };
+  char* const gates = s_dynamic + S::kX * (BACK ? 2 : 1);
+  auto stage_g = [&](int k, int r) { return reinterpret_cast<Pack<G, GV>*>(gates + k * S::kStage + place(r) * GATES * (int)sizeof(G) + lane_g); };
   auto row_of = [&](auto* base, int next, int r) { return base + (int64_t)(warp * R + r) * next; };
 
-  // Brings a tile's rows on their way to a stage. What is copied through registers gets there with `settle`.
+  // Brings a tile's rows on their way to a stage. One thread asks for the boxes; what comes through registers gets to
+  // the stage with `settle`.
   struct Late {
-    Pack<G, GV> gate[S::G_ASYNC ? 1 : R];
-    Pack<T, V> x[S::X_ASYNC ? 1 : R];
-    Pack<T, V> before[S::X_ASYNC || !BACK ? 1 : R];
+    G gate[S::G_ASYNC || S::BOXES && !SHARED ? 1 : R];
+    T x[S::X_ASYNC || S::BOXES ? 1 : R];
+    T before[S::X_ASYNC || S::BOXES || !BACK ? 1 : R];
   } late;
+  const int block_gates = SHARED ? (p.parts == 1 ? (int)p.block_heads : 1) : 0;  // of a row
   auto fetch = [&](const TileInfo& w, int k) {
-    if (lane * V >= (int)w.count) return;
-    const char* g = w.gate + lane_g;
-    const char* x = w.in + lane_x;
-    const char* y = BACK ? w.y + lane_x : nullptr;
+    if constexpr (S::BOXES) {
+      if (threadIdx.x == 0) {
+        unsigned long long* bar = &s_landed[k];
+        char* to = s_dynamic + k * S::kStage;
+        const int y = BACK ? (int)w.row - (TILE - 1) : (int)w.row, z = p.chain_is_sequence ? (int)w.chain : 0;
+        mbar_expect_tx(bar, S::kBoxes);
+        box_load(to, &map_in, (int)w.c0, y, z, bar);
+        if constexpr (BACK) box_load(to + S::kX, &map_y, (int)w.c0, y - 1, z, bar);
+        if constexpr (!SHARED) box_load(to + S::kX * (BACK ? 2 : 1), &map_gate, (int)w.c0, y, z, bar);
+      }
+    }
     const int n = w.rows - warp * R;  // rows of this warp
-    auto rows = [&](auto all) {
+    if constexpr (SHARED) {
+      // the warp's gates, one a lane: row by row, the block's heads of a row side by side
+      const int here = w.count < p.head_size ? 1 : (int)(w.count / p.head_size);
+#pragma unroll
+      for (int j = 0; j < R; ++j) {
+        const int v = j * kWarp + lane, r = v / block_gates, h = v - r * block_gates;
+        if (j * kWarp >= R * block_gates) break;
+        if (r < R && r < n && h < here) late.gate[j] = load_pack<G, 1>(row_of(w.gate, p.next_gate, r), h).v[0];
+      }
+    }
+    if constexpr (!S::BOXES) {
+      if (lane >= (int)w.count) return;
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        if (all || r < n) {
-          if constexpr (S::G_ASYNC) copy_async<sizeof(Pack<G, GV>)>(stage_g(k) + r * kThreads, row_of(g, p.next_gate, r));
-          else late.gate[r] = load_pack<G, GV>(row_of(g, p.next_gate, r), 0);
-          if constexpr (S::X_ASYNC) copy_async<sizeof(Pack<T, V>)>(stage_x(k) + r * kThreads, row_of(x, p.next_in, r));
-          else late.x[r] = load_pack<T, V>(row_of(x, p.next_in, r), 0);
-          if constexpr (BACK) {
-            if (all || w.row - warp * R - r > 0) {
-              if constexpr (S::X_ASYNC) copy_async<sizeof(Pack<T, V>)>(stage_y(k) + r * kThreads, row_of(y, p.next_y, r));
-              else late.before[r] = load_pack<T, V>(row_of(y, p.next_y, r), 0);
-            }
+        if (r >= n) break;
+        const char* x = row_of(w.in + lane_x, p.next_in, r);
+        if constexpr (S::X_ASYNC) copy_async<sizeof(T)>(stage_x(k, r), x); else late.x[r] = load_pack<T, 1>(x, 0).v[0];
+        if constexpr (!SHARED) {
+          const char* g = row_of(w.gate + lane_g, p.next_gate, r);
+          if constexpr (S::G_ASYNC) copy_async<sizeof(G)>(stage_g(k, r), g); else late.gate[r] = load_pack<G, 1>(g, 0).v[0];
+        }
+        if constexpr (BACK) {
+          if (w.row - warp * R - r > 0) {
+            const char* y = row_of(w.y + lane_x, p.next_y, r);
+            if constexpr (S::X_ASYNC) copy_async<sizeof(T)>(stage_y(k, r), y); else late.before[r] = load_pack<T, 1>(y, 0).v[0];
           }
         }
       }
-    };
-    if (n >= R && (!BACK || w.row >= TILE)) rows(std::true_type{}); else rows(std::false_type{});
-  };
-  auto settle = [&](int k) {
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      if constexpr (!S::G_ASYNC) stage_g(k)[r * kThreads] = late.gate[r];
-      if constexpr (!S::X_ASYNC) {
-        stage_x(k)[r * kThreads] = late.x[r];
-        if constexpr (BACK) stage_y(k)[r * kThreads] = late.before[r];
-      }
     }
   };
+  auto settle = [&](int k) {
+    if constexpr (SHARED) {
+#pragma unroll
+      for (int j = 0; j < R; ++j) {
+        const int v = j * kWarp + lane, r = v / block_gates, h = v - r * block_gates;
+        if (j * kWarp >= R * block_gates) break;
+        if (r < R) reinterpret_cast<G*>(gates + k * S::kStage)[place(r) * GATES + h] = late.gate[j];
+      }
+    }
+    if constexpr (!S::BOXES) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        if constexpr (!S::G_ASYNC && !SHARED) stage_g(k, r)->v[0] = late.gate[r];
+        if constexpr (!S::X_ASYNC) {
+          stage_x(k, r)->v[0] = late.x[r];
+          if constexpr (BACK) stage_y(k, r)->v[0] = late.before[r];
+        }
+      }
+    }
+    __syncwarp();  // lanes read one another's gates
+  };
 
+  if (S::BOXES && threadIdx.x == 0) {
+    for (int k = 0; k < kStages; ++k) mbar_init(&s_landed[k], 1);
+    mbar_init_fence();
+  }
   if (threadIdx.x == kThreads) describe_tile(chained ? draw(0) : blockIdx.x, 0);
   __syncthreads();
   if (s_tiles[0].id >= total) return;
@@ -565,12 +616,11 @@ __global__ void __launch_bounds__(kThreads + kWarp * V, 1) recurrence_kernel(Rec
   // ==================================== the warps that compute ================================================
   RowKinds pk{};
   bool parked = false, unsettled = false, p_plain = false;
-  int stage = 0, p_stage = 0;  // of tile i, of the tile in front
   for (unsigned i = 0;; ++i) {
     const int k = i & 1;
     const TileInfo& w = s_tiles[i & 7];
     const bool some = w.id < total;
-    const int s1 = stage + 1 == STAGES ? 0 : stage + 1, s2 = s1 + 1 == STAGES ? 0 : s1 + 1;
+    const int stage = i % kStages, s1 = (i + 1) % kStages, s2 = (i + 2) % kStages, p_stage = (i + 3) % kStages;
     if (i == 0) {
       if (s_tiles[1].id < total) {
         fetch(s_tiles[1], s1);
@@ -612,7 +662,16 @@ __global__ void __launch_bounds__(kThreads + kWarp * V, 1) recurrence_kernel(Rec
       }
 
       // ---- first pass: the stretch's A and B ----------------------------------------------------------------
-      asm volatile("cp.async.wait_group 1;" ::: "memory");  // all but the copies of the tile behind
+      if constexpr (S::BOXES) mbar_wait_bounded(&s_landed[stage], i / kStages & 1, &p.hdr->status);
+      else asm volatile("cp.async.wait_group 1;" ::: "memory");  // all but the copies of the tile behind
+      // all values first: nothing below comes between the loads
+      Pack<G, GV> gate[R];
+      Pack<T, V> x[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        gate[r] = *stage_g(stage, r);
+        x[r] = *stage_x(stage, r);
+      }
       float A[GV], M[GV], B[V], sum[GV];
       fill_n(A, 1.0f);
       fill_n(M, 0.0f);
@@ -629,13 +688,11 @@ __global__ void __launch_bounds__(kThreads + kWarp * V, 1) recurrence_kernel(Rec
             for (int e = 0; e < V; ++e)
               B[e] = p.first && lane * V < (int)w.count ? p.first[(uint64_t)s * p.channels + w.c0 + lane * V + e] : 0.0f;
           }
-          const Pack<G, GV> gate = stage_g(stage)[r * kThreads];
-          const Pack<T, V> x = stage_x(stage)[r * kThreads];
           float a[GV], av[V], xv[V];
 #pragma unroll
-          for (int e = 0; e < GV; ++e) a[e] = to_f32<G>(gate.v[e]);
+          for (int e = 0; e < GV; ++e) a[e] = to_f32<G>(gate[r].v[e]);
 #pragma unroll
-          for (int e = 0; e < V; ++e) xv[e] = to_f32<T>(x.v[e]);
+          for (int e = 0; e < V; ++e) xv[e] = to_f32<T>(x[r].v[e]);
           if (log_gate) {
             float unit[GV];
             fill_n(unit, kLog2e);
@@ -643,7 +700,7 @@ __global__ void __launch_bounds__(kThreads + kWarp * V, 1) recurrence_kernel(Rec
             mul_n(a, a, unit);
 #pragma unroll
             for (int e = 0; e < GV; ++e) a[e] = exp2_fast(a[e]);
-            if constexpr (S::KEEPS_EXP) stage_g(stage)[r * kThreads] = pack_of<G, GV>(a);  // for the second pass
+            if constexpr (S::KEEPS_EXP) *stage_g(stage, r) = pack_of<G, GV>(a);  // for the second pass
           } else {
             float less[GV], one[GV];
             fill_n(one, -1.0f);
@@ -701,7 +758,7 @@ __global__ void __launch_bounds__(kThreads + kWarp * V, 1) recurrence_kernel(Rec
       }
       copies_issued();
     };
-    if constexpr (STAGES > 3) fetch_two_ahead();  // into the stage that the tile before the parked one has left
+    fetch_two_ahead();  // into the stage that the tile before the parked one has left
 
     // ---- second pass: the parked tile's outputs ---------------------------------------------------------------
     if (parked) {
@@ -712,6 +769,14 @@ __global__ void __launch_bounds__(kThreads + kWarp * V, 1) recurrence_kernel(Rec
       float h[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) h[e] = in_front.v[e];
+      Pack<G, GV> gate[R];
+      Pack<T, V> x[R], before[BACK ? R : 1];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        gate[r] = *stage_g(p_stage, r);
+        x[r] = *stage_x(p_stage, r);
+        if constexpr (BACK) before[r] = *stage_y(p_stage, r);
+      }
       char* to = pw.out + lane_x;
       char* to_g = BACK ? pw.dgate + lane_g : nullptr;
       auto second_pass = [&](auto inner, auto log_gate) {
@@ -726,11 +791,9 @@ __global__ void __launch_bounds__(kThreads + kWarp * V, 1) recurrence_kernel(Rec
 #pragma unroll
             for (int e = 0; e < V; ++e) h[e] = p.first && live ? p.first[(uint64_t)s * p.channels + ch + e] : 0.0f;
           }
-          const Pack<G, GV> gate = stage_g(p_stage)[r * kThreads];
-          const Pack<T, V> x = stage_x(p_stage)[r * kThreads];
           float a[GV], av[V], xv[V], out[V], dg[V];
 #pragma unroll
-          for (int e = 0; e < GV; ++e) a[e] = to_f32<G>(gate.v[e]);
+          for (int e = 0; e < GV; ++e) a[e] = to_f32<G>(gate[r].v[e]);
           if (!S::KEEPS_EXP && log_gate) {
             float unit[GV];
             fill_n(unit, kLog2e);
@@ -739,12 +802,11 @@ __global__ void __launch_bounds__(kThreads + kWarp * V, 1) recurrence_kernel(Rec
             for (int e = 0; e < GV; ++e) a[e] = exp2_fast(a[e]);
           }
 #pragma unroll
-          for (int e = 0; e < V; ++e) av[e] = a[SHARED ? 0 : e], xv[e] = to_f32<T>(x.v[e]);
+          for (int e = 0; e < V; ++e) av[e] = a[SHARED ? 0 : e], xv[e] = to_f32<T>(x[r].v[e]);
           if constexpr (BACK) {
-            const Pack<T, V> before = stage_y(p_stage)[r * kThreads];
             float prev[V];
 #pragma unroll
-            for (int e = 0; e < V; ++e) prev[e] = to_f32<T>(before.v[e]);
+            for (int e = 0; e < V; ++e) prev[e] = to_f32<T>(before[r].v[e]);
             if (end) {
 #pragma unroll
               for (int e = 0; e < V; ++e) prev[e] = p.initial && live ? p.initial[(uint64_t)s * p.channels + ch + e] : 0.0f;
@@ -805,13 +867,11 @@ __global__ void __launch_bounds__(kThreads + kWarp * V, 1) recurrence_kernel(Rec
         second_pass(std::false_type{}, logg);
       }
     }
-    if constexpr (STAGES == 3) fetch_two_ahead();  // into the parked tile's stage
     if (!some) return;
+    if (S::KEEPS_EXP && S::BOXES) fence_proxy_async_smem();  // exponentials were stored where boxes will land
     parked = true;
     p_plain = plain;
     pk = kinds;
-    p_stage = stage;
-    stage = s1;
   }
 }
 
@@ -856,10 +916,49 @@ struct Call {
   char* descriptors;
 };
 
+// ---- tensor maps ------------------------------------------------------------------------------------------------------
+
+using EncodeTiled = decltype(&cuTensorMapEncodeTiled);
+EncodeTiled encode_tiled() {  // asked of the runtime, so that the library does not link the driver
+  static const EncodeTiled fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess) {
+      (void)cudaGetLastError();
+      f = nullptr;
+    }
+    return reinterpret_cast<EncodeTiled>(f);
+  }();
+  return fn;
+}
+template <typename T> constexpr CUtensorMapDataType map_type();
+template <> constexpr CUtensorMapDataType map_type<float>() { return CU_TENSOR_MAP_DATA_TYPE_FLOAT32; }
+template <> constexpr CUtensorMapDataType map_type<__half>() { return CU_TENSOR_MAP_DATA_TYPE_FLOAT16; }
+template <> constexpr CUtensorMapDataType map_type<__nv_bfloat16>() { return CU_TENSOR_MAP_DATA_TYPE_BFLOAT16; }
+
+// Boxes of `rows` rows by 128 channels of an array of [sequences][rows][channels]. False where it cannot be had.
+template <typename T>
+bool map_of(CUtensorMap* map, const RowsOf& a, const RecArgs& p, int rows) {
+  constexpr uint64_t E = sizeof(T);
+  const uint64_t sequences = p.chain_is_sequence ? p.sequences : 1;
+  const uint64_t apart = sequences > 1 ? a.seq * E : a.row * E;
+  if (!rows_on(a, E, 16) || a.row == 0 || apart == 0 || apart >= (1ull << 40) || a.row * E >= (1ull << 40)) return false;
+  const cuuint64_t dims[3] = {p.channels, p.chain_rows, sequences};
+  const cuuint64_t strides[2] = {a.row * E, apart};
+  const cuuint32_t box[3] = {4 * kWarp, (cuuint32_t)rows, 1}, ones[3] = {1, 1, 1};
+  return encode_tiled()(map, map_type<T>(), 3, a.data, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+struct Maps {
+  CUtensorMap gate, in, y;
+};
+
 template <typename T, typename G, int V, bool SHARED, bool BACK>
 struct Tag {};
 template <typename T, typename G, int V, bool SHARED, bool BACK>
-int launch_kernel(Call& k, cudaStream_t stream) {
+int launch_kernel(Call& k, const Maps& maps, cudaStream_t stream) {
   RecArgs& p = k.args;
   constexpr uint32_t WIDTH = kWarp * V;
   divide(p, WIDTH, Shape<T, G, V, SHARED, BACK>::ROW);
@@ -889,7 +988,7 @@ int launch_kernel(Call& k, cudaStream_t stream) {
   if (rc == TB200_OK) rc = sm_count_of_device(&sms);
   if (rc) return rc;
   const uint64_t slots = (uint64_t)per_sm * sms;
-  kernel<<<(unsigned)(ctas < slots ? ctas : slots), threads, smem, stream>>>(p);
+  kernel<<<(unsigned)(ctas < slots ? ctas : slots), threads, smem, stream>>>(p, maps.gate, maps.in, maps.y);
   trace_mark(stream, kTraceRecurrence);
   TB200_CUDA_TRY(cudaGetLastError());
   if (BACK && SHARED && p.parts > 1) {
@@ -906,19 +1005,26 @@ template <typename T, typename G, bool BACK>
 int launch_typed(Call& k, cudaStream_t stream) {
   RecArgs& p = k.args;
   const bool shared = p.heads != p.channels;
+  // Four channels a lane, in boxes, where boxes can be had of everything that is read (rows and the blocks' first
+  // channels on 16 bytes), rows are written in whole groups of four and a head's channels divide so; else one.
   constexpr int ST = 4 * sizeof(T), SG = 4 * sizeof(G);
-  // four channels a lane where every row of every array begins on that many elements and a head's channels divide so
-  bool wide = p.channels % 4 == 0 && rows_on(p.in, sizeof(T), ST) && rows_on(p.out, sizeof(T), ST);
-  if (BACK) wide = wide && rows_on(p.y, sizeof(T), ST);
+  Maps maps{};
+  bool wide = p.channels % 4 == 0 && p.chain_rows < (1ull << 31) && encode_tiled() != nullptr && rows_on(p.out, sizeof(T), ST);
   if (shared) {
     wide = wide && p.head_size % 4 == 0;
-  } else {
-    wide = wide && rows_on(p.gate, sizeof(G), SG);
-    if (BACK) wide = wide && rows_on(p.dgate, sizeof(G), SG);
+    divide(p, 4 * kWarp, 0);
+    const uint32_t block = p.parts == 1 ? p.block_heads * p.head_size : p.head_size;
+    wide = wide && block * sizeof(T) % 16 == 0;
+  } else if (BACK) {
+    wide = wide && rows_on(p.dgate, sizeof(G), SG);
   }
+  const int rows = kWarps * (shared ? Shape<T, G, 4, true, BACK>::R : Shape<T, G, 4, false, BACK>::R);
+  wide = wide && map_of<T>(&maps.in, p.in, p, rows);
+  if (BACK) wide = wide && map_of<T>(&maps.y, p.y, p, rows);
+  if (!shared) wide = wide && map_of<G>(&maps.gate, p.gate, p, rows);
   if (shared)
-    return wide ? launch_kernel<T, G, 4, true, BACK>(k, stream) : launch_kernel<T, G, 1, true, BACK>(k, stream);
-  return wide ? launch_kernel<T, G, 4, false, BACK>(k, stream) : launch_kernel<T, G, 1, false, BACK>(k, stream);
+    return wide ? launch_kernel<T, G, 4, true, BACK>(k, maps, stream) : launch_kernel<T, G, 1, true, BACK>(k, maps, stream);
+  return wide ? launch_kernel<T, G, 4, false, BACK>(k, maps, stream) : launch_kernel<T, G, 1, false, BACK>(k, maps, stream);
 }
 
 template <bool BACK>
