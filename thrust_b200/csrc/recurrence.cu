@@ -165,23 +165,32 @@ struct InFront {  // what is known of the tiles in front, nearest first
       maps[j] = j < tile ? ld_relaxed_u64(m) : 0ull;
     }
   }
+  // For a whole warp: from the nearest state that all its channels know.
   __device__ __forceinline__ bool state(float& h) const {
-    bool known = false;
     h = 0.0f;
+    unsigned all_states = 0, all_maps = 0;
+#pragma unroll
+    for (int j = 0; j < kReach; ++j) {
+      all_states |= (unsigned)__all_sync(0xffffffffu, states[j] != 0u) << j;
+      all_maps |= (unsigned)__all_sync(0xffffffffu, maps[j] != 0ull) << j;
+    }
+    if (all_states == 0) return false;
+    const int from = __ffs(all_states) - 1;  // the maps of all nearer tiles are needed
+    if ((~all_maps & ((1u << from) - 1u)) != 0) return false;
 #pragma unroll
     for (int j = kReach - 1; j >= 0; --j) {
-      const float through = apply((unsigned)(~maps[j] >> 32), h, __uint_as_float((unsigned)~maps[j]));
-      h = states[j] != 0u ? __uint_as_float(~states[j]) : through;
-      known = states[j] != 0u || (known && maps[j] != 0ull);
+      if (j > from) continue;
+      h = j == from ? __uint_as_float(~states[j])
+                    : apply((unsigned)(~maps[j] >> 32), h, __uint_as_float((unsigned)~maps[j]));
     }
-    return known;
+    return true;
   }
 };
 __device__ __forceinline__ float state_in_front(InFront& f, const unsigned long long* maps, const unsigned* states,
                                                 uint64_t step, unsigned tile, int* status) {
   float h;
   for (unsigned polls = 0; !f.state(h); ++polls) {
-    if ((polls & 63u) == 63u && ld_relaxed_s32(status) != 0) break;  // someone else gave up
+    if ((polls & 63u) == 63u && __any_sync(0xffffffffu, ld_relaxed_s32(status) != 0)) break;  // someone else gave up
     if (polls >= kSpinLimit) {
       note_timeout(status, kSiteLookback, tile, 0);
       break;
@@ -353,8 +362,14 @@ __device__ __forceinline__ void box_load(void* to, const CUtensorMap* map, int x
                ::"r"(smem_u32(to)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar)) : "memory");
 }
 
-// Barriers between the warps that compute and the warps that join, by the parity of the tile.
-enum : int { kMapsReady = 1, kStatesReady = 3, kJoined = 5 };
+// Barriers: the states in front of a tile's stretches are there, by the parity of the tile; among the warps that join.
+enum : int { kStatesReady = 1, kJoined = 3 };
+__device__ __forceinline__ bool mbar_test(unsigned long long* bar, unsigned parity) {  // without waiting
+  unsigned ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return ok != 0;
+}
 __device__ __forceinline__ void barrier_arrive(int id, int count) {
   asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(count) : "memory");
 }
@@ -376,7 +391,8 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
   // of the stretches: bit 0, a sequence begins among the rows; bit 1, there are rows in front of that
   __shared__ __align__(8) unsigned char s_kinds[2][kWarps];
   __shared__ TileInfo s_tiles[8];  // of the CTA, a ring
-  __shared__ unsigned long long s_landed[kStages];
+  __shared__ unsigned long long s_landed[kStages];  // a stage's boxes
+  __shared__ unsigned long long s_ready[2];         // the maps of all warps' stretches, by the parity of the tile
   auto* s_word = reinterpret_cast<unsigned(*)[kWarps][WIDTH]>(s_dynamic + kStages * S::kStage);
   auto* s_b = reinterpret_cast<float(*)[kWarps][WIDTH]>(s_dynamic + kStages * S::kStage + 2 * S::kJoin);
 
@@ -405,26 +421,25 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
   auto stage_g = [&](int k, int r) { return reinterpret_cast<Pack<G, GV>*>(gates + k * S::kStage + place(r) * GATES * (int)sizeof(G) + lane_g); };
   auto row_of = [&](auto* base, int next, int r) { return base + (int64_t)(warp * R + r) * next; };
 
-  // Brings a tile's rows on their way to a stage. One thread asks for the boxes; what comes through registers gets to
-  // the stage with `settle`.
+  // Brings a tile's rows on their way to a stage. One thread asks for the boxes; the rest every computing warp
+  // fetches for itself, and what comes through registers gets to the stage with `settle`.
   struct Late {
     G gate[S::G_ASYNC || S::BOXES && !SHARED ? 1 : R];
     T x[S::X_ASYNC || S::BOXES ? 1 : R];
     T before[S::X_ASYNC || S::BOXES || !BACK ? 1 : R];
   } late;
   const int block_gates = SHARED ? (p.parts == 1 ? (int)p.block_heads : 1) : 0;  // of a row
+  constexpr int ASKS = CTA - kWarp;  // the thread that asks for the boxes
+  auto fetch_boxes = [&](const TileInfo& w, int k) {
+    unsigned long long* bar = &s_landed[k];
+    char* to = s_dynamic + k * S::kStage;
+    const int y = BACK ? (int)w.row - (TILE - 1) : (int)w.row, z = p.chain_is_sequence ? (int)w.chain : 0;
+    mbar_expect_tx(bar, S::kBoxes);
+    box_load(to, &map_in, (int)w.c0, y, z, bar);
+    if constexpr (BACK) box_load(to + S::kX, &map_y, (int)w.c0, y - 1, z, bar);
+    if constexpr (!SHARED) box_load(to + S::kX * (BACK ? 2 : 1), &map_gate, (int)w.c0, y, z, bar);
+  };
   auto fetch = [&](const TileInfo& w, int k) {
-    if constexpr (S::BOXES) {
-      if (threadIdx.x == 0) {
-        unsigned long long* bar = &s_landed[k];
-        char* to = s_dynamic + k * S::kStage;
-        const int y = BACK ? (int)w.row - (TILE - 1) : (int)w.row, z = p.chain_is_sequence ? (int)w.chain : 0;
-        mbar_expect_tx(bar, S::kBoxes);
-        box_load(to, &map_in, (int)w.c0, y, z, bar);
-        if constexpr (BACK) box_load(to + S::kX, &map_y, (int)w.c0, y - 1, z, bar);
-        if constexpr (!SHARED) box_load(to + S::kX * (BACK ? 2 : 1), &map_gate, (int)w.c0, y, z, bar);
-      }
-    }
     const int n = w.rows - warp * R;  // rows of this warp
     if constexpr (SHARED) {
       // the warp's gates, one a lane: row by row, the block's heads of a row side by side
@@ -478,8 +493,9 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
     __syncwarp();  // lanes read one another's gates
   };
 
-  if (S::BOXES && threadIdx.x == 0) {
+  if (threadIdx.x == ASKS) {
     for (int k = 0; k < kStages; ++k) mbar_init(&s_landed[k], 1);
+    for (int k = 0; k < 2; ++k) mbar_init(&s_ready[k], kWarps);
     mbar_init_fence();
   }
   if (threadIdx.x == kThreads) describe_tile(chained ? draw(0) : blockIdx.x, 0);
@@ -490,6 +506,7 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
     copies_issued();
     settle(0);
   } else {
+    if (S::BOXES && threadIdx.x == ASKS) fetch_boxes(s_tiles[0], 0);
     if (threadIdx.x == kThreads) {
       const unsigned id1 = draw(s_tiles[0].id), id2 = draw(id1);
       describe_tile(id1, 1);
@@ -515,6 +532,7 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
       }
       if (bad) atomicExch(&p.hdr->status, (int)TB200_ERR_INVALID_ARGUMENT);
     }
+    if (S::BOXES && threadIdx.x == ASKS && s_tiles[1].id < total) fetch_boxes(s_tiles[1], 1);
     // of the tile before: its own map and its warps', whether its state is to be published, whether it needs the one in front
     unsigned p_id = 0, p_tile = 0, p_word = 0, p_words[kWarps] = {};
     float p_b = 0.0f, p_bs[kWarps] = {};
@@ -535,9 +553,12 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
       InFront front;
       float in_front = 0.0f;
       bool known = true;
+      unsigned long long* maps_ready = &s_ready[k];
       if (p_wait) {
-        front.look(p.maps + p_at, p.states + p_at, step, p_tile);
-        known = front.state(in_front);
+        do {  // as long as there is nothing else to do
+          front.look(p.maps + p_at, p.states + p_at, step, p_tile);
+          known = front.state(in_front);
+        } while (!known && some && !__any_sync(0xffffffffu, mbar_test(maps_ready, i >> 1 & 1)));
       }
       auto hand_on = [&] {
         if (i > 0) {
@@ -552,8 +573,7 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
         }
         barrier_arrive(kStatesReady + (k ^ 1), CTA);
       };
-      const bool at_once = __all_sync(0xffffffffu, known);
-      if (at_once) hand_on();
+      if (known) hand_on();
 
       // ---- this tile's map; behind a begin only B counts --------------------------------------------------
       unsigned word = 0, tile = 0, words[kWarps] = {};
@@ -562,7 +582,9 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
       bool need = false;
       if (some) {
         tile = s_tiles[i & 7].tile;
-        named_barrier(kMapsReady + k, CTA);
+        mbar_wait_bounded(maps_ready, i >> 1 & 1, &p.hdr->status);
+        // all warps are done with the tile before the parked one: its stage is free
+        if (S::BOXES && threadIdx.x == ASKS && s_tiles[(i + 2) & 7].id < total) fetch_boxes(s_tiles[(i + 2) & 7], (i + 2) % kStages);
         const unsigned long long kinds = *reinterpret_cast<const unsigned long long*>(s_kinds[k]);
         begins = kinds & 0x0101010101010101ull;
         need = (kinds >> 1 & 0x0101010101010101ull & (((begins & -begins) << 1) - 1)) != 0;
@@ -591,8 +613,8 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
           }
         }
       }
-      if (!at_once) {
-        if (!known) in_front = state_in_front(front, p.maps + p_at, p.states + p_at, step, p_tile, &p.hdr->status);
+      if (!known) {
+        in_front = state_in_front(front, p.maps + p_at, p.states + p_at, step, p_tile, &p.hdr->status);
         hand_on();
       }
       if (!some) return;
@@ -621,7 +643,7 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
     const TileInfo& w = s_tiles[i & 7];
     const bool some = w.id < total;
     const int stage = i % kStages, s1 = (i + 1) % kStages, s2 = (i + 2) % kStages, p_stage = (i + 3) % kStages;
-    if (i == 0) {
+    if ((!S::BOXES || SHARED) && i == 0) {
       if (s_tiles[1].id < total) {
         fetch(s_tiles[1], s1);
         unsettled = true;
@@ -744,7 +766,8 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
         const bool in_front = (kinds.inside & ((kinds.begin & -kinds.begin) - 1u)) != 0;
         s_kinds[k][warp] = (unsigned char)((kinds.begin != 0) | in_front << 1);
       }
-      barrier_arrive(kMapsReady + k, CTA);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s_ready[k]);
     }
     if (unsettled) settle(s1);  // what was fetched a step ago, for the tile behind this one
     unsettled = false;
@@ -758,7 +781,7 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
       }
       copies_issued();
     };
-    fetch_two_ahead();  // into the stage that the tile before the parked one has left
+    if constexpr (!S::BOXES || SHARED) fetch_two_ahead();  // into the stage that the tile before the parked one has left
 
     // ---- second pass: the parked tile's outputs ---------------------------------------------------------------
     if (parked) {
@@ -828,10 +851,10 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
             fill_n(out, 0.0f);
             fill_n(dg, 0.0f);
           }
-          if (live) store_floats<T, V>(row_of(to, p.next_out, r), 0, out);
+          if ((inner && !SHARED) || live) store_floats<T, V>(row_of(to, p.next_out, r), 0, out);
           if constexpr (BACK) {
             if constexpr (!SHARED) {
-              if (live) store_floats<G, V>(row_of(to_g, p.next_dgate, r), 0, dg);
+              if (inner || live) store_floats<G, V>(row_of(to_g, p.next_dgate, r), 0, dg);
             } else {
               // the head's lanes are neighbours; the first of them gathers the sum
               float sum = 0.0f;
@@ -861,7 +884,9 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
           }
         }
       };
-      if (p_plain) {
+      if (!SHARED && p_plain && !live) {
+        // nothing to write
+      } else if (p_plain) {
         if (logg) second_pass(std::true_type{}, std::true_type{}); else second_pass(std::true_type{}, std::false_type{});
       } else {
         second_pass(std::false_type{}, logg);
