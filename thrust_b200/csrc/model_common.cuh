@@ -71,6 +71,66 @@ __device__ __forceinline__ void store_floats(char* base, uint64_t element, const
   }
 }
 
+// 2^x, off by 2^-22 of the value; denormal results count as zero.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x));
+  return e;
+}
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Two channels at once: the packed 32-bit instructions of this architecture do two in the issue slot of one.
+__device__ __forceinline__ void fma2(float& d0, float& d1, float a0, float a1, float b0, float b1, float c0, float c1) {
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d0), "=f"(d1) : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
+}
+__device__ __forceinline__ void mul2(float& d0, float& d1, float a0, float a1, float b0, float b1) {
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d0), "=f"(d1) : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+__device__ __forceinline__ void add2(float& d0, float& d1, float a0, float a1, float b0, float b1) {
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d0), "=f"(d1) : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+template <int N>
+__device__ __forceinline__ void fma_n(float (&d)[N], const float (&a)[N], const float (&b)[N], const float (&c)[N]) {
+  if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) fma2(d[i], d[i + 1], a[i], a[i + 1], b[i], b[i + 1], c[i], c[i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) d[i] = fmaf(a[i], b[i], c[i]);
+  }
+}
+template <int N>
+__device__ __forceinline__ void mul_n(float (&d)[N], const float (&a)[N], const float (&b)[N]) {
+  if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) mul2(d[i], d[i + 1], a[i], a[i + 1], b[i], b[i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) d[i] = a[i] * b[i];
+  }
+}
+template <int N>
+__device__ __forceinline__ void add_n(float (&d)[N], const float (&a)[N], const float (&b)[N]) {
+  if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) add2(d[i], d[i + 1], a[i], a[i + 1], b[i], b[i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) d[i] = a[i] + b[i];
+  }
+}
+template <int N>
+__device__ __forceinline__ void fill_n(float (&d)[N], float v) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) d[i] = v;
+}
+
 // exp(g) - 1 for g in [-0.3, 0]: its power series up to g^7 (the next term is 5e-9 of the value).
 __device__ __forceinline__ float exp_minus_1(float g) {
   float p = 1.0f / 5040;

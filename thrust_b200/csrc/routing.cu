@@ -11,6 +11,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "model_common.cuh"
 
@@ -33,20 +34,36 @@ __device__ __forceinline__ int64_t id_at(const Ids& d, uint64_t row, uint32_t sl
   return d.bytes == 4 ? (int64_t)static_cast<const int32_t*>(d.ids)[i] : static_cast<const int64_t*>(d.ids)[i];
 }
 
-// The ids of rows [r0, r1) into a CTA's counters.
+// The ids of rows [r0, r1) into a CTA's counters. Eight ids a thread are on their way before the first is counted: a
+// CTA that waits for one after the other spends a memory latency on each.
 __device__ __forceinline__ void count_rows(const Ids& d, const uint8_t* mask, uint64_t r0, uint64_t r1, uint32_t experts,
                                            unsigned* counters) {
-  const uint64_t n = (r1 - r0) * d.k;
-  auto count = [&](auto i) {  // 32-bit indices where they suffice: a division of 64 bits costs more than the rest
-    const uint64_t row = r0 + i / (decltype(i))d.k;
-    if (mask && !mask[row]) return;
-    const int64_t id = id_at(d, row, (uint32_t)(i % (decltype(i))d.k));
-    if (id >= 0 && id < (int64_t)experts) atomicAdd(&counters[id], 1u);
-  };
-  if (n < (1ull << 31)) {
-    for (uint32_t i = threadIdx.x; i < (uint32_t)n; i += kRouteThreads) count(i);
-  } else {
-    for (uint64_t i = threadIdx.x; i < n; i += kRouteThreads) count(i);
+  constexpr int U = 8;
+  const bool dense = d.stride == d.k && mask == nullptr;
+  // pieces of rows whose ids are numbered in 32 bits: a division of 64 bits costs more than the rest
+  for (uint64_t at = r0; at < r1;) {
+    const uint64_t most = (1u << 30) / d.k + 1;
+    const uint64_t end = r1 - at < most ? r1 : at + most;
+    const uint32_t n = (uint32_t)((end - at) * d.k);
+    for (uint32_t i0 = threadIdx.x; i0 < n; i0 += U * kRouteThreads) {
+      int64_t id[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const uint32_t i = i0 + u * kRouteThreads;
+        id[u] = -1;
+        if (i >= n) continue;
+        if (dense) {
+          id[u] = id_at(d, at, i);
+        } else {
+          const uint32_t row = i / d.k;
+          if (mask == nullptr || mask[at + row]) id[u] = id_at(d, at + row, i - row * d.k);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (id[u] >= 0 && id[u] < (int64_t)experts) atomicAdd(&counters[id[u]], 1u);
+    }
+    at = end;
   }
 }
 
@@ -110,7 +127,8 @@ expert_counts_kernel(Ids ids, const uint8_t* mask, uint64_t rows, uint64_t rows_
 
 // ---- rows of logits over lanes ------------------------------------------------------------------------
 
-// A row over `lanes` (a power of two) lanes: element i of step j is expert (j * lanes + lane) * 8 + i.
+// A row over L (a power of two) lanes: element i of step j is expert (j * L + lane) * 8 + i. Places beyond the last expert
+// hold -inf, like disabled experts.
 template <typename T, int J>
 struct RowPack {
   Pack<T, 8> p[J];
@@ -123,56 +141,68 @@ __device__ __forceinline__ Pack<T, 8> load8(const char* base, uint64_t element) 
   for (int i = 0; i < (int)(sizeof(p) / 16); ++i) reinterpret_cast<uint4*>(&p)[i] = __ldcs(at + i);
   return p;
 }
-template <typename T, int J, bool VEC>
-__device__ __forceinline__ void load_row(const RowsOf& z, uint64_t row, uint32_t lanes, uint32_t lane, uint32_t experts,
+template <typename T, int J, int L, bool VEC>
+__device__ __forceinline__ void load_row(const RowsOf& z, uint64_t row, bool on, uint32_t lane, uint32_t experts,
                                          RowPack<T, J>& out) {
+  const T none = from_f32<T>(__int_as_float(0xff800000));
 #pragma unroll
   for (int j = 0; j < J; ++j) {
-    const uint32_t e = (j * lanes + lane) * 8;
+    const uint32_t e = (j * L + lane) * 8;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out.p[j].v[i] = none;
     if constexpr (VEC) {
-      if (e < experts) out.p[j] = load8<T>(z.data, row * z.row + e);
+      if (on && e < experts) out.p[j] = load8<T>(z.data, row * z.row + e);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (e + i < experts) out.p[j].v[i] = *reinterpret_cast<const T*>(z.data + (row * z.row + e + i) * sizeof(T));
+        if (on && e + i < experts) out.p[j].v[i] = *reinterpret_cast<const T*>(z.data + (row * z.row + e + i) * sizeof(T));
     }
   }
 }
-__device__ __forceinline__ float lanes_max(float v, uint32_t lanes) {
-  for (uint32_t off = 1; off < lanes; off *= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
+template <int L>
+__device__ __forceinline__ float lanes_max(float v) {
+#pragma unroll
+  for (int off = 1; off < L; off *= 2) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
   return v;
 }
-__device__ __forceinline__ float lanes_sum(float v, uint32_t lanes) {
-  for (uint32_t off = 1; off < lanes; off *= 2) v += __shfl_xor_sync(0xffffffffu, v, off);
+template <int L>
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+  for (int off = 1; off < L; off *= 2) v += __shfl_xor_sync(0xffffffffu, v, off);
   return v;
 }
-// Softmax of a row in 32 bits. -inf is a disabled expert; a row of nothing else has no probabilities (zeros).
-template <typename T, int J>
-__device__ __forceinline__ void softmax_row(const RowPack<T, J>& row, uint32_t lanes, uint32_t lane, uint32_t experts,
-                                            float (&p)[J * 8]) {
+// Softmax of a row in 32 bits: p[e] = e[e] * the value returned. A row of nothing but -inf has no probabilities: zero.
+template <typename T, int J, int L>
+__device__ __forceinline__ float softmax_row(const RowPack<T, J>& row, float (&e)[J * 8]) {
   const float none = __int_as_float(0xff800000);
   float top = none;
 #pragma unroll
   for (int j = 0; j < J; ++j)
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float z = (j * lanes + lane) * 8 + i < experts ? to_f32<T>(row.p[j].v[i]) : none;
-      p[j * 8 + i] = z;
-      top = fmaxf(top, z);
+      e[j * 8 + i] = to_f32<T>(row.p[j].v[i]);
+      top = fmaxf(top, e[j * 8 + i]);
     }
-  top = lanes_max(top, lanes);
+  top = lanes_max<L>(top);
+  float unit[J * 8], base[J * 8];
+  fill_n(unit, kLog2e);
+  fill_n(base, top == none ? 0.0f : -top);  // the difference first: logits near the end of the type's range stay in it
+  add_n(e, e, base);
+  mul_n(e, e, unit);
   float sum = 0.0f;
-  const float base = top == none ? 0.0f : top;
 #pragma unroll
   for (int i = 0; i < J * 8; ++i) {
-    p[i] = __expf(p[i] - base);
-    sum += p[i];
+    e[i] = exp2_fast(e[i]);
+    sum += e[i];
   }
-  sum = lanes_sum(sum, lanes);
-  const float scale = top == none && sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-  for (int i = 0; i < J * 8; ++i) p[i] *= scale;
+  sum = lanes_sum<L>(sum);
+  float scale;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(scale) : "f"(sum));  // the sum is 1 at least, or zero
+  return sum == 0.0f ? 0.0f : scale;
 }
+
+// Rows that a warp has on their way at once, for each of its row groups.
+template <int J> constexpr int kRowsAtOnce = J == 1 ? 4 : J == 2 ? 2 : 1;
 
 struct Spans {  // packed sequences over the rows, or one sequence
   const void* offsets;
@@ -205,7 +235,7 @@ struct BalanceArgs {
   const uint8_t* mask;
   Spans spans;
   uint64_t rows_of_cta;
-  uint32_t experts, lanes;
+  uint32_t experts;
   float scale;  // fixed point: one is `scale`
   float* loss;
   uint64_t* counts;
@@ -218,7 +248,7 @@ struct BalanceArgs {
   unsigned* poison;            // [sequences] a probability was NaN
 };
 
-template <typename T, int J, bool VEC>
+template <typename T, int J, int L, bool VEC>
 __global__ void __launch_bounds__(kRouteThreads) balance_kernel(BalanceArgs a) {
   __shared__ unsigned s_count[kMaxBalanceExperts];
   __shared__ float s_sum[kRouteWarps][J * 256];
@@ -226,7 +256,8 @@ __global__ void __launch_bounds__(kRouteThreads) balance_kernel(BalanceArgs a) {
   __shared__ float s_loss[kRouteWarps];
   __shared__ unsigned s_last;
   const unsigned lane = lane_id(), warp = threadIdx.x / kWarp;
-  const uint32_t lanes = a.lanes, groups = kWarp / lanes, in_row = lane % lanes, group = lane / lanes;
+  constexpr uint32_t groups = kWarp / L;
+  const uint32_t in_row = lane % L, group = lane / L;
   const uint64_t r0 = blockIdx.x * a.rows_of_cta, r1 = min(r0 + a.rows_of_cta, a.spans.rows);
 
   if (blockIdx.x == 0 && a.spans.bytes) {  // empty sequences belong to no CTA's rows; bad offsets are reported
@@ -256,29 +287,34 @@ __global__ void __launch_bounds__(kRouteThreads) balance_kernel(BalanceArgs a) {
 
     float acc[J * 8] = {};
     unsigned kept = 0;
-    for (uint64_t base = from + warp * groups; base < to; base += kRouteWarps * groups) {
-      const uint64_t row = base + group;
-      const bool on = row < to && (a.mask == nullptr || a.mask[row]);
-      RowPack<T, J> pack = {};
-      if (on) load_row<T, J, VEC>(a.z, row, lanes, in_row, a.experts, pack);
-      float p[J * 8];
-      softmax_row<T, J>(pack, lanes, in_row, a.experts, p);
-      if (on) {
-        kept += in_row == 0;
+    constexpr int U = kRowsAtOnce<J>;
+    for (uint64_t base = from + warp * groups; base < to; base += U * kRouteWarps * groups) {
+      RowPack<T, J> pack[U];
+      bool on[U];
 #pragma unroll
-        for (int i = 0; i < J * 8; ++i) acc[i] += p[i];
+      for (int u = 0; u < U; ++u) {
+        const uint64_t row = base + u * kRouteWarps * groups + group;
+        on[u] = row < to && (a.mask == nullptr || a.mask[row]);
+        load_row<T, J, L, VEC>(a.z, row, on[u], in_row, a.experts, pack[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {  // rows that do not count hold -inf alone
+        float e[J * 8], scale[J * 8];
+        fill_n(scale, softmax_row<T, J, L>(pack[u], e));
+        fma_n(acc, e, scale, acc);
+        kept += on[u] && in_row == 0;
       }
     }
     // over the row groups of a warp, then over the warps, in a fixed order
 #pragma unroll
     for (int i = 0; i < J * 8; ++i)
-      for (uint32_t off = lanes; off < kWarp; off *= 2) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], off);
+      for (int off = L; off < kWarp; off *= 2) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], off);
     for (int off = 16; off > 0; off /= 2) kept += __shfl_xor_sync(0xffffffffu, kept, off);
     if (group == 0) {
 #pragma unroll
       for (int j = 0; j < J; ++j)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s_sum[warp][(j * lanes + in_row) * 8 + i] = acc[j * 8 + i];
+        for (int i = 0; i < 8; ++i) s_sum[warp][(j * L + in_row) * 8 + i] = acc[j * 8 + i];
     }
     if (lane == 0) s_tokens[warp] = kept;
     __syncthreads();
@@ -314,7 +350,7 @@ __global__ void __launch_bounds__(kRouteThreads) balance_kernel(BalanceArgs a) {
         a.weights[s * a.experts + e] = w;
         part += w * (float)((double)__ldcg(&a.sums[s * a.experts + e]) / (double)a.scale);
       }
-      part = lanes_sum(part, kWarp);
+      part = lanes_sum<kWarp>(part);
       if (lane == 0) s_loss[warp] = part;
       __syncthreads();
       if (threadIdx.x == 0) {
@@ -334,61 +370,78 @@ struct BalanceBackArgs {
   const uint8_t* mask;
   Spans spans;
   uint64_t rows_of_warp;
-  uint32_t experts, lanes;
+  uint32_t experts;
 };
 
-template <typename T, int J, bool VEC>
+template <typename T, int J, int L, bool VEC>
 __global__ void __launch_bounds__(kRouteThreads) balance_backward_kernel(BalanceBackArgs a) {
   const unsigned lane = lane_id();
-  const uint32_t lanes = a.lanes, groups = kWarp / lanes, in_row = lane % lanes, group = lane / lanes;
+  constexpr uint32_t groups = kWarp / L;
+  const uint32_t in_row = lane % L, group = lane / L;
   const uint64_t warp = blockIdx.x * (uint64_t)kRouteWarps + threadIdx.x / kWarp;
   const uint64_t r0 = warp * a.rows_of_warp, r1 = min(r0 + a.rows_of_warp, a.spans.rows);
   uint64_t s = ~0ull, end = 0;  // the sequence whose weights are held, and its end
   float w[J * 8] = {};
   float scale = 0.0f;
-  for (uint64_t base = r0; base < r1; base += groups) {
-    const uint64_t row = base + group;
-    const bool valid = row < r1;
-    if (valid && (s == ~0ull || row >= end)) {
-      if (s == ~0ull) s = sequence_of(a.spans, row);
-      while (s < a.spans.sequences && row >= begin_of(a.spans, s + 1)) ++s;
-      end = s < a.spans.sequences ? begin_of(a.spans, s + 1) : a.spans.rows;
-      const bool some = s < a.spans.sequences && row >= begin_of(a.spans, s);
-      scale = some ? a.dloss[s] : 0.0f;
+  constexpr int U = kRowsAtOnce<J>;
+  for (uint64_t at = r0; at < r1; at += U * groups) {
+    RowPack<T, J> pack[U];
+    bool on[U];
 #pragma unroll
-      for (int j = 0; j < J; ++j)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint32_t e = (j * lanes + in_row) * 8 + i;
-          w[j * 8 + i] = some && e < a.experts ? a.weights[s * a.experts + e] : 0.0f;
-        }
+    for (int u = 0; u < U; ++u) {
+      const uint64_t row = at + u * groups + group;
+      on[u] = row < r1 && (a.mask == nullptr || a.mask[row]);
+      load_row<T, J, L, VEC>(a.z, row, on[u], in_row, a.experts, pack[u]);
     }
-    const bool on = valid && s < a.spans.sequences && (a.mask == nullptr || a.mask[row]);
-    RowPack<T, J> pack = {};
-    if (on) load_row<T, J, VEC>(a.z, row, lanes, in_row, a.experts, pack);
-    float p[J * 8];
-    softmax_row<T, J>(pack, lanes, in_row, a.experts, p);
-    float dot = 0.0f;
 #pragma unroll
-    for (int i = 0; i < J * 8; ++i) dot = fmaf(p[i], w[i], dot);
-    dot = lanes_sum(dot, lanes);
-    if (!valid) continue;
+    for (int u = 0; u < U; ++u) {
+      const uint64_t row = at + u * groups + group;
+      const bool valid = row < r1;
+      if (valid && (s == ~0ull || row >= end)) {
+        if (s == ~0ull) s = sequence_of(a.spans, row);
+        while (s < a.spans.sequences && row >= begin_of(a.spans, s + 1)) ++s;
+        end = s < a.spans.sequences ? begin_of(a.spans, s + 1) : a.spans.rows;
+        const bool some = s < a.spans.sequences && row >= begin_of(a.spans, s);
+        scale = some ? a.dloss[s] : 0.0f;
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-      const uint32_t e = (j * lanes + in_row) * 8;
-      Pack<T, 8> out;
+        for (int j = 0; j < J; ++j)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) out.v[i] = from_f32<T>(on ? scale * p[j * 8 + i] * (w[j * 8 + i] - dot) : 0.0f);
-      if constexpr (VEC) {
-        if (e < a.experts) {
-          uint4* at = reinterpret_cast<uint4*>(a.dz.data + (row * a.dz.row + e) * sizeof(T));
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t e = (j * L + in_row) * 8 + i;
+            w[j * 8 + i] = some && e < a.experts ? a.weights[s * a.experts + e] : 0.0f;
+          }
+      }
+      const bool kept = on[u] && s < a.spans.sequences;
+      float e[J * 8];
+      const float share = softmax_row<T, J, L>(pack[u], e);
+      float dot = 0.0f;
 #pragma unroll
-          for (int i = 0; i < (int)(sizeof(out) / 16); ++i) at[i] = reinterpret_cast<const uint4*>(&out)[i];
+      for (int i = 0; i < J * 8; ++i) dot = fmaf(e[i], w[i], dot);
+      dot = lanes_sum<L>(dot) * share;
+      float less[J * 8], factor[J * 8], d[J * 8];
+      fill_n(less, -dot);
+      fill_n(factor, kept ? scale * share : 0.0f);
+      add_n(d, w, less);
+      mul_n(e, e, factor);
+      mul_n(d, d, e);
+      if (!valid) continue;
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const uint32_t first = (j * L + in_row) * 8;
+        Pack<T, 8> out;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) out.v[i] = from_f32<T>(d[j * 8 + i]);
+        if constexpr (VEC) {
+          if (first < a.experts) {
+            uint4* to = reinterpret_cast<uint4*>(a.dz.data + (row * a.dz.row + first) * sizeof(T));
+#pragma unroll
+            for (int i = 0; i < (int)(sizeof(out) / 16); ++i) to[i] = reinterpret_cast<const uint4*>(&out)[i];
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (first + i < a.experts) *reinterpret_cast<T*>(a.dz.data + (row * a.dz.row + first + i) * sizeof(T)) = out.v[i];
         }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (e + i < a.experts) *reinterpret_cast<T*>(a.dz.data + (row * a.dz.row + e + i) * sizeof(T)) = out.v[i];
       }
     }
   }
@@ -399,22 +452,27 @@ uint32_t lanes_of(uint32_t experts) {  // lanes that share a row
   while (lanes < kWarp && lanes * 8 < experts) lanes *= 2;
   return lanes;
 }
-// Calls f(type tag, J, VEC) for a row of this type and size.
+// Calls f(type tag, J, L, VEC) for a row of this type and size.
 template <typename F>
 int by_row(int dtype, uint32_t experts, bool vec, F f) {
-  auto with = [&](auto tag) -> int {
-    using T = decltype(tag);
-    auto sized = [&](auto v) -> int {
-      if (experts <= 256) return f(tag, std::integral_constant<int, 1>{}, v);
-      if (experts <= 512) return f(tag, std::integral_constant<int, 2>{}, v);
-      return f(tag, std::integral_constant<int, 4>{}, v);
-    };
-    (void)sizeof(T);
-    return vec ? sized(std::true_type{}) : sized(std::false_type{});
+  using std::integral_constant;
+  auto sized = [&](auto tag, auto v) -> int {
+    constexpr integral_constant<int, 1> one{};
+    if (experts > 512) return f(tag, integral_constant<int, 4>{}, integral_constant<int, 32>{}, v);
+    if (experts > 256) return f(tag, integral_constant<int, 2>{}, integral_constant<int, 32>{}, v);
+    switch (lanes_of(experts)) {
+      case 1: return f(tag, one, integral_constant<int, 1>{}, v);
+      case 2: return f(tag, one, integral_constant<int, 2>{}, v);
+      case 4: return f(tag, one, integral_constant<int, 4>{}, v);
+      case 8: return f(tag, one, integral_constant<int, 8>{}, v);
+      case 16: return f(tag, one, integral_constant<int, 16>{}, v);
+      default: return f(tag, one, integral_constant<int, 32>{}, v);
+    }
   };
-  if (dtype == TB200_F32) return with(float{});
-  if (dtype == TB200_F16) return with(__half{});
-  return with(__nv_bfloat16{});
+  auto typed = [&](auto tag) -> int { return vec ? sized(tag, std::true_type{}) : sized(tag, std::false_type{}); };
+  if (dtype == TB200_F32) return typed(float{});
+  if (dtype == TB200_F16) return typed(__half{});
+  return typed(__nv_bfloat16{});
 }
 
 int check_ids(const void* ids, uint64_t rows, uint32_t k, uint64_t stride, int bytes) {
@@ -504,7 +562,6 @@ extern "C" int tb200_balance_loss(void* d_temp, size_t* temp_bytes, const tb200_
   a.mask = d_mask;
   a.spans = Spans{d_offsets, offset_bytes, sequences, rows};
   a.experts = experts;
-  a.lanes = lanes_of(experts);
   int bits = 62;  // a sum of all rows stays below 2^62
   while (bits > 1 && (rows >> (62 - bits)) != 0) --bits;
   a.scale = ldexpf(1.0f, bits);
@@ -517,15 +574,15 @@ extern "C" int tb200_balance_loss(void* d_temp, size_t* temp_bytes, const tb200_
   a.tokens = a.totals + cells;
   a.done = reinterpret_cast<unsigned*>(a.tokens + sequences);
   a.poison = a.done + sequences;
-  // rows of a CTA: enough to be worth its share of the sums, few enough for two waves of CTAs
-  const uint64_t least = 4ull * kRouteWarps * (kWarp / a.lanes);
-  uint64_t per = (rows + 2ull * sms - 1) / (2ull * sms);
+  // rows of a CTA: enough to be worth its share of the sums, few enough for the CTAs that fit
+  const uint64_t least = (uint64_t)kRouteWarps * (kWarp / lanes_of(experts));
+  uint64_t per = (rows + 4ull * sms - 1) / (4ull * sms);
   if (per < least) per = least;
   a.rows_of_cta = per;
   const unsigned grid = (unsigned)((rows + per - 1) / per);
   const bool vec = experts % 8 == 0 && rows_on(a.z, tb, 16);
-  return by_row(dtype, experts, vec, [&](auto tag, auto j, auto v) -> int {
-    balance_kernel<decltype(tag), decltype(j)::value, decltype(v)::value><<<grid, kRouteThreads, 0, stream>>>(a);
+  return by_row(dtype, experts, vec, [&](auto tag, auto j, auto l, auto v) -> int {
+    balance_kernel<decltype(tag), decltype(j)::value, decltype(l)::value, decltype(v)::value><<<grid, kRouteThreads, 0, stream>>>(a);
     trace_mark(stream, kTraceBalanceLoss);
     return (int)cudaGetLastError();
   });
@@ -554,14 +611,13 @@ extern "C" int tb200_balance_loss_backward(const tb200_rows* logits, int dtype, 
   a.mask = d_mask;
   a.spans = Spans{d_offsets, offset_bytes, sequences, rows};
   a.experts = experts;
-  a.lanes = lanes_of(experts);
-  a.rows_of_warp = 4ull * (kWarp / a.lanes);
+  a.rows_of_warp = (experts <= 256 ? 4ull : experts <= 512 ? 4ull : 2ull) * (kWarp / lanes_of(experts));
   const uint64_t warps = (rows + a.rows_of_warp - 1) / a.rows_of_warp;
   const uint64_t grid = (warps + kRouteWarps - 1) / kRouteWarps;
   if (grid > 0x7fffffffull) return TB200_ERR_UNSUPPORTED;
   const bool vec = experts % 8 == 0 && rows_on(a.z, tb, 16) && rows_on(a.dz, tb, 16);
-  return by_row(dtype, experts, vec, [&](auto tag, auto j, auto v) -> int {
-    balance_backward_kernel<decltype(tag), decltype(j)::value, decltype(v)::value>
+  return by_row(dtype, experts, vec, [&](auto tag, auto j, auto l, auto v) -> int {
+    balance_backward_kernel<decltype(tag), decltype(j)::value, decltype(l)::value, decltype(v)::value>
         <<<(unsigned)grid, kRouteThreads, 0, stream>>>(a);
     trace_mark(stream, kTraceBalanceLoss);
     return (int)cudaGetLastError();
