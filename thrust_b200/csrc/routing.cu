@@ -202,7 +202,7 @@ __device__ __forceinline__ float softmax_row(const RowPack<T, J>& row, float (&e
 }
 
 // Rows that a warp has on their way at once, for each of its row groups.
-template <int J> constexpr int kRowsAtOnce = J == 1 ? 4 : J == 2 ? 2 : 1;
+template <typename T, int J> constexpr int kRowsAtOnce = J == 1 ? (sizeof(T) == 2 ? 3 : 2) : 1;
 
 struct Spans {  // packed sequences over the rows, or one sequence
   const void* offsets;
@@ -249,7 +249,7 @@ struct BalanceArgs {
 };
 
 template <typename T, int J, int L, bool VEC>
-__global__ void __launch_bounds__(kRouteThreads) balance_kernel(BalanceArgs a) {
+__global__ void __launch_bounds__(kRouteThreads, J == 1 ? 3 : 1) balance_kernel(BalanceArgs a) {
   __shared__ unsigned s_count[kMaxBalanceExperts];
   __shared__ float s_sum[kRouteWarps][J * 256];
   __shared__ unsigned s_tokens[kRouteWarps];
@@ -282,27 +282,36 @@ __global__ void __launch_bounds__(kRouteThreads) balance_kernel(BalanceArgs a) {
     const uint64_t from = max(begin, r0), to = min(end, r1);
     if (from >= to) continue;
     for (uint32_t e = threadIdx.x; e < a.experts; e += kRouteThreads) s_count[e] = 0;
-    __syncthreads();
-    count_rows(a.ids, a.mask, from, to, a.experts, s_count);
-
     float acc[J * 8] = {};
     unsigned kept = 0;
-    constexpr int U = kRowsAtOnce<J>;
-    for (uint64_t base = from + warp * groups; base < to; base += U * kRouteWarps * groups) {
-      RowPack<T, J> pack[U];
-      bool on[U];
+    // the next rows are on their way while these are worked on
+    constexpr int U = kRowsAtOnce<T, J>;
+    RowPack<T, J> pack[U], ahead[U];
+    bool on[U], on_ahead[U];
+    auto fetch = [&](uint64_t base, RowPack<T, J>(&into)[U], bool(&counts)[U]) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const uint64_t row = base + u * kRouteWarps * groups + group;
-        on[u] = row < to && (a.mask == nullptr || a.mask[row]);
-        load_row<T, J, L, VEC>(a.z, row, on[u], in_row, a.experts, pack[u]);
+        counts[u] = row < to && (a.mask == nullptr || a.mask[row]);
+        load_row<T, J, L, VEC>(a.z, row, counts[u], in_row, a.experts, into[u]);
       }
+    };
+    fetch(from + warp * groups, pack, on);
+    __syncthreads();
+    count_rows(a.ids, a.mask, from, to, a.experts, s_count);
+    for (uint64_t base = from + warp * groups; base < to; base += U * kRouteWarps * groups) {
+      fetch(base + U * kRouteWarps * groups, ahead, on_ahead);
 #pragma unroll
       for (int u = 0; u < U; ++u) {  // rows that do not count hold -inf alone
         float e[J * 8], scale[J * 8];
         fill_n(scale, softmax_row<T, J, L>(pack[u], e));
         fma_n(acc, e, scale, acc);
         kept += on[u] && in_row == 0;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        pack[u] = ahead[u];
+        on[u] = on_ahead[u];
       }
     }
     // over the row groups of a warp, then over the warps, in a fixed order
@@ -374,7 +383,7 @@ struct BalanceBackArgs {
 };
 
 template <typename T, int J, int L, bool VEC>
-__global__ void __launch_bounds__(kRouteThreads) balance_backward_kernel(BalanceBackArgs a) {
+__global__ void __launch_bounds__(kRouteThreads, J == 1 ? 3 : 1) balance_backward_kernel(BalanceBackArgs a) {
   const unsigned lane = lane_id();
   constexpr uint32_t groups = kWarp / L;
   const uint32_t in_row = lane % L, group = lane / L;
@@ -383,16 +392,20 @@ __global__ void __launch_bounds__(kRouteThreads) balance_backward_kernel(Balance
   uint64_t s = ~0ull, end = 0;  // the sequence whose weights are held, and its end
   float w[J * 8] = {};
   float scale = 0.0f;
-  constexpr int U = kRowsAtOnce<J>;
-  for (uint64_t at = r0; at < r1; at += U * groups) {
-    RowPack<T, J> pack[U];
-    bool on[U];
+  constexpr int U = kRowsAtOnce<T, J>;
+  RowPack<T, J> pack[U], ahead[U];
+  bool on[U], on_ahead[U];
+  auto fetch = [&](uint64_t at, RowPack<T, J>(&into)[U], bool(&counts)[U]) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const uint64_t row = at + u * groups + group;
-      on[u] = row < r1 && (a.mask == nullptr || a.mask[row]);
-      load_row<T, J, L, VEC>(a.z, row, on[u], in_row, a.experts, pack[u]);
+      counts[u] = row < r1 && (a.mask == nullptr || a.mask[row]);
+      load_row<T, J, L, VEC>(a.z, row, counts[u], in_row, a.experts, into[u]);
     }
+  };
+  fetch(r0, pack, on);
+  for (uint64_t at = r0; at < r1; at += U * groups) {
+    fetch(at + U * groups, ahead, on_ahead);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const uint64_t row = at + u * groups + group;
@@ -444,8 +457,15 @@ __global__ void __launch_bounds__(kRouteThreads) balance_backward_kernel(Balance
         }
       }
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      pack[u] = ahead[u];
+      on[u] = on_ahead[u];
+    }
   }
 }
+
+template <int WHICH, typename... T> struct Tag {};
 
 uint32_t lanes_of(uint32_t experts) {  // lanes that share a row
   uint32_t lanes = 1;
@@ -574,15 +594,17 @@ extern "C" int tb200_balance_loss(void* d_temp, size_t* temp_bytes, const tb200_
   a.tokens = a.totals + cells;
   a.done = reinterpret_cast<unsigned*>(a.tokens + sequences);
   a.poison = a.done + sequences;
-  // rows of a CTA: enough to be worth its share of the sums, few enough for the CTAs that fit
-  const uint64_t least = (uint64_t)kRouteWarps * (kWarp / lanes_of(experts));
-  uint64_t per = (rows + 4ull * sms - 1) / (4ull * sms);
-  if (per < least) per = least;
-  a.rows_of_cta = per;
-  const unsigned grid = (unsigned)((rows + per - 1) / per);
   const bool vec = experts % 8 == 0 && rows_on(a.z, tb, 16);
   return by_row(dtype, experts, vec, [&](auto tag, auto j, auto l, auto v) -> int {
-    balance_kernel<decltype(tag), decltype(j)::value, decltype(l)::value, decltype(v)::value><<<grid, kRouteThreads, 0, stream>>>(a);
+    auto kernel = balance_kernel<decltype(tag), decltype(j)::value, decltype(l)::value, decltype(v)::value>;
+    int per_sm = 0;
+    const int rc = resident_ctas<Tag<0, decltype(tag), decltype(j), decltype(l), decltype(v)>>(kernel, kRouteThreads, 0, &per_sm);
+    if (rc) return rc;
+    // as many CTAs as fit, each with one row at least for every row group of its warps
+    const uint64_t slots = (uint64_t)per_sm * sms, least = (uint64_t)kRouteWarps * (kWarp / decltype(l)::value);
+    a.rows_of_cta = (rows + slots - 1) / slots;
+    if (a.rows_of_cta < least) a.rows_of_cta = least;
+    kernel<<<(unsigned)((rows + a.rows_of_cta - 1) / a.rows_of_cta), kRouteThreads, 0, stream>>>(a);
     trace_mark(stream, kTraceBalanceLoss);
     return (int)cudaGetLastError();
   });
@@ -611,14 +633,21 @@ extern "C" int tb200_balance_loss_backward(const tb200_rows* logits, int dtype, 
   a.mask = d_mask;
   a.spans = Spans{d_offsets, offset_bytes, sequences, rows};
   a.experts = experts;
-  a.rows_of_warp = (experts <= 256 ? 4ull : experts <= 512 ? 4ull : 2ull) * (kWarp / lanes_of(experts));
-  const uint64_t warps = (rows + a.rows_of_warp - 1) / a.rows_of_warp;
-  const uint64_t grid = (warps + kRouteWarps - 1) / kRouteWarps;
-  if (grid > 0x7fffffffull) return TB200_ERR_UNSUPPORTED;
+  int sms = 0;
+  const int rc = sm_count_of_device(&sms);
+  if (rc) return rc;
   const bool vec = experts % 8 == 0 && rows_on(a.z, tb, 16) && rows_on(a.dz, tb, 16);
   return by_row(dtype, experts, vec, [&](auto tag, auto j, auto l, auto v) -> int {
-    balance_backward_kernel<decltype(tag), decltype(j)::value, decltype(l)::value, decltype(v)::value>
-        <<<(unsigned)grid, kRouteThreads, 0, stream>>>(a);
+    auto kernel = balance_backward_kernel<decltype(tag), decltype(j)::value, decltype(l)::value, decltype(v)::value>;
+    int per_sm = 0;
+    const int rc = resident_ctas<Tag<1, decltype(tag), decltype(j), decltype(l), decltype(v)>>(kernel, kRouteThreads, 0, &per_sm);
+    if (rc) return rc;
+    // as many warps as fit, each with one row at least for every row group
+    const uint64_t slots = (uint64_t)per_sm * sms * kRouteWarps, least = kWarp / decltype(l)::value;
+    a.rows_of_warp = (rows + slots - 1) / slots;
+    if (a.rows_of_warp < least) a.rows_of_warp = least;
+    const uint64_t warps = (rows + a.rows_of_warp - 1) / a.rows_of_warp;
+    kernel<<<(unsigned)((warps + kRouteWarps - 1) / kRouteWarps), kRouteThreads, 0, stream>>>(a);
     trace_mark(stream, kTraceBalanceLoss);
     return (int)cudaGetLastError();
   });
