@@ -42,7 +42,7 @@ def _load() -> C.CDLL:
             "(thrust_b200 has no CPU or PyTorch fallback)")
     lib = C.CDLL(str(_LIB_PATH))
     vp, sz, u64, i32, u32 = C.c_void_p, C.c_size_t, C.c_uint64, C.c_int, C.c_uint32
-    psz, rows = C.POINTER(C.c_size_t), C.POINTER(Rows)
+    psz, rows = C.POINTER(C.c_size_t), vp  # rows: address of a tb200_rows
     sigs = {
         "tb200_version": ([], i32),
         "tb200_error_string": ([i32], C.c_char_p),

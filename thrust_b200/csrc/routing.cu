@@ -260,6 +260,14 @@ __global__ void __launch_bounds__(kRouteThreads, J == 1 ? 3 : 1) balance_kernel(
   const uint32_t in_row = lane % L, group = lane / L;
   const uint64_t r0 = blockIdx.x * a.rows_of_cta, r1 = min(r0 + a.rows_of_cta, a.spans.rows);
 
+  if (gridDim.x == 1) {  // the scratch is not cleared for a single CTA
+    unsigned* words = reinterpret_cast<unsigned*>(a.sums);
+    const uint64_t cells = a.spans.sequences * a.experts;
+    for (uint64_t i = threadIdx.x; i < cells * 4 + a.spans.sequences * 4; i += kRouteThreads) words[i] = 0;
+    if (threadIdx.x == 0) a.hdr->status = TB200_OK;
+    __threadfence();
+    __syncthreads();
+  }
   if (blockIdx.x == 0 && a.spans.bytes) {  // empty sequences belong to no CTA's rows; bad offsets are reported
     bool bad = threadIdx.x == 0 && raw_offset(a.spans, a.spans.sequences) != (int64_t)begin_of(a.spans, a.spans.sequences);
     for (uint64_t s = threadIdx.x; s < a.spans.sequences; s += kRouteThreads) {
@@ -566,8 +574,8 @@ extern "C" int tb200_balance_loss(void* d_temp, size_t* temp_bytes, const tb200_
   if (sequences && (!d_loss || !d_counts || !d_weights)) return TB200_ERR_INVALID_ARGUMENT;
   if (reinterpret_cast<uintptr_t>(d_counts) % 8 ||
       (reinterpret_cast<uintptr_t>(d_loss) | reinterpret_cast<uintptr_t>(d_weights)) % 4) return TB200_ERR_INVALID_ARGUMENT;
-  TB200_CUDA_TRY(cudaMemsetAsync(d_temp, 0, need, stream));
   if (rows == 0 || sequences == 0) {
+    TB200_CUDA_TRY(cudaMemsetAsync(d_temp, 0, kHeaderBytes, stream));
     if (sequences == 0) return TB200_OK;
     TB200_CUDA_TRY(cudaMemsetAsync(d_loss, 0, sequences * sizeof(float), stream));
     TB200_CUDA_TRY(cudaMemsetAsync(d_counts, 0, cells * sizeof(uint64_t), stream));
@@ -604,7 +612,9 @@ extern "C" int tb200_balance_loss(void* d_temp, size_t* temp_bytes, const tb200_
     const uint64_t slots = (uint64_t)per_sm * sms, least = (uint64_t)kRouteWarps * (kWarp / decltype(l)::value);
     a.rows_of_cta = (rows + slots - 1) / slots;
     if (a.rows_of_cta < least) a.rows_of_cta = least;
-    kernel<<<(unsigned)((rows + a.rows_of_cta - 1) / a.rows_of_cta), kRouteThreads, 0, stream>>>(a);
+    const unsigned grid = (unsigned)((rows + a.rows_of_cta - 1) / a.rows_of_cta);
+    if (grid > 1) TB200_CUDA_TRY(cudaMemsetAsync(d_temp, 0, need, stream));
+    kernel<<<grid, kRouteThreads, 0, stream>>>(a);
     trace_mark(stream, kTraceBalanceLoss);
     return (int)cudaGetLastError();
   });

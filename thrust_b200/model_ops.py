@@ -14,20 +14,44 @@ from typing import Optional, Tuple
 import torch
 
 from . import _capi as capi
-from .algorithms import _On, _finish, _stream, _temp
 
 _FLOATS = {torch.float32: capi.F32, torch.float16: capi.F16, torch.bfloat16: capi.BF16}
 _INDEX_BYTES = {torch.int32: 4, torch.int64: 8}
 
+# A decoding step makes these calls for a few microseconds of work, so what they cost on the host is kept small: tensors
+# are asked for little, arrays of rows go over as plain words, the current device is looked at only where there are
+# several, and the current stream is asked for as a number.
+_several_devices = lru_cache(maxsize=1)(lambda: torch.cuda.device_count() > 1)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
-def _require_cuda(device, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError(f"{name} must be a CUDA tensor (thrust_b200 has no CPU path)")
-        if t.device != device:
-            raise ValueError(f"{name} lies on {t.device}, not on {device}")
+
+def _call(function, what: str, index: int, *args) -> None:
+    if _several_devices() and torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            rc = function(*args)
+    else:
+        rc = function(*args)
+    if rc:
+        capi.check(rc, what)
+
+
+def _status(temp: torch.Tensor, stream: int, what: str, index: int, sync: bool) -> None:
+    if sync:
+        _call(capi.lib.tb200_temp_status, what, index, temp.data_ptr(), stream)
+
+
+def _device_of(name: str, t: torch.Tensor) -> int:
+    index = t.get_device()
+    if index < 0:
+        raise ValueError(f"{name} must be a CUDA tensor (thrust_b200 has no CPU path)")
+    return index
+
+
+def _same_device(index: int, name: str, t: Optional[torch.Tensor]) -> None:
+    if t is not None and t.get_device() != index:
+        _device_of(name, t)
+        raise ValueError(f"{name} lies on {t.device}, not on cuda:{index}")
 
 
 def _float_code(t: torch.Tensor, name: str) -> int:
@@ -37,18 +61,36 @@ def _float_code(t: torch.Tensor, name: str) -> int:
         raise TypeError(f"{name} must be float32, float16 or bfloat16, not {t.dtype}") from None
 
 
-def _rows(t: torch.Tensor, name: str) -> capi.Rows:
-    """A [rows, channels] or [sequences, rows, channels] tensor whose channels are adjacent, by its strides."""
+def _types(x: torch.Tensor, name: str, gate: torch.Tensor) -> Tuple[int, int]:
+    xd, gd = _float_code(x, name), _float_code(gate, "gate")
+    if gd != xd and gd != capi.F32:
+        raise TypeError(f"gate must have the type of {name} or float32")
+    return xd, gd
+
+
+def _rows(t: torch.Tensor, name: str) -> Tuple[int, int, int]:
+    """A [rows, channels] or [sequences, rows, channels] tensor with adjacent channels, as the words of a tb200_rows."""
     stride = t.stride()
     if stride[-1] != 1 and t.shape[-1] > 1 and t.numel():
         raise ValueError(f"the channels of {name} must be adjacent in memory (its last stride is {stride[-1]})")
-    return capi.Rows(t.data_ptr(), stride[-2], stride[0] if t.dim() == 3 else 0)
+    return t.data_ptr(), stride[-2], stride[0] if len(stride) == 3 else 0
+
+
+class _Arrays:
+    """Several tb200_rows one behind the other; at[i] is the address of the i-th."""
+    __slots__ = ("words", "at")
+
+    def __init__(self, *rows):
+        flat = [w for r in rows for w in r]
+        self.words = (C.c_uint64 * len(flat))(*flat)
+        base = C.addressof(self.words)
+        self.at = [base + 24 * i for i in range(len(rows))]
 
 
 def _states(t: Optional[torch.Tensor], shape, name: str) -> Optional[int]:
     if t is None:
         return None
-    if t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous():
+    if t.dtype != torch.float32 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous float32 tensor of shape {list(shape)}")
     return t.data_ptr()
 
@@ -61,23 +103,22 @@ def _offsets(t: Optional[torch.Tensor]) -> Tuple[int, Optional[int]]:
     return _INDEX_BYTES[t.dtype], t.data_ptr()
 
 
-def _shape(x: torch.Tensor, gate: torch.Tensor, offsets: Optional[torch.Tensor], log_gate: bool, fill: bool, name: str):
-    """(shape structure, sequences) of a recurrence over x with these gates."""
-    packed = offsets is not None
-    if x.dim() != (2 if packed else 3):
-        raise ValueError(f"{name} must be [rows, channels] with offsets, [sequences, rows, channels] without")
-    if gate.shape[:-1] != x.shape[:-1] or gate.dim() != x.dim():
-        raise ValueError(f"gate must have a row for each row of {name}")
-    channels, heads = x.shape[-1], gate.shape[-1]
-    if channels == 0 or heads == 0 or channels % heads:
-        raise ValueError("a row must have a gate for each channel, or for each group of channels / gates neighbours")
-    xd, gd = _float_code(x, name), _float_code(gate, "gate")
-    if gd != xd and gd != capi.F32:
-        raise TypeError(f"gate must have the type of {name} or float32")
-    obytes, optr = _offsets(offsets)
-    sequences = offsets.numel() - 1 if packed else x.shape[0]
-    return capi.RecurrenceShape(sequences, x.shape[-2], channels, heads, xd, gd, int(bool(log_gate)), obytes,
-                                int(fill)), sequences, optr
+def _empty_like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
+def _output(out: Optional[torch.Tensor], like: torch.Tensor, name: str) -> torch.Tensor:
+    if out is None:
+        return _empty_like(like)
+    if out.shape != like.shape or out.dtype != like.dtype:
+        raise ValueError(f"out must have the shape and type of {name}")
+    return out
+
+
+def _scratch(need: int, like: torch.Tensor, temp: Optional[torch.Tensor]) -> torch.Tensor:
+    if temp is not None and temp.numel() >= need:
+        return temp
+    return like.new_empty((need,), dtype=torch.uint8)
 
 
 @lru_cache(maxsize=512)
@@ -89,13 +130,23 @@ def _recurrence_bytes(back: bool, *dims) -> int:
     else:
         rc = capi.lib.tb200_linear_recurrence(None, C.byref(need), C.byref(s), *(None,) * 7)
     capi.check(rc, "tb200_linear_recurrence(size)")
-    return need.value
+    return max(need.value, 256)
 
 
-def _scratch(back: bool, s, device, temp: Optional[torch.Tensor]) -> torch.Tensor:
-    need = _recurrence_bytes(back, s.sequences, s.rows, s.channels, s.heads, s.dtype, s.gate_dtype, s.log_gate,
-                             s.offset_bytes, s.fill_outside)
-    return _temp(need, device) if temp is None or temp.numel() < need else temp
+def _shape(x: torch.Tensor, gate: torch.Tensor, offsets: Optional[torch.Tensor], log_gate: bool, fill: bool, name: str):
+    """(the words of the shape, address of the offsets) of a recurrence over x with these gates."""
+    xs, gs = x.shape, gate.shape
+    if len(xs) != (3 if offsets is None else 2):
+        raise ValueError(f"{name} must be [rows, channels] with offsets, [sequences, rows, channels] without")
+    if gs[:-1] != xs[:-1] or len(gs) != len(xs):
+        raise ValueError(f"gate must have a row for each row of {name}")
+    channels, heads = xs[-1], gs[-1]
+    if channels == 0 or heads == 0 or channels % heads:
+        raise ValueError("a row must have a gate for each channel, or for each group of channels / gates neighbours")
+    xd, gd = _types(x, name, gate)
+    obytes, optr = _offsets(offsets)
+    sequences = xs[0] if offsets is None else offsets.shape[0] - 1
+    return (sequences, xs[-2], channels, heads, xd, gd, 1 if log_gate else 0, obytes, 1 if fill else 0), optr
 
 
 def linear_recurrence(x: torch.Tensor, gate: torch.Tensor, initial: Optional[torch.Tensor] = None,
@@ -112,24 +163,20 @@ def linear_recurrence(x: torch.Tensor, gate: torch.Tensor, initial: Optional[tor
     ``out`` may be x. Packed rows behind the last sequence are left as they were in ``out``, and zero in a fresh y.
     Results are reproducible from run to run. A value that is not finite makes the rows behind it, in its sequence and
     channel, not finite."""
-    _require_cuda(x.device, x=x, gate=gate, initial=initial, offsets=offsets, out=out)
-    s, sequences, optr = _shape(x, gate, offsets, log_gate, out is None, "x")
-    states = (sequences, x.shape[-1])
+    index = _device_of("x", x)
+    for name, t in (("gate", gate), ("initial", initial), ("offsets", offsets), ("out", out), ("temp", temp)):
+        _same_device(index, name, t)
+    dims, optr = _shape(x, gate, offsets, log_gate, out is None, "x")
+    states = (dims[0], dims[2])
     iptr = _states(initial, states, "initial")
-    if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    elif out.shape != x.shape or out.dtype != x.dtype:
-        raise ValueError("out must have the shape and type of x")
-    rg, rx, ry = _rows(gate, "gate"), _rows(x, "x"), _rows(out, "out")
-    final = torch.empty(states, dtype=torch.float32, device=x.device)
-    with _On(x.device):
-        stream = _stream(x)
-        temp = _scratch(False, s, x.device, temp)
-        have = C.c_size_t(temp.numel())
-        capi.check(capi.lib.tb200_linear_recurrence(temp.data_ptr(), C.byref(have), C.byref(s), optr, C.byref(rg),
-                                                    C.byref(rx), C.byref(ry), iptr, final.data_ptr(), stream),
-                   "tb200_linear_recurrence")
-        _finish(temp, stream, "tb200_linear_recurrence", sync)
+    out = _output(out, x, "x")
+    arrays = _Arrays(_rows(gate, "gate"), _rows(x, "x"), _rows(out, "out"))
+    final = x.new_empty(states, dtype=torch.float32)
+    temp = _scratch(_recurrence_bytes(False, *dims), x, temp)
+    shape, have, stream = capi.RecurrenceShape(*dims), C.c_size_t(temp.numel()), _raw_stream(index)
+    _call(capi.lib.tb200_linear_recurrence, "tb200_linear_recurrence", index, temp.data_ptr(), C.byref(have),
+          C.byref(shape), optr, *arrays.at, iptr, final.data_ptr(), stream)
+    _status(temp, stream, "tb200_linear_recurrence", index, sync)
     return out, final
 
 
@@ -142,25 +189,22 @@ def linear_recurrence_backward(gate: torch.Tensor, y: torch.Tensor, dy: torch.Te
     dy is the gradient of y, ``dfinal`` that of the final states (None: zero); ``initial``, ``offsets`` and ``log_gate``
     as in the forward call. dx has dy's type, dgate the gates' shape and type (summed over the channels that share a
     gate), dinitial is float32 [sequences, channels]. Packed rows behind the last sequence have zero gradients."""
-    _require_cuda(dy.device, dy=dy, gate=gate, y=y, initial=initial, dfinal=dfinal, offsets=offsets)
+    index = _device_of("dy", dy)
+    for name, t in (("gate", gate), ("y", y), ("initial", initial), ("dfinal", dfinal), ("offsets", offsets), ("temp", temp)):
+        _same_device(index, name, t)
     if y.shape != dy.shape or y.dtype != dy.dtype:
         raise ValueError("y and dy must have the same shape and type")
-    s, sequences, optr = _shape(dy, gate, offsets, log_gate, True, "dy")
-    states = (sequences, dy.shape[-1])
+    dims, optr = _shape(dy, gate, offsets, log_gate, True, "dy")
+    states = (dims[0], dims[2])
     iptr, fptr = _states(initial, states, "initial"), _states(dfinal, states, "dfinal")
-    dx = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
-    dgate = torch.empty(gate.shape, dtype=gate.dtype, device=dy.device)
-    dinitial = torch.empty(states, dtype=torch.float32, device=dy.device)
-    rg, ry, rdy = _rows(gate, "gate"), _rows(y, "y"), _rows(dy, "dy")
-    rdx, rdg = _rows(dx, "dx"), _rows(dgate, "dgate")
-    with _On(dy.device):
-        stream = _stream(dy)
-        temp = _scratch(True, s, dy.device, temp)
-        have = C.c_size_t(temp.numel())
-        capi.check(capi.lib.tb200_linear_recurrence_backward(
-            temp.data_ptr(), C.byref(have), C.byref(s), optr, C.byref(rg), C.byref(ry), C.byref(rdy), C.byref(rdx),
-            C.byref(rdg), iptr, fptr, dinitial.data_ptr(), stream), "tb200_linear_recurrence_backward")
-        _finish(temp, stream, "tb200_linear_recurrence_backward", sync)
+    dx, dgate = _empty_like(dy), _empty_like(gate)
+    dinitial = dy.new_empty(states, dtype=torch.float32)
+    arrays = _Arrays(_rows(gate, "gate"), _rows(y, "y"), _rows(dy, "dy"), _rows(dx, "dx"), _rows(dgate, "dgate"))
+    temp = _scratch(_recurrence_bytes(True, *dims), dy, temp)
+    shape, have, stream = capi.RecurrenceShape(*dims), C.c_size_t(temp.numel()), _raw_stream(index)
+    _call(capi.lib.tb200_linear_recurrence_backward, "tb200_linear_recurrence_backward", index, temp.data_ptr(),
+          C.byref(have), C.byref(shape), optr, *arrays.at, iptr, fptr, dinitial.data_ptr(), stream)
+    _status(temp, stream, "tb200_linear_recurrence_backward", index, sync)
     return dx, dgate, dinitial
 
 
@@ -174,46 +218,49 @@ def linear_recurrence_step(state: torch.Tensor, x: torch.Tensor, gate: torch.Ten
     them; None: state r). A row whose slot lies outside the pool (a negative one, say, where a batch is padded) gets a
     zero y and changes nothing; rows that name the same slot are applied in their order. Enqueues one kernel and
     returns without waiting."""
-    _require_cuda(x.device, x=x, state=state, gate=gate, slots=slots, out=out)
-    if x.dim() != 2 or state.dim() != 2 or state.dtype != torch.float32 or state.shape[1] != x.shape[1]:
+    index = _device_of("x", x)
+    _same_device(index, "state", state)
+    _same_device(index, "gate", gate)
+    _same_device(index, "slots", slots)
+    _same_device(index, "out", out)
+    xs, ss, gs = x.shape, state.shape, gate.shape
+    if len(xs) != 2 or len(ss) != 2 or state.dtype != torch.float32 or ss[1] != xs[1]:
         raise ValueError("x must be [rows, channels] and state float32 [slots, channels]")
-    rows, channels = x.shape
-    if gate.dim() != 2 or gate.shape[0] != rows or gate.shape[1] == 0 or channels == 0 or channels % gate.shape[1]:
+    rows, channels = xs
+    if len(gs) != 2 or gs[0] != rows or gs[1] == 0 or channels == 0 or channels % gs[1]:
         raise ValueError("gate must be [rows, channels], or [rows, heads] with a number of heads that divides the channels")
-    xd, gd = _float_code(x, "x"), _float_code(gate, "gate")
-    if gd != xd and gd != capi.F32:
-        raise TypeError("gate must have the type of x or float32")
+    xd, gd = _types(x, "x", gate)
     sbytes, sptr = 0, None
     if slots is not None:
         if slots.dtype not in _INDEX_BYTES or slots.shape != (rows,) or not slots.is_contiguous():
             raise ValueError("slots must be a contiguous 1-D tensor of an int32 or int64 for each row")
         sbytes, sptr = _INDEX_BYTES[slots.dtype], slots.data_ptr()
-    elif rows > state.shape[0]:
+    elif rows > ss[0]:
         raise ValueError("x has more rows than there are states")
-    if state.shape[0] > 1 and state.stride(0) < channels:
+    pool, apart, _ = _rows(state, "state")
+    if ss[0] <= 1:
+        apart = channels
+    elif apart < channels:
         raise ValueError("the states of the pool overlap")
-    if out is None:
-        out = torch.empty((rows, channels), dtype=x.dtype, device=x.device)
-    elif out.shape != x.shape or out.dtype != x.dtype:
-        raise ValueError("out must have the shape and type of x")
-    rs, rg, rx, ry = _rows(state, "state"), _rows(gate, "gate"), _rows(x, "x"), _rows(out, "out")
-    with _On(x.device):
-        capi.check(capi.lib.tb200_linear_recurrence_step(
-            rs.data, state.shape[0], max(rs.row_stride, channels), sptr, sbytes, C.byref(rg), C.byref(rx), C.byref(ry), rows,
-            channels, gate.shape[1], xd, gd, int(bool(log_gate)), _stream(x)), "tb200_linear_recurrence_step")
+    out = _output(out, x, "x")
+    arrays = _Arrays(_rows(gate, "gate"), _rows(x, "x"), _rows(out, "out"))
+    _call(capi.lib.tb200_linear_recurrence_step, "tb200_linear_recurrence_step", index, pool, ss[0], apart, sptr, sbytes,
+          *arrays.at, rows, channels, gs[1], xd, gd, 1 if log_gate else 0, _raw_stream(index))
     return out
 
 
 def _ids(ids: torch.Tensor) -> Tuple[int, int, int, int]:
     """(rows, ids of a row, distance of rows, bytes of an id)"""
-    if ids.dtype not in _INDEX_BYTES or ids.dim() not in (1, 2):
+    width, shape = _INDEX_BYTES.get(ids.dtype), ids.shape
+    if width is None or len(shape) not in (1, 2):
         raise ValueError("ids must be an int32 or int64 tensor [rows, k], or [rows]")
-    if ids.dim() == 1:
-        return ids.shape[0], 1, ids.stride(0) if ids.shape[0] > 1 else 1, _INDEX_BYTES[ids.dtype]
-    rows, k = ids.shape
-    if k == 0 or (rows and k > 1 and ids.stride(1) != 1) or (rows > 1 and ids.stride(0) < k):
+    stride = ids.stride()
+    if len(shape) == 1:
+        return shape[0], 1, stride[0] if shape[0] > 1 else 1, width
+    rows, k = shape
+    if k == 0 or (rows and k > 1 and stride[1] != 1) or (rows > 1 and stride[0] < k):
         raise ValueError("the ids of a row must be adjacent in memory, at least one, and rows must not overlap")
-    return rows, k, ids.stride(0) if rows > 1 else k, _INDEX_BYTES[ids.dtype]
+    return rows, k, stride[0] if rows > 1 else k, width
 
 
 def _mask(mask: Optional[torch.Tensor], rows: int) -> Optional[int]:
@@ -248,29 +295,26 @@ def expert_counts(ids: torch.Tensor, experts: int, mask: Optional[torch.Tensor] 
     [rows]. counts[e] is how often e occurs in rows whose mask (bool [rows], None: all) is set; ids outside
     [0, experts) are not counted. begins is the exclusive prefix sum of the counts: where each expert's tokens begin
     once (id, token) pairs are sorted with ``sort_by_key``. At most 8192 experts."""
-    _require_cuda(ids.device, ids=ids, mask=mask)
+    index = _device_of("ids", ids)
+    _same_device(index, "mask", mask)
+    _same_device(index, "temp", temp)
     rows, k, stride, width = _ids(ids)
     mptr = _mask(mask, rows)
-    need = _counts_bytes(experts)
-    both = torch.empty(2 * experts + 1, dtype=torch.int64, device=ids.device)
-    counts, begins = both[:experts], both[experts:]
-    with _On(ids.device):
-        stream = _stream(ids)
-        if temp is None or temp.numel() < need:
-            temp = _temp(need, ids.device)
-        have = C.c_size_t(temp.numel())
-        capi.check(capi.lib.tb200_expert_counts(temp.data_ptr(), C.byref(have), ids.data_ptr(), rows, k, stride, width,
-                                                mptr, experts, counts.data_ptr(), begins.data_ptr(), stream),
-                   "tb200_expert_counts")
-        _finish(temp, stream, "tb200_expert_counts", sync)
+    temp = _scratch(_counts_bytes(experts), ids, temp)
+    counts, begins = ids.new_empty((experts,), dtype=torch.int64), ids.new_empty((experts + 1,), dtype=torch.int64)
+    have, raw = C.c_size_t(temp.numel()), _raw_stream(index)
+    _call(capi.lib.tb200_expert_counts, "tb200_expert_counts", index, temp.data_ptr(), C.byref(have), ids.data_ptr(), rows,
+          k, stride, width, mptr, experts, counts.data_ptr(), begins.data_ptr(), raw)
+    _status(temp, raw, "tb200_expert_counts", index, sync)
     return counts, begins
 
 
 def _logits(logits: torch.Tensor, offsets: Optional[torch.Tensor]):
-    if logits.dim() != 2 or logits.shape[1] == 0:
+    shape = logits.shape
+    if len(shape) != 2 or shape[1] == 0:
         raise ValueError("logits must be [rows, experts]")
     obytes, optr = _offsets(offsets)
-    return _float_code(logits, "logits"), obytes, optr, 1 if offsets is None else offsets.numel() - 1
+    return _float_code(logits, "logits"), obytes, optr, 1 if offsets is None else offsets.shape[0] - 1, shape[0], shape[1]
 
 
 def balance_loss(logits: torch.Tensor, ids: torch.Tensor, mask: Optional[torch.Tensor] = None,
@@ -287,27 +331,23 @@ def balance_loss(logits: torch.Tensor, ids: torch.Tensor, mask: Optional[torch.T
     which is 1 when both are balanced, and 0 without any rows. A logit of -inf is a disabled expert; a row of nothing
     else has no probabilities. weights is the derivative of a sequence's loss by each of its probabilities: what
     ``balance_loss_backward`` needs besides the logits. Results are reproducible from run to run."""
-    _require_cuda(logits.device, logits=logits, ids=ids, mask=mask, offsets=offsets)
-    dtype, obytes, optr, sequences = _logits(logits, offsets)
-    rows, k, stride, width = _ids(ids)
-    if rows != logits.shape[0]:
+    index = _device_of("logits", logits)
+    for name, t in (("ids", ids), ("mask", mask), ("offsets", offsets), ("temp", temp)):
+        _same_device(index, name, t)
+    dtype, obytes, optr, sequences, rows, experts = _logits(logits, offsets)
+    id_rows, k, stride, width = _ids(ids)
+    if id_rows != rows:
         raise ValueError("logits and ids differ in rows")
-    experts = logits.shape[1]
-    mptr, rz = _mask(mask, rows), _rows(logits, "logits")
-    need = _balance_bytes(dtype, obytes, sequences, experts)
-    loss = torch.empty(sequences, dtype=torch.float32, device=logits.device)
-    counts = torch.empty((sequences, experts), dtype=torch.int64, device=logits.device)
-    weights = torch.empty((sequences, experts), dtype=torch.float32, device=logits.device)
-    with _On(logits.device):
-        stream = _stream(logits)
-        if temp is None or temp.numel() < need:
-            temp = _temp(need, logits.device)
-        have = C.c_size_t(temp.numel())
-        capi.check(capi.lib.tb200_balance_loss(
-            temp.data_ptr(), C.byref(have), C.byref(rz), dtype, ids.data_ptr(), k, stride, width, mptr, optr, obytes,
-            sequences, rows, experts, loss.data_ptr(), counts.data_ptr(), weights.data_ptr(), stream),
-            "tb200_balance_loss")
-        _finish(temp, stream, "tb200_balance_loss", sync)
+    mptr, arrays = _mask(mask, rows), _Arrays(_rows(logits, "logits"))
+    temp = _scratch(_balance_bytes(dtype, obytes, sequences, experts), logits, temp)
+    loss = logits.new_empty((sequences,), dtype=torch.float32)
+    counts = logits.new_empty((sequences, experts), dtype=torch.int64)
+    weights = logits.new_empty((sequences, experts), dtype=torch.float32)
+    have, stream = C.c_size_t(temp.numel()), _raw_stream(index)
+    _call(capi.lib.tb200_balance_loss, "tb200_balance_loss", index, temp.data_ptr(), C.byref(have), arrays.at[0], dtype,
+          ids.data_ptr(), k, stride, width, mptr, optr, obytes, sequences, rows, experts, loss.data_ptr(),
+          counts.data_ptr(), weights.data_ptr(), stream)
+    _status(temp, stream, "tb200_balance_loss", index, sync)
     return loss, counts, weights
 
 
@@ -317,18 +357,14 @@ def balance_loss_backward(logits: torch.Tensor, weights: torch.Tensor, dloss: to
     """Gradient of ``balance_loss`` by the logits, in their type, from its weights and dloss (float32 [sequences], the
     gradient of the losses); mask and offsets as in the forward call. Zero for masked rows and rows of no sequence.
     ``out`` may be logits. Enqueues one kernel and returns without waiting."""
-    _require_cuda(logits.device, logits=logits, weights=weights, dloss=dloss, mask=mask, offsets=offsets, out=out)
-    dtype, obytes, optr, sequences = _logits(logits, offsets)
-    rows, experts = logits.shape
+    index = _device_of("logits", logits)
+    for name, t in (("weights", weights), ("dloss", dloss), ("mask", mask), ("offsets", offsets), ("out", out)):
+        _same_device(index, name, t)
+    dtype, obytes, optr, sequences, rows, experts = _logits(logits, offsets)
     wptr = _states(weights, (sequences, experts), "weights")
     lptr = _states(dloss, (sequences,), "dloss")
-    if out is None:
-        out = torch.empty((rows, experts), dtype=logits.dtype, device=logits.device)
-    elif out.shape != logits.shape or out.dtype != logits.dtype:
-        raise ValueError("out must have the shape and type of logits")
-    mptr, rz, rd = _mask(mask, rows), _rows(logits, "logits"), _rows(out, "out")
-    with _On(logits.device):
-        capi.check(capi.lib.tb200_balance_loss_backward(C.byref(rz), dtype, wptr, lptr, mptr, optr, obytes, sequences, rows,
-                                                        experts, C.byref(rd), _stream(logits)),
-                   "tb200_balance_loss_backward")
+    out = _output(out, logits, "logits")
+    mptr, arrays = _mask(mask, rows), _Arrays(_rows(logits, "logits"), _rows(out, "out"))
+    _call(capi.lib.tb200_balance_loss_backward, "tb200_balance_loss_backward", index, arrays.at[0], dtype, wptr, lptr, mptr,
+          optr, obytes, sequences, rows, experts, arrays.at[1], _raw_stream(index))
     return out
