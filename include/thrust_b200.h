@@ -262,7 +262,7 @@ int tb200_histogram_sorted(const void* d_sorted, uint64_t n, int dtype, const vo
  * (sequences + 1 ascending DEVICE integers of offset_bytes, from 0 to at most `rows`; empty
  * sequences allowed). Rows behind the last sequence are left as they were, or written as zeros
  * where fill_outside != 0. A tb200_rows names an array by its first element and its strides in
- * elements; the channels of a row are adjacent; sequence_stride is ignored for packed rows.
+ * elements (row strides up to 2^28); the channels of a row are adjacent; sequence_stride is ignored for packed rows.
  * heads gates a row: heads == channels is a gate for each channel, otherwise heads divides
  * channels and channels / heads neighbouring channels share a gate. dtype (x, y and their
  * gradients): F32, F16 or BF16; gate_dtype: dtype or F32. d_initial, d_final and their
@@ -316,8 +316,8 @@ int tb200_expert_counts(void* d_temp, size_t* temp_bytes, const void* d_ids, uin
                         uint64_t id_stride, int id_bytes, const uint8_t* d_mask, uint32_t experts,
                         uint64_t* d_counts, uint64_t* d_begins, tb200_stream_t stream);
 
-/* Balance loss of router logits (rows x experts of F32, F16 or BF16, experts <= 1024, by strides;
- * sequence_stride ignored) and the ids chosen, for each of `sequences` sequences of packed rows
+/* Balance loss of router logits (rows x experts of F32, F16 or BF16, experts <= 1024, rows < 2^31,
+ * by strides of up to 2^28 elements; sequence_stride ignored) and the ids chosen, for each of `sequences` sequences of packed rows
  * (d_offsets as for the recurrence; offset_bytes 0: one sequence of all rows). With p the softmax
  * of a token's logits (zero where all of them are -inf), n the sequence's tokens with a mask that
  * is not 0 and c[e] its counts over these, as above:

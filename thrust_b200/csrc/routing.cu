@@ -128,34 +128,59 @@ expert_counts_kernel(Ids ids, const uint8_t* mask, uint64_t rows, uint64_t rows_
 // ---- rows of logits over lanes ------------------------------------------------------------------------
 
 // A row over L (a power of two) lanes: element i of step j is expert (j * L + lane) * 8 + i. Places beyond the last expert
-// hold -inf, like disabled experts.
+// hold -inf, like disabled experts. Eight elements stay in the words that they came in until they are worked on.
+template <typename T> constexpr int kWordsOf8 = sizeof(T) * 8 / 4;
 template <typename T, int J>
 struct RowPack {
-  Pack<T, 8> p[J];
+  unsigned w[J * kWordsOf8<T>];
 };
+template <typename T> __device__ constexpr unsigned none_word();
+template <> __device__ constexpr unsigned none_word<float>() { return 0xff800000u; }
+template <> __device__ constexpr unsigned none_word<__half>() { return 0xfc00fc00u; }
+template <> __device__ constexpr unsigned none_word<__nv_bfloat16>() { return 0xff80ff80u; }
+
 template <typename T>
-__device__ __forceinline__ Pack<T, 8> load8(const char* base, uint64_t element) {
-  Pack<T, 8> p;
-  const uint4* at = reinterpret_cast<const uint4*>(base + element * sizeof(T));
+__device__ __forceinline__ void unpack8(const unsigned* w, float* f) {
 #pragma unroll
-  for (int i = 0; i < (int)(sizeof(p) / 16); ++i) reinterpret_cast<uint4*>(&p)[i] = __ldcs(at + i);
-  return p;
+  for (int i = 0; i < kWordsOf8<T>; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      f[i] = __uint_as_float(w[i]);
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {  // the upper half of a float32
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    } else {
+      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      f[2 * i] = v.x;
+      f[2 * i + 1] = v.y;
+    }
+  }
 }
 template <typename T, int J, int L, bool VEC>
-__device__ __forceinline__ void load_row(const RowsOf& z, uint64_t row, bool on, uint32_t lane, uint32_t experts,
-                                         RowPack<T, J>& out) {
-  const T none = from_f32<T>(__int_as_float(0xff800000));
+__device__ __forceinline__ void load_row(const char* row, bool on, uint32_t lane, uint32_t experts, RowPack<T, J>& out) {
 #pragma unroll
   for (int j = 0; j < J; ++j) {
     const uint32_t e = (j * L + lane) * 8;
+    unsigned* w = &out.w[j * kWordsOf8<T>];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) out.p[j].v[i] = none;
+    for (int i = 0; i < kWordsOf8<T>; ++i) w[i] = none_word<T>();
     if constexpr (VEC) {
-      if (on && e < experts) out.p[j] = load8<T>(z.data, row * z.row + e);
+      if (on && e < experts) {
+#pragma unroll
+        for (int i = 0; i < kWordsOf8<T> / 4; ++i) {
+          const uint4 v = __ldcs(reinterpret_cast<const uint4*>(row + e * sizeof(T)) + i);
+          w[4 * i] = v.x;
+          w[4 * i + 1] = v.y;
+          w[4 * i + 2] = v.z;
+          w[4 * i + 3] = v.w;
+        }
+      }
     } else {
+      Pack<T, 8> p;
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (on && e + i < experts) out.p[j].v[i] = *reinterpret_cast<const T*>(z.data + (row * z.row + e + i) * sizeof(T));
+        p.v[i] = on && e + i < experts ? reinterpret_cast<const T*>(row)[e + i] : from_f32<T>(__int_as_float(0xff800000));
+#pragma unroll
+      for (int i = 0; i < kWordsOf8<T>; ++i) w[i] = reinterpret_cast<const unsigned*>(&p)[i];
     }
   }
 }
@@ -177,25 +202,23 @@ __device__ __forceinline__ float softmax_row(const RowPack<T, J>& row, float (&e
   const float none = __int_as_float(0xff800000);
   float top = none;
 #pragma unroll
-  for (int j = 0; j < J; ++j)
+  for (int j = 0; j < J; ++j) unpack8<T>(&row.w[j * kWordsOf8<T>], &e[j * 8]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      e[j * 8 + i] = to_f32<T>(row.p[j].v[i]);
-      top = fmaxf(top, e[j * 8 + i]);
-    }
+  for (int i = 0; i < J * 8; ++i) top = fmaxf(top, e[i]);
   top = lanes_max<L>(top);
   float unit[J * 8], base[J * 8];
   fill_n(unit, kLog2e);
   fill_n(base, top == none ? 0.0f : -top);  // the difference first: logits near the end of the type's range stay in it
   add_n(e, e, base);
   mul_n(e, e, unit);
-  float sum = 0.0f;
+  float part[2] = {0.0f, 0.0f};
 #pragma unroll
-  for (int i = 0; i < J * 8; ++i) {
+  for (int i = 0; i < J * 8; i += 2) {
     e[i] = exp2_fast(e[i]);
-    sum += e[i];
+    e[i + 1] = exp2_fast(e[i + 1]);
+    add2(part[0], part[1], part[0], part[1], e[i], e[i + 1]);
   }
-  sum = lanes_sum<L>(sum);
+  const float sum = lanes_sum<L>(part[0] + part[1]);
   float scale;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(scale) : "f"(sum));  // the sum is 1 at least, or zero
   return sum == 0.0f ? 0.0f : scale;
@@ -296,18 +319,21 @@ __global__ void __launch_bounds__(kRouteThreads, J == 1 ? 3 : 1) balance_kernel(
     constexpr int U = kRowsAtOnce<T, J>;
     RowPack<T, J> pack[U], ahead[U];
     bool on[U], on_ahead[U];
-    auto fetch = [&](uint64_t base, RowPack<T, J>(&into)[U], bool(&counts)[U]) {
+    const uint32_t here = (uint32_t)(to - from);
+    const char* const rows_here = a.z.data + from * a.z.row * sizeof(T);
+    const uint32_t row_bytes = (uint32_t)(a.z.row * sizeof(T));
+    auto fetch = [&](uint32_t base, RowPack<T, J>(&into)[U], bool(&counts)[U]) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const uint64_t row = base + u * kRouteWarps * groups + group;
-        counts[u] = row < to && (a.mask == nullptr || a.mask[row]);
-        load_row<T, J, L, VEC>(a.z, row, counts[u], in_row, a.experts, into[u]);
+        const uint32_t row = base + u * kRouteWarps * groups + group;
+        counts[u] = row < here && (a.mask == nullptr || a.mask[from + row]);
+        load_row<T, J, L, VEC>(rows_here + (uint64_t)row * row_bytes, counts[u], in_row, a.experts, into[u]);
       }
     };
-    fetch(from + warp * groups, pack, on);
+    fetch(warp * groups, pack, on);
     __syncthreads();
     count_rows(a.ids, a.mask, from, to, a.experts, s_count);
-    for (uint64_t base = from + warp * groups; base < to; base += U * kRouteWarps * groups) {
+    for (uint32_t base = warp * groups; base < here; base += U * kRouteWarps * groups) {
       fetch(base + U * kRouteWarps * groups, ahead, on_ahead);
 #pragma unroll
       for (int u = 0; u < U; ++u) {  // rows that do not count hold -inf alone
@@ -397,32 +423,40 @@ __global__ void __launch_bounds__(kRouteThreads, J == 1 ? 3 : 1) balance_backwar
   const uint32_t in_row = lane % L, group = lane / L;
   const uint64_t warp = blockIdx.x * (uint64_t)kRouteWarps + threadIdx.x / kWarp;
   const uint64_t r0 = warp * a.rows_of_warp, r1 = min(r0 + a.rows_of_warp, a.spans.rows);
-  uint64_t s = ~0ull, end = 0;  // the sequence whose weights are held, and its end
+  if (r0 >= r1) return;
+  uint64_t s = ~0ull;     // the sequence whose weights are held,
+  uint32_t held_to = 0;   // its end among the warp's rows,
+  bool some = false;      // and whether there is one
   float w[J * 8] = {};
   float scale = 0.0f;
   constexpr int U = kRowsAtOnce<T, J>;
   RowPack<T, J> pack[U], ahead[U];
   bool on[U], on_ahead[U];
-  auto fetch = [&](uint64_t at, RowPack<T, J>(&into)[U], bool(&counts)[U]) {
+  const uint32_t here = (uint32_t)(r1 - r0), row_bytes = (uint32_t)(a.z.row * sizeof(T)), out_bytes = (uint32_t)(a.dz.row * sizeof(T));
+  const char* const rows_here = a.z.data + r0 * a.z.row * sizeof(T);
+  char* const out_here = a.dz.data + r0 * a.dz.row * sizeof(T);
+  auto fetch = [&](uint32_t at, RowPack<T, J>(&into)[U], bool(&counts)[U]) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const uint64_t row = at + u * groups + group;
-      counts[u] = row < r1 && (a.mask == nullptr || a.mask[row]);
-      load_row<T, J, L, VEC>(a.z, row, counts[u], in_row, a.experts, into[u]);
+      const uint32_t row = at + u * groups + group;
+      counts[u] = row < here && (a.mask == nullptr || a.mask[r0 + row]);
+      load_row<T, J, L, VEC>(rows_here + (uint64_t)row * row_bytes, counts[u], in_row, a.experts, into[u]);
     }
   };
-  fetch(r0, pack, on);
-  for (uint64_t at = r0; at < r1; at += U * groups) {
+  fetch(0, pack, on);
+  for (uint32_t at = 0; at < here; at += U * groups) {
     fetch(at + U * groups, ahead, on_ahead);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const uint64_t row = at + u * groups + group;
-      const bool valid = row < r1;
-      if (valid && (s == ~0ull || row >= end)) {
-        if (s == ~0ull) s = sequence_of(a.spans, row);
-        while (s < a.spans.sequences && row >= begin_of(a.spans, s + 1)) ++s;
-        end = s < a.spans.sequences ? begin_of(a.spans, s + 1) : a.spans.rows;
-        const bool some = s < a.spans.sequences && row >= begin_of(a.spans, s);
+      const uint32_t row = at + u * groups + group;
+      const bool valid = row < here;
+      if (valid && row >= held_to) {
+        const uint64_t at_row = r0 + row;
+        if (s == ~0ull) s = sequence_of(a.spans, at_row);
+        while (s < a.spans.sequences && at_row >= begin_of(a.spans, s + 1)) ++s;
+        const uint64_t end = s < a.spans.sequences ? begin_of(a.spans, s + 1) : a.spans.rows;
+        held_to = end - r0 < here ? (uint32_t)(end - r0) : here;
+        some = s < a.spans.sequences && at_row >= begin_of(a.spans, s);
         scale = some ? a.dloss[s] : 0.0f;
 #pragma unroll
         for (int j = 0; j < J; ++j)
@@ -432,13 +466,13 @@ __global__ void __launch_bounds__(kRouteThreads, J == 1 ? 3 : 1) balance_backwar
             w[j * 8 + i] = some && e < a.experts ? a.weights[s * a.experts + e] : 0.0f;
           }
       }
-      const bool kept = on[u] && s < a.spans.sequences;
+      const bool kept = on[u] && some;
       float e[J * 8];
       const float share = softmax_row<T, J, L>(pack[u], e);
-      float dot = 0.0f;
+      float part[2] = {0.0f, 0.0f};
 #pragma unroll
-      for (int i = 0; i < J * 8; ++i) dot = fmaf(e[i], w[i], dot);
-      dot = lanes_sum<L>(dot) * share;
+      for (int i = 0; i < J * 8; i += 2) fma2(part[0], part[1], e[i], e[i + 1], w[i], w[i + 1], part[0], part[1]);
+      const float dot = lanes_sum<L>(part[0] + part[1]) * share;
       float less[J * 8], factor[J * 8], d[J * 8];
       fill_n(less, -dot);
       fill_n(factor, kept ? scale * share : 0.0f);
@@ -449,19 +483,19 @@ __global__ void __launch_bounds__(kRouteThreads, J == 1 ? 3 : 1) balance_backwar
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         const uint32_t first = (j * L + in_row) * 8;
+        char* to = out_here + (uint64_t)row * out_bytes + first * sizeof(T);
         Pack<T, 8> out;
 #pragma unroll
         for (int i = 0; i < 8; ++i) out.v[i] = from_f32<T>(d[j * 8 + i]);
         if constexpr (VEC) {
           if (first < a.experts) {
-            uint4* to = reinterpret_cast<uint4*>(a.dz.data + (row * a.dz.row + first) * sizeof(T));
 #pragma unroll
-            for (int i = 0; i < (int)(sizeof(out) / 16); ++i) to[i] = reinterpret_cast<const uint4*>(&out)[i];
+            for (int i = 0; i < (int)(sizeof(out) / 16); ++i) reinterpret_cast<uint4*>(to)[i] = reinterpret_cast<const uint4*>(&out)[i];
           }
         } else {
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            if (first + i < a.experts) *reinterpret_cast<T*>(a.dz.data + (row * a.dz.row + first + i) * sizeof(T)) = out.v[i];
+            if (first + i < a.experts) reinterpret_cast<T*>(to)[i] = out.v[i];
         }
       }
     }
@@ -568,6 +602,7 @@ extern "C" int tb200_balance_loss(void* d_temp, size_t* temp_bytes, const tb200_
   if (reinterpret_cast<uintptr_t>(d_temp) % 256) return TB200_ERR_INVALID_ARGUMENT;
   int rc = check_ids(d_ids, rows, k, id_stride, id_bytes);
   if (rc) return rc;
+  if (rows >= (1ull << 31) || (rows && logits && logits->row_stride > (1u << 28))) return TB200_ERR_UNSUPPORTED;
   const int tb = model_bytes(dtype);
   if (rows && !good_rows(logits, tb)) return TB200_ERR_INVALID_ARGUMENT;
   if (offset_bytes && (!d_offsets || reinterpret_cast<uintptr_t>(d_offsets) % offset_bytes)) return TB200_ERR_INVALID_ARGUMENT;
@@ -627,11 +662,12 @@ extern "C" int tb200_balance_loss_backward(const tb200_rows* logits, int dtype, 
   using namespace tb200;
   const int tb = model_bytes(dtype);
   if (experts == 0) return TB200_ERR_INVALID_ARGUMENT;
-  if (tb == 0 || experts > kMaxBalanceExperts || sequences > 0x7fffffffull || rows > (1ull << 40)) return TB200_ERR_UNSUPPORTED;
+  if (tb == 0 || experts > kMaxBalanceExperts || sequences > 0x7fffffffull || rows >= (1ull << 31)) return TB200_ERR_UNSUPPORTED;
   if (offset_bytes != 0 && offset_bytes != 4 && offset_bytes != 8) return TB200_ERR_INVALID_ARGUMENT;
   if (offset_bytes == 0 && sequences != 1) return TB200_ERR_INVALID_ARGUMENT;
   if (rows == 0) return TB200_OK;
   if (!good_rows(logits, tb) || !good_rows(dlogits, tb)) return TB200_ERR_INVALID_ARGUMENT;
+  if (logits->row_stride > (1u << 28) || dlogits->row_stride > (1u << 28)) return TB200_ERR_UNSUPPORTED;
   if (offset_bytes && (!d_offsets || reinterpret_cast<uintptr_t>(d_offsets) % offset_bytes)) return TB200_ERR_INVALID_ARGUMENT;
   if (sequences && (!d_weights || !d_dloss)) return TB200_ERR_INVALID_ARGUMENT;
   if ((reinterpret_cast<uintptr_t>(d_weights) | reinterpret_cast<uintptr_t>(d_dloss)) % 4) return TB200_ERR_INVALID_ARGUMENT;
