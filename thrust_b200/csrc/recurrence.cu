@@ -89,10 +89,12 @@ __device__ __forceinline__ unsigned state_bits(float h) {
 
 // The state in front of a tile, for one channel: from the nearest known state among the tiles in front, through the maps
 // of the tiles between, in the order of the rows. A known state is itself the one in front of its tile put through that
-// tile's map, so the value is the same wherever the walk begins, to the bit. At most kReach tiles back; where no state is
-// known there, the wait is for one to come closer, which the tile right behind the last known state always brings about.
+// tile's map, so the value is the same wherever the walk begins, to the bit. Eight tiles back, and eight more where all
+// the maps of the first eight but none of their states are known (few chains, many tiles of each in work); where no
+// state is known there either, the wait is for one to come closer, which the tile right behind the last known state
+// always brings about.
 constexpr int kReach = 8;
-struct InFront {  // what is known of the tiles in front, nearest first
+struct InFront {  // what is known of eight tiles in front, nearest first
   unsigned long long maps[kReach];
   unsigned states[kReach];
   __device__ __forceinline__ void look(const unsigned long long* m, const unsigned* s, uint64_t step, unsigned tile) {
@@ -104,38 +106,58 @@ struct InFront {  // what is known of the tiles in front, nearest first
       maps[j] = j < tile ? ld_relaxed_u64(m) : 0ull;
     }
   }
-  // For a whole warp: from the nearest state that all its channels know.
-  __device__ __forceinline__ bool state(float& h) const {
-    h = 0.0f;
+  // For a whole warp: the distance of the nearest state that all its channels know, with all maps nearer than it; kReach
+  // where there are only maps, more where some are missing.
+  __device__ __forceinline__ int nearest() const {
     unsigned all_states = 0, all_maps = 0;
 #pragma unroll
     for (int j = 0; j < kReach; ++j) {
       all_states |= (unsigned)__all_sync(0xffffffffu, states[j] != 0u) << j;
       all_maps |= (unsigned)__all_sync(0xffffffffu, maps[j] != 0ull) << j;
     }
-    if (all_states == 0) return false;
-    const int from = __ffs(all_states) - 1;  // the maps of all nearer tiles are needed
-    if ((~all_maps & ((1u << from) - 1u)) != 0) return false;
+    const int from = __ffs(all_states | 1u << kReach) - 1;
+    return (~all_maps & ((1u << from) - 1u)) != 0 ? kReach + 1 : from;
+  }
+  // From the state at a distance, or from h where that is kReach, through the nearer maps.
+  __device__ __forceinline__ float through(int from, float h) const {
 #pragma unroll
     for (int j = kReach - 1; j >= 0; --j) {
       if (j > from) continue;
       h = j == from ? __uint_as_float(~states[j])
                     : apply((unsigned)(~maps[j] >> 32), h, __uint_as_float((unsigned)~maps[j]));
     }
-    return true;
+    return h;
   }
 };
-__device__ __forceinline__ float state_in_front(InFront& f, const unsigned long long* maps, const unsigned* states,
-                                                uint64_t step, unsigned tile, int* status) {
-  float h;
-  for (unsigned polls = 0; !f.state(h); ++polls) {
+// One look. True where the state is known.
+__device__ __forceinline__ bool look_for_state(const unsigned long long* maps, const unsigned* states, uint64_t step,
+                                               unsigned tile, float& h) {
+  InFront near;
+  near.look(maps, states, step, tile);
+  int from = near.nearest();
+  if (from > kReach) return false;
+  if (from == kReach) {
+    if (tile <= kReach) return false;
+    InFront far;
+    far.look(maps - kReach * step, states - kReach * step, step, tile - kReach);
+    from = far.nearest();
+    if (from >= kReach) return false;
+    h = far.through(from, 0.0f);
+    from = kReach;
+  }
+  h = near.through(from, h);
+  return true;
+}
+__device__ __forceinline__ float wait_for_state(const unsigned long long* maps, const unsigned* states, uint64_t step,
+                                                unsigned tile, int* status) {
+  float h = 0.0f;
+  for (unsigned polls = 0; !look_for_state(maps, states, step, tile, h); ++polls) {
     if ((polls & 63u) == 63u && __any_sync(0xffffffffu, ld_relaxed_s32(status) != 0)) break;  // someone else gave up
     if (polls >= kSpinLimit) {
       note_timeout(status, kSiteLookback, tile, 0);
       break;
     }
     backoff(polls);
-    f.look(maps, states, step, tile);
   }
   return h;
 }
@@ -489,14 +511,12 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
       const uint64_t p_at = (uint64_t)p_id * WIDTH + c;
       // ---- the states in front of the stretches of the tile before: at once where they are known by now, ---------
       // ---- else after this tile's map is out -----------------------------------------------------------------------
-      InFront front;
       float in_front = 0.0f;
       bool known = true;
       unsigned long long* maps_ready = &s_ready[k];
       if (p_wait) {
         do {  // as long as there is nothing else to do
-          front.look(p.maps + p_at, p.states + p_at, step, p_tile);
-          known = front.state(in_front);
+          known = look_for_state(p.maps + p_at, p.states + p_at, step, p_tile, in_front);
         } while (!known && some && !__any_sync(0xffffffffu, mbar_test(maps_ready, i >> 1 & 1)));
       }
       auto hand_on = [&] {
@@ -553,7 +573,7 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
         }
       }
       if (!known) {
-        in_front = state_in_front(front, p.maps + p_at, p.states + p_at, step, p_tile, &p.hdr->status);
+        in_front = wait_for_state(p.maps + p_at, p.states + p_at, step, p_tile, &p.hdr->status);
         hand_on();
       }
       if (!some) return;
