@@ -58,7 +58,7 @@ struct RecArgs {
   float* partial;               // backward, a head over several blocks: their sums, [rows][heads][parts]
   TempHeader* hdr;
   uint32_t blocks, chains;      // blocks of channels, chains
-  Divisor by_blocks, by_chains;
+  Divisor by_blocks, by_chains, by_gates;  // by_gates: heads in a block
   // bytes from a row to the next one with the recurrence
   int next_gate, next_in, next_out, next_y, next_dgate;
   uint64_t tiles;               // of a chain
@@ -352,6 +352,7 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
   // of the stretches: bit 0, a sequence begins among the rows; bit 1, there are rows in front of that
   __shared__ __align__(8) unsigned char s_kinds[2][kWarps];
   __shared__ TileInfo s_tiles[8];  // of the CTA, a ring
+  __shared__ float s_heads[SHARED && BACK ? kWarps : 1][SHARED && BACK ? R : 1][kWarp + 1];
   __shared__ unsigned long long s_landed[kStages];  // a stage's boxes
   __shared__ unsigned long long s_ready[2];         // the maps of all warps' stretches, by the parity of the tile
   auto* s_word = reinterpret_cast<unsigned(*)[kWarps][WIDTH]>(s_dynamic + kStages * S::kStage);
@@ -372,6 +373,7 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
   const int lane_x = lane * V * (int)sizeof(T);
   const int lane_head = SHARED && p.parts == 1 ? lane * V / (int)p.head_size : 0;
   const int lane_g = SHARED ? lane_head * (int)sizeof(G) : lane * V * (int)sizeof(G);
+  const int head_lanes = SHARED ? (p.parts == 1 ? (int)p.head_size / V : kWarp) : 1;
   constexpr int GATES = SHARED ? kWarp : WIDTH;  // places for gates in a row of a stage
 
   // row r of the warp in a stage; rows lie in the order of memory
@@ -404,12 +406,11 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
     const int n = w.rows - warp * R;  // rows of this warp
     if constexpr (SHARED) {
       // the warp's gates, one a lane: row by row, the block's heads of a row side by side
-      const int here = w.count < p.head_size ? 1 : (int)(w.count / p.head_size);
 #pragma unroll
       for (int j = 0; j < R; ++j) {
-        const int v = j * kWarp + lane, r = v / block_gates, h = v - r * block_gates;
+        const int v = j * kWarp + lane, r = (int)p.by_gates.of(v), h = v - r * block_gates;
         if (j * kWarp >= R * block_gates) break;
-        if (r < R && r < n && h < here) late.gate[j] = load_pack<G, 1>(row_of(w.gate, p.next_gate, r), h).v[0];
+        if (r < R && r < n && w.head + h < p.heads) late.gate[j] = load_pack<G, 1>(row_of(w.gate, p.next_gate, r), h).v[0];
       }
     }
     if constexpr (!S::BOXES) {
@@ -436,7 +437,7 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
     if constexpr (SHARED) {
 #pragma unroll
       for (int j = 0; j < R; ++j) {
-        const int v = j * kWarp + lane, r = v / block_gates, h = v - r * block_gates;
+        const int v = j * kWarp + lane, r = (int)p.by_gates.of(v), h = v - r * block_gates;
         if (j * kWarp >= R * block_gates) break;
         if (r < R) reinterpret_cast<G*>(gates + k * S::kStage)[place(r) * GATES + h] = late.gate[j];
       }
@@ -761,6 +762,7 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
       }
       char* to = pw.out + lane_x;
       char* to_g = BACK ? pw.dgate + lane_g : nullptr;
+      float head_sum[SHARED && BACK ? R : 1] = {};
       auto second_pass = [&](auto inner, auto log_gate) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
@@ -815,26 +817,9 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
             if constexpr (!SHARED) {
               if (inner || live) store_floats<G, V>(row_of(to_g, p.next_dgate, r), 0, dg);
             } else {
-              // the head's lanes are neighbours; the first of them gathers the sum
-              float sum = 0.0f;
 #pragma unroll
-              for (int e = 0; e < V; ++e) sum += dg[e];
-              if (!live) sum = 0.0f;
-              const int per = p.parts == 1 ? (int)p.head_size / V : kWarp;
-              const int place = lane % per;
-              for (int off = 1; off < per; off *= 2) {
-                const float other = __shfl_down_sync(0xffffffffu, sum, off);
-                if (place + off < per) sum += other;
-              }
-              if (live && place == 0) {
-                if (p.parts == 1) {
-                  const float one[1] = {sum};
-                  store_floats<G, 1>(row_of(to_g, p.next_dgate, r), 0, one);
-                } else {
-                  const uint64_t flat = pw.chain * p.chain_rows + (uint64_t)(pw.row - warp * R - r);
-                  p.partial[(flat * p.heads + pw.head) * p.parts + pw.block % p.parts] = sum;
-                }
-              }
+              for (int e = 0; e < V; ++e) head_sum[r] += dg[e];
+              if (!live) head_sum[r] = 0.0f;
             }
           }
           if (in && end && p.last && live) {
@@ -849,6 +834,28 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
         if (logg) second_pass(std::true_type{}, std::true_type{}); else second_pass(std::true_type{}, std::false_type{});
       } else {
         second_pass(std::false_type{}, logg);
+      }
+      if constexpr (SHARED && BACK) {
+        // the lanes' sums meet in shared memory: a lane adds up one row of one head, in the order of the channels
+        // (shuffles here are compiled to a form that takes 300 cycles each)
+        float(*sums)[kWarp + 1] = s_heads[warp];
+#pragma unroll
+        for (int r = 0; r < R; ++r) sums[r][lane] = head_sum[r];
+        __syncwarp();
+        for (int v = lane; v < R * block_gates; v += kWarp) {
+          const int r = (int)p.by_gates.of(v), h = v - r * block_gates;
+          const bool there = p_plain || (pk.inside >> r & 1) || (p.fill && warp * R + r < pw.rows);
+          if (!there || h * head_lanes * V >= (int)pw.count) continue;
+          float one[1] = {0.0f};
+          for (int l = 0; l < head_lanes; ++l) one[0] += sums[r][h * head_lanes + l];
+          if (p.parts == 1) {
+            store_floats<G, 1>(row_of(pw.dgate, p.next_dgate, r), h, one);
+          } else {
+            const uint64_t flat = pw.chain * p.chain_rows + (uint64_t)(pw.row - warp * R - r);
+            p.partial[(flat * p.heads + pw.head) * p.parts + pw.block % p.parts] = one[0];
+          }
+        }
+        __syncwarp();
       }
     }
     if (!some) return;
@@ -956,6 +963,7 @@ int launch_kernel(Call& k, const Maps& maps, cudaStream_t stream) {
   }
   p.by_blocks = divisor(p.blocks);
   p.by_chains = divisor(p.chains);
+  p.by_gates = divisor(SHARED && p.parts == 1 ? p.block_heads : 1);
   const auto next = [](const RowsOf& a, int elem) { return (int)(a.row * elem) * (BACK ? -1 : 1); };
   for (const RowsOf* a : {&p.gate, &p.in, &p.out, &p.y, &p.dgate})
     if (a->row > (1u << 28)) return TB200_ERR_UNSUPPORTED;  // a tile's rows are reached by 32-bit steps
