@@ -8,6 +8,7 @@ here records itself for autograd.
 from __future__ import annotations
 
 import ctypes as C
+import threading
 from functools import lru_cache
 from typing import Optional, Tuple
 
@@ -76,15 +77,23 @@ def _rows(t: torch.Tensor, name: str) -> Tuple[int, int, int]:
     return t.data_ptr(), stride[-2], stride[0] if len(stride) == 3 else 0
 
 
-class _Arrays:
-    """Several tb200_rows one behind the other; at[i] is the address of the i-th."""
-    __slots__ = ("words", "at")
+class _Words(threading.local):
+    """A thread's room for five tb200_rows one behind the other; a call has read them when it returns."""
 
-    def __init__(self, *rows):
-        flat = [w for r in rows for w in r]
-        self.words = (C.c_uint64 * len(flat))(*flat)
+    def __init__(self):
+        self.words = (C.c_uint64 * 15)()
         base = C.addressof(self.words)
-        self.at = [base + 24 * i for i in range(len(rows))]
+        self.at = tuple(base + 24 * i for i in range(5))
+
+
+_words = _Words()
+
+
+def _arrays(*rows) -> Tuple[int, ...]:
+    """The addresses of these arrays of rows, written into the thread's room."""
+    flat = [w for r in rows for w in r]
+    _words.words[:len(flat)] = flat
+    return _words.at[:len(rows)]
 
 
 def _states(t: Optional[torch.Tensor], shape, name: str) -> Optional[int]:
@@ -170,12 +179,12 @@ def linear_recurrence(x: torch.Tensor, gate: torch.Tensor, initial: Optional[tor
     states = (dims[0], dims[2])
     iptr = _states(initial, states, "initial")
     out = _output(out, x, "x")
-    arrays = _Arrays(_rows(gate, "gate"), _rows(x, "x"), _rows(out, "out"))
+    arrays = _arrays(_rows(gate, "gate"), _rows(x, "x"), _rows(out, "out"))
     final = x.new_empty(states, dtype=torch.float32)
     temp = _scratch(_recurrence_bytes(False, *dims), x, temp)
     shape, have, stream = capi.RecurrenceShape(*dims), C.c_size_t(temp.numel()), _raw_stream(index)
     _call(capi.lib.tb200_linear_recurrence, "tb200_linear_recurrence", index, temp.data_ptr(), C.byref(have),
-          C.byref(shape), optr, *arrays.at, iptr, final.data_ptr(), stream)
+          C.byref(shape), optr, *arrays, iptr, final.data_ptr(), stream)
     _status(temp, stream, "tb200_linear_recurrence", index, sync)
     return out, final
 
@@ -199,11 +208,11 @@ def linear_recurrence_backward(gate: torch.Tensor, y: torch.Tensor, dy: torch.Te
     iptr, fptr = _states(initial, states, "initial"), _states(dfinal, states, "dfinal")
     dx, dgate = _empty_like(dy), _empty_like(gate)
     dinitial = dy.new_empty(states, dtype=torch.float32)
-    arrays = _Arrays(_rows(gate, "gate"), _rows(y, "y"), _rows(dy, "dy"), _rows(dx, "dx"), _rows(dgate, "dgate"))
+    arrays = _arrays(_rows(gate, "gate"), _rows(y, "y"), _rows(dy, "dy"), _rows(dx, "dx"), _rows(dgate, "dgate"))
     temp = _scratch(_recurrence_bytes(True, *dims), dy, temp)
     shape, have, stream = capi.RecurrenceShape(*dims), C.c_size_t(temp.numel()), _raw_stream(index)
     _call(capi.lib.tb200_linear_recurrence_backward, "tb200_linear_recurrence_backward", index, temp.data_ptr(),
-          C.byref(have), C.byref(shape), optr, *arrays.at, iptr, fptr, dinitial.data_ptr(), stream)
+          C.byref(have), C.byref(shape), optr, *arrays, iptr, fptr, dinitial.data_ptr(), stream)
     _status(temp, stream, "tb200_linear_recurrence_backward", index, sync)
     return dx, dgate, dinitial
 
@@ -243,9 +252,9 @@ def linear_recurrence_step(state: torch.Tensor, x: torch.Tensor, gate: torch.Ten
     elif apart < channels:
         raise ValueError("the states of the pool overlap")
     out = _output(out, x, "x")
-    arrays = _Arrays(_rows(gate, "gate"), _rows(x, "x"), _rows(out, "out"))
+    arrays = _arrays(_rows(gate, "gate"), _rows(x, "x"), _rows(out, "out"))
     _call(capi.lib.tb200_linear_recurrence_step, "tb200_linear_recurrence_step", index, pool, ss[0], apart, sptr, sbytes,
-          *arrays.at, rows, channels, gs[1], xd, gd, 1 if log_gate else 0, _raw_stream(index))
+          *arrays, rows, channels, gs[1], xd, gd, 1 if log_gate else 0, _raw_stream(index))
     return out
 
 
@@ -338,13 +347,13 @@ def balance_loss(logits: torch.Tensor, ids: torch.Tensor, mask: Optional[torch.T
     id_rows, k, stride, width = _ids(ids)
     if id_rows != rows:
         raise ValueError("logits and ids differ in rows")
-    mptr, arrays = _mask(mask, rows), _Arrays(_rows(logits, "logits"))
+    mptr, arrays = _mask(mask, rows), _arrays(_rows(logits, "logits"))
     temp = _scratch(_balance_bytes(dtype, obytes, sequences, experts), logits, temp)
     loss = logits.new_empty((sequences,), dtype=torch.float32)
     counts = logits.new_empty((sequences, experts), dtype=torch.int64)
     weights = logits.new_empty((sequences, experts), dtype=torch.float32)
     have, stream = C.c_size_t(temp.numel()), _raw_stream(index)
-    _call(capi.lib.tb200_balance_loss, "tb200_balance_loss", index, temp.data_ptr(), C.byref(have), arrays.at[0], dtype,
+    _call(capi.lib.tb200_balance_loss, "tb200_balance_loss", index, temp.data_ptr(), C.byref(have), arrays[0], dtype,
           ids.data_ptr(), k, stride, width, mptr, optr, obytes, sequences, rows, experts, loss.data_ptr(),
           counts.data_ptr(), weights.data_ptr(), stream)
     _status(temp, stream, "tb200_balance_loss", index, sync)
@@ -364,7 +373,7 @@ def balance_loss_backward(logits: torch.Tensor, weights: torch.Tensor, dloss: to
     wptr = _states(weights, (sequences, experts), "weights")
     lptr = _states(dloss, (sequences,), "dloss")
     out = _output(out, logits, "logits")
-    mptr, arrays = _mask(mask, rows), _Arrays(_rows(logits, "logits"), _rows(out, "out"))
-    _call(capi.lib.tb200_balance_loss_backward, "tb200_balance_loss_backward", index, arrays.at[0], dtype, wptr, lptr, mptr,
-          optr, obytes, sequences, rows, experts, arrays.at[1], _raw_stream(index))
+    mptr, arrays = _mask(mask, rows), _arrays(_rows(logits, "logits"), _rows(out, "out"))
+    _call(capi.lib.tb200_balance_loss_backward, "tb200_balance_loss_backward", index, arrays[0], dtype, wptr, lptr, mptr,
+          optr, obytes, sequences, rows, experts, arrays[1], _raw_stream(index))
     return out
