@@ -399,3 +399,64 @@ def test_streams_and_graphs(cuda_device):
         y2, f2 = tb.linear_recurrence(sx, gate, log_gate=True)
         g2 = tb.linear_recurrence_backward(gate, y2, sdy, log_gate=True)
         assert torch.equal(y, y2) and torch.equal(f, f2) and all(torch.equal(a, b) for a, b in zip(grads, g2))
+
+
+def test_short_sequences_that_lie_apart(cuda_device):
+    """Sequences of a few rows in a time-major batch: no two of them lie behind one another."""
+    rng = np.random.default_rng(12)
+    for rows, channels in ((5, 64), (1, 20), (32, 136)):
+        x, gate = make(rng, (40, rows), channels, channels, "bf16", "f32", True, cuda_device)
+        apart = x.transpose(0, 1).contiguous().transpose(0, 1)
+        a, b = tb.linear_recurrence(x, gate, log_gate=True), tb.linear_recurrence(apart, gate, log_gate=True)
+        wy, wf = reference(x, gate, None, None, True)
+        for y, final in (a, b):
+            close(y, wy, x.dtype, rows, what="y")
+            close(final, wf, torch.float32, rows, what="final")
+        ga = tb.linear_recurrence_backward(gate, a[0], x, log_gate=True)
+        gb = tb.linear_recurrence_backward(gate, a[0], apart, log_gate=True)
+        wx, wg, wi, size = reference_backward(gate, a[0], x, None, None, None, True)
+        for g in (ga, gb):
+            close(g[0], wx, x.dtype, rows, what="dx")
+            close(g[1], wg, gate.dtype, rows, float(wx.abs().max() * a[0].float().abs().max().cpu()) + float(size.max()), "dgate")
+
+
+@pytest.mark.parametrize("heads", [96, 3])
+def test_one_long_sequence(cuda_device, heads):
+    """Hundreds of tiles in a row, most of them in work at once: against 64 bits, and the same to the bit every time."""
+    rng = np.random.default_rng(13)
+    x, gate = make(rng, (1, 20011), 96, heads, "f32", "f32", True, cuda_device)
+    y, final = tb.linear_recurrence(x, gate, log_gate=True)
+    wy, wf = reference(x, gate, None, None, True)
+    m = memory_of(gate, True, 20011)
+    close(y, wy, torch.float32, m, what="y")
+    close(final, wf, torch.float32, m, float(wy.abs().max()), "final")
+    dy = torch.from_numpy(rng.standard_normal((1, 20011, 96))).to(cuda_device, torch.float32)
+    grads = tb.linear_recurrence_backward(gate, y, dy, log_gate=True)
+    wx, wg, wi, size = reference_backward(gate, y, dy, None, None, None, True)
+    close(grads[0], wx, torch.float32, m, what="dx")
+    close(grads[1], wg, torch.float32, m, float(wx.abs().max() * wy.abs().max()) * (96 // heads) + float(size.max()), "dgate")
+    for _ in range(5):
+        again = tb.linear_recurrence(x, gate, log_gate=True)
+        g2 = tb.linear_recurrence_backward(gate, y, dy, log_gate=True)
+        assert torch.equal(again[0], y) and torch.equal(again[1], final) and all(torch.equal(a, b) for a, b in zip(grads, g2))
+
+
+def test_refusals_of_tensors(cuda_device):
+    x = torch.zeros(2, 5, 8, device=cuda_device)
+    offsets = torch.tensor([0, 5], device=cuda_device)
+    bad = [dict(x=x[0]), dict(offsets=offsets), dict(gate=x[:1]), dict(gate=x[..., :3]), dict(x=x.double()),
+           dict(gate=x.half()), dict(initial=torch.zeros(2, 4, device=cuda_device)), dict(out=x[:1].expand(2, 5, 8)),
+           dict(initial=torch.zeros(2, 8)), dict(x=torch.zeros(2, 8, 5, device=cuda_device).transpose(1, 2)),
+           dict(out=torch.zeros(2, 5, 8, device=cuda_device, dtype=torch.half)), dict(gate=x[..., :0])]
+    for change in bad:
+        with pytest.raises((ValueError, TypeError)):
+            tb.linear_recurrence(**{"x": x, "gate": x, **change})
+    with pytest.raises(ValueError):
+        tb.linear_recurrence_backward(x, x, x[:, :4])
+    state = torch.zeros(3, 8, device=cuda_device)
+    for change in (dict(state=state.half()), dict(slots=torch.zeros(2, device=cuda_device)), dict(gate=x[0, :1]),
+                   dict(slots=torch.zeros(2, dtype=torch.int32)), dict(state=state[:, :4]), dict(state=state[:1].expand(3, 8))):
+        with pytest.raises((ValueError, TypeError)):
+            tb.linear_recurrence_step(**{"state": state, "x": x[0], "gate": x[0], "slots": torch.zeros(5, dtype=torch.int32, device=cuda_device), **change})
+    with pytest.raises(ValueError):
+        tb.linear_recurrence_step(state, x[0], x[0])  # more rows than states

@@ -290,3 +290,22 @@ def test_layer_of_recurrence_and_routing(cuda_device):
     for got, want in ((dx, x64.grad), (dgate, g64.grad), (y.T @ dz, r64.grad)):
         # single-precision products of 64 channels in front and behind: a few hundred roundings of 2^-24
         assert float((got.double().cpu() - want).abs().max()) <= 1e-4 * float(want.abs().max())
+
+
+def test_refusals_of_tensors(cuda_device):
+    z, ids = torch.zeros(6, 8, device=cuda_device), torch.zeros(6, 2, dtype=torch.int64, device=cuda_device)
+    mask = torch.ones(6, dtype=torch.bool, device=cuda_device)
+    for call in (lambda: tb.expert_counts(ids.float(), 8), lambda: tb.expert_counts(ids, 8, mask=mask[:5]),
+                 lambda: tb.expert_counts(ids, 8, mask=mask.float()), lambda: tb.expert_counts(ids.T, 8), lambda: tb.expert_counts(ids, 8, mask=mask.cpu()),
+                 lambda: tb.balance_loss(z, ids[:5]), lambda: tb.balance_loss(z.double(), ids), lambda: tb.balance_loss(z[0], ids),
+                 lambda: tb.balance_loss(z, ids, offsets=torch.zeros(2, device=cuda_device)), lambda: tb.balance_loss(z.T, ids),
+                 lambda: tb.balance_loss_backward(z, z, torch.zeros(1, device=cuda_device)),
+                 lambda: tb.balance_loss_backward(z, z[:1].contiguous(), torch.zeros(2, device=cuda_device)),
+                 lambda: tb.balance_loss_backward(z, z[:1].contiguous(), torch.zeros(1, device=cuda_device), out=z[:1].expand(6, 8))):
+        with pytest.raises((ValueError, TypeError)):
+            call()
+    for experts in (0, 8193):
+        with pytest.raises(tb.Tb200Error):
+            tb.expert_counts(ids, experts)
+    with pytest.raises(tb.Tb200Error):
+        tb.balance_loss(torch.zeros(6, 1025, device=cuda_device), ids)

@@ -7,7 +7,11 @@
 // Layout. A row of logits is spread over 1 to 32 lanes, eight experts to a lane and step, so that a lane loads 16 bytes
 // of a 16-bit type at once, sums over a row are shuffles among its lanes, and the column sums stay in the lane's own
 // registers for all rows of a CTA. Registers are summed over warps in a fixed order, and the CTAs' sums are added as
-// 64-bit integers, whose order does not matter: reproducible, and finished by whichever CTA is last.
+// 64-bit integers, whose order does not matter: reproducible, and finished by whichever CTA is last. Rows are fetched a
+// step ahead of the arithmetic, which is what bounds these kernels: 150 instructions a row of 256 experts, half of them
+// exponentials, conversions and shuffles. Measured (calls): loss of 65536 x 256 bf16 with 8 ids a row 22.5 us (floor
+// 5.6), gradient of 131072 x 128 bf16 20.5 us (floor 10.3; 262144 x 256 in 64 us, 4.2 TB/s), 262144 x 8 ids of 64 bits
+// 12 us in the kernel (floor 2.6; shared-memory atomics and a memory latency for each batch of ids).
 #include <cuda_runtime.h>
 
 #include <cstdint>

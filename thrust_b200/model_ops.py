@@ -121,6 +121,8 @@ def _output(out: Optional[torch.Tensor], like: torch.Tensor, name: str) -> torch
         return _empty_like(like)
     if out.shape != like.shape or out.dtype != like.dtype:
         raise ValueError(f"out must have the shape and type of {name}")
+    if any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
+        raise ValueError("the rows of out share memory")
     return out
 
 
