@@ -209,22 +209,30 @@ __device__ bool mark_rows(const RecArgs& p, uint64_t r0, uint64_t r1, bool at_en
     if (end < hi) hi = end;
   }
   if (lo > 0 && lo <= p.sequences && offset_at(p, lo) > r1) return true;  // inner rows of one sequence
-  for (uint64_t j = lo + lane; j <= p.sequences; j += kWarp) {
-    const uint64_t v = offset_at(p, j);
-    if (v > r1) break;
-    if (j > 0 && v > r0 && offset_at(p, j - 1) < v) {  // sequence j - 1 ends in front of boundary j
-      m.seq[v - 1 - r0] = (int)(j - 1);
-      atomicOr(reinterpret_cast<unsigned*>(m.kind) + (v - 1 - r0) / 4, 2u << (8 * ((v - 1 - r0) % 4)));
-    }
-    if (j < p.sequences && (v < r1 || at_end)) {
-      const uint64_t end = offset_at(p, j + 1);
-      if (end > v && v < r1 && v >= r0) {
-        m.seq[v - r0] = (int)j;
-        atomicOr(reinterpret_cast<unsigned*>(m.kind) + (v - r0) / 4, 1u << (8 * ((v - r0) % 4)));
-      } else if (end <= v && p.last != nullptr) {
-        for (uint32_t c = c0; c < c0 + count; ++c) p.last[j * p.channels + c] = p.first ? p.first[j * p.channels + c] : 0.0f;
+  for (uint64_t base = lo; base <= p.sequences; base += kWarp) {
+    const uint64_t j = base + lane;
+    const bool here = j <= p.sequences && offset_at(p, j) <= r1;
+    bool empty = false;
+    if (here) {
+      const uint64_t v = offset_at(p, j);
+      if (j > 0 && v > r0 && offset_at(p, j - 1) < v) {  // sequence j - 1 ends in front of boundary j
+        m.seq[v - 1 - r0] = (int)(j - 1);
+        atomicOr(reinterpret_cast<unsigned*>(m.kind) + (v - 1 - r0) / 4, 2u << (8 * ((v - 1 - r0) % 4)));
+      }
+      if (j < p.sequences && (v < r1 || at_end)) {
+        const uint64_t end = offset_at(p, j + 1);
+        if (end > v && v < r1 && v >= r0) {
+          m.seq[v - r0] = (int)j;
+          atomicOr(reinterpret_cast<unsigned*>(m.kind) + (v - r0) / 4, 1u << (8 * ((v - r0) % 4)));
+        }
+        empty = end <= v;
       }
     }
+    for (unsigned left = __ballot_sync(0xffffffffu, empty && p.last != nullptr); left != 0; left &= left - 1) {
+      const uint64_t row = (base + __ffs(left) - 1) * p.channels;  // all lanes hand its states through
+      for (uint32_t c = c0 + lane; c < c0 + count; c += kWarp) p.last[row + c] = p.first ? p.first[row + c] : 0.0f;
+    }
+    if (!__all_sync(0xffffffffu, here)) break;
   }
   return false;
 }
@@ -290,7 +298,6 @@ __device__ __forceinline__ void describe(const RecArgs& p, unsigned id, unsigned
 // Which of the warp's rows are what: bit r of a mask is row r.
 struct RowKinds {
   unsigned inside, begin, end;  // rows of a sequence; its first and last one with the recurrence
-  int seq;                      // lane r: the sequence of row r, where that is a first or last one
 };
 template <int TILE, bool BACK>
 __device__ void marks_of_tile(const RecArgs& p, const TileInfo& w, Marks<TILE>& m) {  // for one warp
@@ -367,6 +374,7 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
   __shared__ Marks<TILE> s_marks[4];  // a ring
   // of the stretches: bit 0, a sequence begins among the rows; bit 1, there are rows in front of that
   __shared__ __align__(8) unsigned char s_kinds[2][kWarps];
+  __shared__ int s_seq[2][kWarps][R];  // sequences of first and last rows, by the parity of the tile
   __shared__ TileInfo s_tiles[8];  // of the CTA, a ring
   __shared__ float s_heads[SHARED && BACK ? kWarps : 1][SHARED && BACK ? R : 1][kWarp + 1];
   __shared__ unsigned long long s_landed[kStages];  // a stage's boxes
@@ -627,21 +635,21 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
       copies_issued();
     }
     const bool plain = p.offsets ? s_marks[i & 3].plain : w.plain;
-    RowKinds kinds{ALL, 0, 0, 0};
+    RowKinds kinds{ALL, 0, 0};
     if (some) {
       // ---- first and last rows of sequences ---------------------------------------------------------------
       if (!plain) {
         const int n = max(0, min(R, w.rows - warp * R));
         const bool valid = lane < n;
+        int seq = w.chain;  // of row `lane`, where that is a first or last one
         const int64_t mine = valid ? (BACK ? w.row - warp * R - lane : w.row + warp * R + lane) : 0;  // lane r: row r
         unsigned m_first = 0, m_last = 0;
         kinds.inside = (1u << n) - 1;
-        kinds.seq = w.chain;
         if (p.offsets != nullptr) {
           const uint64_t lo = (uint64_t)w.tile * TILE, hi = min(lo + TILE, p.chain_rows);
           const int64_t r0 = BACK ? p.chain_rows - hi : lo;
           const unsigned kind = valid ? s_marks[i & 3].kind[mine - r0] : 0;
-          if (kind) kinds.seq = s_marks[i & 3].seq[mine - r0];
+          if (kind) seq = s_marks[i & 3].seq[mine - r0];
           m_first = __ballot_sync(0xffffffffu, kind & 1);
           m_last = __ballot_sync(0xffffffffu, kind & 2);
           kinds.inside = __ballot_sync(0xffffffffu, valid && (uint64_t)mine >= s_marks[i & 3].from && (uint64_t)mine < s_marks[i & 3].to);
@@ -651,12 +659,14 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
         } else {  // sequences of equal length behind one another
           const uint64_t s = p.chain_rows >> 32 ? (uint64_t)mine / p.length : (uint32_t)mine / (uint32_t)p.length;
           const uint64_t t = (uint64_t)mine - s * p.length;
-          kinds.seq = (int)s;
+          seq = (int)s;
           m_first = __ballot_sync(0xffffffffu, valid && t == 0);
           m_last = __ballot_sync(0xffffffffu, valid && t == p.length - 1);
         }
         kinds.begin = BACK ? m_last : m_first;
         kinds.end = BACK ? m_first : m_last;
+        if (lane < R) s_seq[k][warp][lane] = seq;
+        __syncwarp();
       }
 
       // ---- first pass: the stretch's A and B ----------------------------------------------------------------
@@ -681,10 +691,10 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
           if (!inner && !(kinds.inside >> r & 1)) continue;
           const bool begin = !inner && (kinds.begin >> r & 1);
           if (begin) {
-            const int s = __shfl_sync(0xffffffffu, kinds.seq, r);
+            const uint64_t s = s_seq[k][warp][r];
 #pragma unroll
             for (int e = 0; e < V; ++e)
-              B[e] = p.first && lane * V < (int)w.count ? p.first[(uint64_t)s * p.channels + w.c0 + lane * V + e] : 0.0f;
+              B[e] = p.first && lane * V < (int)w.count ? p.first[s * p.channels + w.c0 + lane * V + e] : 0.0f;
           }
           float a[GV], av[V], xv[V];
 #pragma unroll
@@ -786,10 +796,10 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
           if (!in && !(p.fill && warp * R + r < pw.rows)) continue;
           const bool begin = !inner && (pk.begin >> r & 1);
           const bool end = !inner && (pk.end >> r & 1);
-          const int s = inner ? 0 : __shfl_sync(0xffffffffu, pk.seq, r);
+          const uint64_t s = inner ? 0 : s_seq[k ^ 1][warp][r];
           if (begin) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) h[e] = p.first && live ? p.first[(uint64_t)s * p.channels + ch + e] : 0.0f;
+            for (int e = 0; e < V; ++e) h[e] = p.first && live ? p.first[s * p.channels + ch + e] : 0.0f;
           }
           float a[GV], av[V], xv[V], out[V], dg[V];
 #pragma unroll
@@ -809,7 +819,7 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
             for (int e = 0; e < V; ++e) prev[e] = to_f32<T>(before[r].v[e]);
             if (end) {
 #pragma unroll
-              for (int e = 0; e < V; ++e) prev[e] = p.initial && live ? p.initial[(uint64_t)s * p.channels + ch + e] : 0.0f;
+              for (int e = 0; e < V; ++e) prev[e] = p.initial && live ? p.initial[s * p.channels + ch + e] : 0.0f;
             }
             add_n(out, xv, h);
             mul_n(h, av, out);
@@ -840,7 +850,7 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
           }
           if (in && end && p.last && live) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) p.last[(uint64_t)s * p.channels + ch + e] = h[e];
+            for (int e = 0; e < V; ++e) p.last[s * p.channels + ch + e] = h[e];
           }
         }
       };
