@@ -166,7 +166,7 @@ __device__ __forceinline__ float wait_for_state(const unsigned long long* maps, 
                                                 unsigned tile, int* status) {
   float h = 0.0f;
   for (unsigned polls = 0; !look_for_state(maps, states, step, tile, h); ++polls) {
-    if ((polls & 63u) == 63u && __any_sync(0xffffffffu, ld_relaxed_s32(status) != 0)) break;  // someone else gave up
+    if ((polls & 63u) == 63u && __any_sync(0xffffffffu, ld_relaxed_s32(status) == (int)TB200_ERR_WAIT_TIMEOUT)) break;  // someone else gave up
     if (polls >= kSpinLimit) {
       note_timeout(status, kSiteLookback, tile, 0);
       break;
@@ -354,6 +354,19 @@ __device__ __forceinline__ bool mbar_test(unsigned long long* bar, unsigned pari
 }
 __device__ __forceinline__ void barrier_arrive(int id, int count) {
   asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(count) : "memory");
+}
+
+// Waits for a phase of a barrier; where that takes about a second, or someone else has given up waiting, carries on with
+// the status raised. Other errors in the status do not end a wait: boxes may be on their way.
+__device__ __forceinline__ void mbar_wait(unsigned long long* bar, unsigned parity, int* status) {
+  for (unsigned spins = 0; !mbar_try_wait(bar, parity); ++spins) {
+    if ((spins & 1023u) != 1023u) continue;
+    if (ld_relaxed_s32(status) == (int)TB200_ERR_WAIT_TIMEOUT) return;
+    if (spins >= kSpinLimit) {
+      note_timeout(status, kSiteMbarrier, smem_u32(bar), parity);
+      return;
+    }
+  }
 }
 
 // One CTA on an SM, which takes tile after tile. Eight warps compute: the first pass over tile i as soon as its rows have
@@ -566,7 +579,7 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
       bool need = false;
       if (some) {
         tile = s_tiles[i & 7].tile;
-        mbar_wait_bounded(maps_ready, i >> 1 & 1, &p.hdr->status);
+        mbar_wait(maps_ready, i >> 1 & 1, &p.hdr->status);
         // all warps are done with the tile before the parked one: its stage is free
         if (S::BOXES && threadIdx.x == ASKS && s_tiles[(i + 2) & 7].id < total) fetch_boxes(s_tiles[(i + 2) & 7], (i + 2) % kStages);
         const unsigned long long kinds = *reinterpret_cast<const unsigned long long*>(s_kinds[k]);
@@ -670,7 +683,7 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
       }
 
       // ---- first pass: the stretch's A and B ----------------------------------------------------------------
-      if constexpr (S::BOXES) mbar_wait_bounded(&s_landed[stage], i / kStages & 1, &p.hdr->status);
+      if constexpr (S::BOXES) mbar_wait(&s_landed[stage], i / kStages & 1, &p.hdr->status);
       else asm volatile("cp.async.wait_group 1;" ::: "memory");  // all but the copies of the tile behind
       // all values first: nothing below comes between the loads
       Pack<G, GV> gate[R];
