@@ -651,6 +651,9 @@ extern "C" int tb200_balance_loss(void* d_temp, size_t* temp_bytes, const tb200_
     const uint64_t slots = (uint64_t)per_sm * sms, least = (uint64_t)kRouteWarps * (kWarp / decltype(l)::value);
     a.rows_of_cta = (rows + slots - 1) / slots;
     if (a.rows_of_cta < least) a.rows_of_cta = least;
+    // Up to 2^15 probabilities one CTA does it all: no clear of the scratch in front, nothing to join behind. 1024 rows
+    // of 8 experts: kernel 9.4 us instead of 8.4 us on four CTAs, the call 17.7 us instead of 20.3 us.
+    if (rows * experts <= 32768) a.rows_of_cta = rows;
     const unsigned grid = (unsigned)((rows + a.rows_of_cta - 1) / a.rows_of_cta);
     if (grid > 1) TB200_CUDA_TRY(cudaMemsetAsync(d_temp, 0, need, stream));
     kernel<<<grid, kRouteThreads, 0, stream>>>(a);

@@ -116,6 +116,11 @@ def _empty_like(t: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
 
 
+def _new(shape, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    """A fresh contiguous tensor of one or two dimensions, the cheapest way there is."""
+    return torch.empty_strided(shape, (1,) if len(shape) == 1 else (shape[1], 1), dtype=dtype, device=device)
+
+
 def _output(out: Optional[torch.Tensor], like: torch.Tensor, name: str) -> torch.Tensor:
     if out is None:
         return _empty_like(like)
@@ -129,7 +134,7 @@ def _output(out: Optional[torch.Tensor], like: torch.Tensor, name: str) -> torch
 def _scratch(need: int, like: torch.Tensor, temp: Optional[torch.Tensor]) -> torch.Tensor:
     if temp is not None and temp.numel() >= need:
         return temp
-    return like.new_empty((need,), dtype=torch.uint8)
+    return _new((need,), torch.uint8, like.device)
 
 
 @lru_cache(maxsize=512)
@@ -182,7 +187,7 @@ def linear_recurrence(x: torch.Tensor, gate: torch.Tensor, initial: Optional[tor
     iptr = _states(initial, states, "initial")
     out = _output(out, x, "x")
     arrays = _arrays(_rows(gate, "gate"), _rows(x, "x"), _rows(out, "out"))
-    final = x.new_empty(states, dtype=torch.float32)
+    final = _new(states, torch.float32, x.device)
     temp = _scratch(_recurrence_bytes(False, *dims), x, temp)
     shape, have, stream = capi.RecurrenceShape(*dims), C.c_size_t(temp.numel()), _raw_stream(index)
     _call(capi.lib.tb200_linear_recurrence, "tb200_linear_recurrence", index, temp.data_ptr(), C.byref(have),
@@ -209,7 +214,7 @@ def linear_recurrence_backward(gate: torch.Tensor, y: torch.Tensor, dy: torch.Te
     states = (dims[0], dims[2])
     iptr, fptr = _states(initial, states, "initial"), _states(dfinal, states, "dfinal")
     dx, dgate = _empty_like(dy), _empty_like(gate)
-    dinitial = dy.new_empty(states, dtype=torch.float32)
+    dinitial = _new(states, torch.float32, dy.device)
     arrays = _arrays(_rows(gate, "gate"), _rows(y, "y"), _rows(dy, "dy"), _rows(dx, "dx"), _rows(dgate, "dgate"))
     temp = _scratch(_recurrence_bytes(True, *dims), dy, temp)
     shape, have, stream = capi.RecurrenceShape(*dims), C.c_size_t(temp.numel()), _raw_stream(index)
@@ -312,7 +317,8 @@ def expert_counts(ids: torch.Tensor, experts: int, mask: Optional[torch.Tensor] 
     rows, k, stride, width = _ids(ids)
     mptr = _mask(mask, rows)
     temp = _scratch(_counts_bytes(experts), ids, temp)
-    counts, begins = ids.new_empty((experts,), dtype=torch.int64), ids.new_empty((experts + 1,), dtype=torch.int64)
+    device = ids.device
+    counts, begins = _new((experts,), torch.int64, device), _new((experts + 1,), torch.int64, device)
     have, raw = C.c_size_t(temp.numel()), _raw_stream(index)
     _call(capi.lib.tb200_expert_counts, "tb200_expert_counts", index, temp.data_ptr(), C.byref(have), ids.data_ptr(), rows,
           k, stride, width, mptr, experts, counts.data_ptr(), begins.data_ptr(), raw)
@@ -351,9 +357,8 @@ def balance_loss(logits: torch.Tensor, ids: torch.Tensor, mask: Optional[torch.T
         raise ValueError("logits and ids differ in rows")
     mptr, arrays = _mask(mask, rows), _arrays(_rows(logits, "logits"))
     temp = _scratch(_balance_bytes(dtype, obytes, sequences, experts), logits, temp)
-    loss = logits.new_empty((sequences,), dtype=torch.float32)
-    counts = logits.new_empty((sequences, experts), dtype=torch.int64)
-    weights = logits.new_empty((sequences, experts), dtype=torch.float32)
+    device, cells = logits.device, (sequences, experts)
+    loss, counts, weights = _new((sequences,), torch.float32, device), _new(cells, torch.int64, device), _new(cells, torch.float32, device)
     have, stream = C.c_size_t(temp.numel()), _raw_stream(index)
     _call(capi.lib.tb200_balance_loss, "tb200_balance_loss", index, temp.data_ptr(), C.byref(have), arrays[0], dtype,
           ids.data_ptr(), k, stride, width, mptr, optr, obytes, sequences, rows, experts, loss.data_ptr(),
