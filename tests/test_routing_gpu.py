@@ -219,6 +219,45 @@ def test_strided_logits_and_sequences_without_rows(cuda_device):
         assert e.value.code == capi.ERR_INVALID_ARGUMENT
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("experts", [8, 13, 64, 256, 600])
+def test_rows_behind_the_last_sequence_are_not_looked_at(cuda_device, dtype, experts):
+    """The tail of a padded buffer holds anything: NaN, infinities, whatever. Its gradients are zero, masked or not."""
+    rng = np.random.default_rng(experts)
+    lengths, tail = [0, 30, 0, 70, 0], 41
+    rows = sum(lengths) + tail
+    z = torch.from_numpy(rng.standard_normal((rows, experts))).to(cuda_device, TYPES[dtype])
+    ids = torch.from_numpy(rng.integers(0, experts, size=(rows, 2))).to(cuda_device)
+    offsets = torch.from_numpy(np.cumsum([0, *lengths])).to(cuda_device, torch.int32)
+    garbage, garbage_ids = z.clone(), ids.clone()
+    end = rows - tail
+    garbage[end::4] = float("nan")
+    garbage[end + 1::4] = float("inf")
+    garbage[end + 2::4, 1] = float("inf")
+    garbage[end + 3::4, -1] = float("nan")
+    garbage_ids[end:] = -(10 ** 12)
+    odd = torch.arange(rows, device=cuda_device) % 3 != 0
+    dloss = torch.full((len(lengths),), 1000.0, device=cuda_device)
+    for mask in (None, odd):
+        want = tb.balance_loss(z, ids, mask=mask, offsets=offsets)
+        got = tb.balance_loss(garbage, garbage_ids, mask=mask, offsets=offsets)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        grad = tb.balance_loss_backward(z, want[2], dloss, mask=mask, offsets=offsets)
+        out = torch.full_like(z, 3.0)
+        tb.balance_loss_backward(garbage, want[2], dloss, mask=mask, offsets=offsets, out=out)
+        assert torch.equal(out, grad) and not out[end:].any() and out[:end].any()
+        none = tb.balance_loss_backward(garbage, want[2][:0].contiguous(), dloss[:0], mask=mask, offsets=offsets[:1])
+        assert none.shape == z.shape and not none.any()  # no sequences at all
+    # what belongs to one sequence alone does not reach another: its weights, its dloss, its rows
+    dloss[1] = float("inf")
+    weights = want[2].clone()
+    weights[1, 0] = float("nan")
+    garbage[:lengths[1]] = float("nan")
+    out = tb.balance_loss_backward(garbage, weights, dloss, mask=odd, offsets=offsets)
+    assert torch.equal(out[lengths[1]:], grad[lengths[1]:]) and not out[~odd].any()
+    assert torch.isnan(out[:lengths[1]][odd[:lengths[1]]]).all()
+
+
 def test_captured_and_replayed(cuda_device):
     z, ids, mask, _, _ = build((5000, 128, 4, "bf16"), cuda_device, True)
     dloss = torch.full((1,), 100.0, device=cuda_device)

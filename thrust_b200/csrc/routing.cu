@@ -479,10 +479,11 @@ __global__ void __launch_bounds__(kRouteThreads, J == 1 ? 3 : 1) balance_backwar
       const float dot = lanes_sum<L>(part[0] + part[1]) * share;
       float less[J * 8], factor[J * 8], d[J * 8];
       fill_n(less, -dot);
-      fill_n(factor, kept ? scale * share : 0.0f);
+      fill_n(factor, scale * share);
       add_n(d, w, less);
       mul_n(e, e, factor);
       mul_n(d, d, e);
+      if (!kept) fill_n(d, 0.0f);  // not by a factor of zero: rows of no sequence may hold NaN or infinities
       if (!valid) continue;
 #pragma unroll
       for (int j = 0; j < J; ++j) {
