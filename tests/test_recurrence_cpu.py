@@ -72,3 +72,59 @@ def test_python_front_end_refuses_cpu_tensors():
     with pytest.raises(TypeError):  # no other algorithm takes the 16-bit floating types
         tb.tb200_dtype(torch.zeros(2, dtype=torch.bfloat16))
     assert capi.lib.tb200_scan(None, C.byref(C.c_size_t(0)), None, None, 4, capi.BF16, 0, None, None) == capi.ERR_UNSUPPORTED
+
+
+def rows_at(address):
+    r = capi.Rows.from_address(address)
+    return r.data, r.row_stride, r.sequence_stride
+
+
+@pytest.mark.parametrize("interrupted", ["_new", "_scratch", "_raw_stream", "_call"])
+def test_a_call_within_a_call_keeps_its_arrays(monkeypatch, interrupted):
+    """A finaliser or a signal handler may make one of these calls while another one is being put together."""
+    ops = tb.model_ops
+    seen, armed = [], []
+    small = torch.zeros(1, 2, 3)
+    inner = {"recurrence": lambda: ops.linear_recurrence(small, small, sync=False),
+             "balance": lambda: ops.balance_loss_backward(small[0], small[0, :1].contiguous(), torch.zeros(1))}
+
+    def record(function, what, index, *args):
+        seen.append((what, [rows_at(a) for a in args if isinstance(a, int) and a in rooms()]))
+
+    def rooms():
+        return {address for room in all_rooms for address in room.at}
+
+    all_rooms, room_init = [], ops._Room.__init__
+    monkeypatch.setattr(ops._Room, "__init__", lambda self: (room_init(self), all_rooms.append(self))[0])
+    monkeypatch.setattr(ops, "_rooms", [])
+    monkeypatch.setattr(ops, "_device_of", lambda name, t: 0)
+    monkeypatch.setattr(ops, "_same_device", lambda index, name, t: None)
+    monkeypatch.setattr(ops, "_raw_stream", lambda index: 0)
+    monkeypatch.setattr(ops, "_call", record)
+    plain = getattr(ops, interrupted)
+
+    def interrupt(*args):
+        if armed:
+            armed.pop()()
+        return plain(*args)
+
+    monkeypatch.setattr(ops, interrupted, interrupt)
+    x, gate = torch.zeros(2, 50, 8), torch.zeros(2, 50, 4)
+    state, row = torch.zeros(7, 8), torch.zeros(5, 8)
+    z, ids = torch.zeros(40, 16), torch.zeros(40, 2, dtype=torch.int64)
+    calls = {"tb200_linear_recurrence": (lambda: ops.linear_recurrence(x, gate, sync=False), [gate, x]),
+             "tb200_linear_recurrence_backward": (lambda: ops.linear_recurrence_backward(gate, x, x, sync=False), [gate, x, x]),
+             "tb200_linear_recurrence_step": (lambda: ops.linear_recurrence_step(state, row, row), [row, row]),
+             "tb200_balance_loss": (lambda: ops.balance_loss(z, ids, sync=False), [z]),
+             "tb200_balance_loss_backward": (lambda: ops.balance_loss_backward(z, z[:1].contiguous(), torch.zeros(1)), [z])}
+    for what, (call, inputs) in calls.items():
+        for other in inner.values():
+            del seen[:]
+            armed[:] = [other]
+            call()
+            found = [arrays for name, arrays in seen if name == what and len(arrays) >= len(inputs) and
+                     arrays[0][0] == inputs[0].data_ptr()]
+            assert len(found) == 1, (what, interrupted, seen)
+            for got, t in zip(found[0], inputs):
+                assert got == (t.data_ptr(), t.stride(-2), t.stride(0) if t.dim() == 3 else 0), (what, interrupted)
+    assert 1 <= len(all_rooms) <= 2  # given back and used again

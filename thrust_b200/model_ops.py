@@ -8,9 +8,8 @@ here records itself for autograd.
 from __future__ import annotations
 
 import ctypes as C
-import threading
 from functools import lru_cache
-from typing import Optional, Tuple
+from typing import List, Optional, Tuple
 
 import torch
 
@@ -77,8 +76,8 @@ def _rows(t: torch.Tensor, name: str) -> Tuple[int, int, int]:
     return t.data_ptr(), stride[-2], stride[0] if len(stride) == 3 else 0
 
 
-class _Words(threading.local):
-    """A thread's room for five tb200_rows one behind the other; a call has read them when it returns."""
+class _Room:
+    """Room for five tb200_rows one behind the other, as a call hands them over; it has read them when it returns."""
 
     def __init__(self):
         self.words = (C.c_uint64 * 15)()
@@ -86,14 +85,20 @@ class _Words(threading.local):
         self.at = tuple(base + 24 * i for i in range(5))
 
 
-_words = _Words()
+# Rooms that no call is using. A call takes one for itself, so that neither another thread nor a finaliser or signal handler
+# that makes such a call in between writes into it; pop and append are one step each.
+_rooms: List[_Room] = []
 
 
-def _arrays(*rows) -> Tuple[int, ...]:
-    """The addresses of these arrays of rows, written into the thread's room."""
+def _arrays(*rows) -> Tuple[_Room, Tuple[int, ...]]:
+    """These arrays of rows in a room of their own, and their addresses there. The caller gives the room back."""
+    try:
+        room = _rooms.pop()
+    except IndexError:
+        room = _Room()
     flat = [w for r in rows for w in r]
-    _words.words[:len(flat)] = flat
-    return _words.at[:len(rows)]
+    room.words[:len(flat)] = flat
+    return room, room.at[:len(rows)]
 
 
 def _states(t: Optional[torch.Tensor], shape, name: str) -> Optional[int]:
@@ -186,12 +191,13 @@ def linear_recurrence(x: torch.Tensor, gate: torch.Tensor, initial: Optional[tor
     states = (dims[0], dims[2])
     iptr = _states(initial, states, "initial")
     out = _output(out, x, "x")
-    arrays = _arrays(_rows(gate, "gate"), _rows(x, "x"), _rows(out, "out"))
+    room, arrays = _arrays(_rows(gate, "gate"), _rows(x, "x"), _rows(out, "out"))
     final = _new(states, torch.float32, x.device)
     temp = _scratch(_recurrence_bytes(False, *dims), x, temp)
     shape, have, stream = capi.RecurrenceShape(*dims), C.c_size_t(temp.numel()), _raw_stream(index)
     _call(capi.lib.tb200_linear_recurrence, "tb200_linear_recurrence", index, temp.data_ptr(), C.byref(have),
           C.byref(shape), optr, *arrays, iptr, final.data_ptr(), stream)
+    _rooms.append(room)
     _status(temp, stream, "tb200_linear_recurrence", index, sync)
     return out, final
 
@@ -215,11 +221,12 @@ def linear_recurrence_backward(gate: torch.Tensor, y: torch.Tensor, dy: torch.Te
     iptr, fptr = _states(initial, states, "initial"), _states(dfinal, states, "dfinal")
     dx, dgate = _empty_like(dy), _empty_like(gate)
     dinitial = _new(states, torch.float32, dy.device)
-    arrays = _arrays(_rows(gate, "gate"), _rows(y, "y"), _rows(dy, "dy"), _rows(dx, "dx"), _rows(dgate, "dgate"))
+    room, arrays = _arrays(_rows(gate, "gate"), _rows(y, "y"), _rows(dy, "dy"), _rows(dx, "dx"), _rows(dgate, "dgate"))
     temp = _scratch(_recurrence_bytes(True, *dims), dy, temp)
     shape, have, stream = capi.RecurrenceShape(*dims), C.c_size_t(temp.numel()), _raw_stream(index)
     _call(capi.lib.tb200_linear_recurrence_backward, "tb200_linear_recurrence_backward", index, temp.data_ptr(),
           C.byref(have), C.byref(shape), optr, *arrays, iptr, fptr, dinitial.data_ptr(), stream)
+    _rooms.append(room)
     _status(temp, stream, "tb200_linear_recurrence_backward", index, sync)
     return dx, dgate, dinitial
 
@@ -259,9 +266,10 @@ def linear_recurrence_step(state: torch.Tensor, x: torch.Tensor, gate: torch.Ten
     elif apart < channels:
         raise ValueError("the states of the pool overlap")
     out = _output(out, x, "x")
-    arrays = _arrays(_rows(gate, "gate"), _rows(x, "x"), _rows(out, "out"))
+    room, arrays = _arrays(_rows(gate, "gate"), _rows(x, "x"), _rows(out, "out"))
     _call(capi.lib.tb200_linear_recurrence_step, "tb200_linear_recurrence_step", index, pool, ss[0], apart, sptr, sbytes,
           *arrays, rows, channels, gs[1], xd, gd, 1 if log_gate else 0, _raw_stream(index))
+    _rooms.append(room)
     return out
 
 
@@ -355,7 +363,7 @@ def balance_loss(logits: torch.Tensor, ids: torch.Tensor, mask: Optional[torch.T
     id_rows, k, stride, width = _ids(ids)
     if id_rows != rows:
         raise ValueError("logits and ids differ in rows")
-    mptr, arrays = _mask(mask, rows), _arrays(_rows(logits, "logits"))
+    mptr, (room, arrays) = _mask(mask, rows), _arrays(_rows(logits, "logits"))
     temp = _scratch(_balance_bytes(dtype, obytes, sequences, experts), logits, temp)
     device, cells = logits.device, (sequences, experts)
     loss, counts, weights = _new((sequences,), torch.float32, device), _new(cells, torch.int64, device), _new(cells, torch.float32, device)
@@ -363,6 +371,7 @@ def balance_loss(logits: torch.Tensor, ids: torch.Tensor, mask: Optional[torch.T
     _call(capi.lib.tb200_balance_loss, "tb200_balance_loss", index, temp.data_ptr(), C.byref(have), arrays[0], dtype,
           ids.data_ptr(), k, stride, width, mptr, optr, obytes, sequences, rows, experts, loss.data_ptr(),
           counts.data_ptr(), weights.data_ptr(), stream)
+    _rooms.append(room)
     _status(temp, stream, "tb200_balance_loss", index, sync)
     return loss, counts, weights
 
@@ -380,7 +389,8 @@ def balance_loss_backward(logits: torch.Tensor, weights: torch.Tensor, dloss: to
     wptr = _states(weights, (sequences, experts), "weights")
     lptr = _states(dloss, (sequences,), "dloss")
     out = _output(out, logits, "logits")
-    mptr, arrays = _mask(mask, rows), _arrays(_rows(logits, "logits"), _rows(out, "out"))
+    mptr, (room, arrays) = _mask(mask, rows), _arrays(_rows(logits, "logits"), _rows(out, "out"))
     _call(capi.lib.tb200_balance_loss_backward, "tb200_balance_loss_backward", index, arrays[0], dtype, wptr, lptr, mptr,
           optr, obytes, sequences, rows, experts, arrays[1], _raw_stream(index))
+    _rooms.append(room)
     return out
