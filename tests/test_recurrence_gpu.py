@@ -441,6 +441,24 @@ def test_one_long_sequence(cuda_device, heads):
         assert torch.equal(again[0], y) and torch.equal(again[1], final) and all(torch.equal(a, b) for a, b in zip(grads, g2))
 
 
+@pytest.mark.parametrize("sequences,rows,channels,heads,dtype", [
+    (700, 40, 136, 136, "bf16"), (700, 40, 135, 135, "bf16"), (900, 30, 64, 4, "f32"), (3, 900, 64, 64, "bf16")])
+def test_scratch_of_a_call_that_gave_up(cuda_device, sequences, rows, channels, heads, dtype):
+    """What an earlier call left in the scratch, a time-out in its status among it, means nothing to the next one."""
+    rng = np.random.default_rng(17)
+    x, gate = make(rng, (sequences, rows), channels, heads, dtype, "f32", True, cuda_device)
+    temp = torch.empty(8 << 20, dtype=torch.uint8, device=cuda_device)
+    want = tb.linear_recurrence(x, gate, log_gate=True)
+    grads = tb.linear_recurrence_backward(gate, want[0], x, log_gate=True)
+    for word in (capi.ERR_WAIT_TIMEOUT, capi.ERR_INVALID_ARGUMENT, -1):
+        for _ in range(3):
+            temp.view(torch.int32).fill_(word)
+            got = tb.linear_recurrence(x, gate, log_gate=True, temp=temp)
+            temp.view(torch.int32).fill_(word)
+            g2 = tb.linear_recurrence_backward(gate, want[0], x, log_gate=True, temp=temp)
+            assert all(torch.equal(a, b) for a, b in zip(got + g2, want + grads))
+
+
 def test_refusals_of_tensors(cuda_device):
     x = torch.zeros(2, 5, 8, device=cuda_device)
     offsets = torch.tensor([0, 5], device=cuda_device)

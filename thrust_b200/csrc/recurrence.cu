@@ -356,13 +356,15 @@ __device__ __forceinline__ void barrier_arrive(int id, int count) {
   asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(count) : "memory");
 }
 
-// Waits for a phase of a barrier; where that takes about a second, or someone else has given up waiting, carries on with
-// the status raised. Other errors in the status do not end a wait: boxes may be on their way.
-__device__ __forceinline__ void mbar_wait(unsigned long long* bar, unsigned parity, int* status) {
+// Waits for a phase of one of the CTA's own barriers; where that takes about a second, carries on with the status raised.
+// Boxes land and warps arrive whatever became of other CTAs, so nothing that the status says ends a wait: boxes may be on
+// their way, and in scratch that no tile waits in the status is whatever was there until block 0, one of its first
+// instructions, sets it. Once a wait of the CTA ran out, its others wait a 64th of that.
+__device__ __forceinline__ void mbar_wait(unsigned long long* bar, unsigned parity, int* status, volatile int* gave_up) {
   for (unsigned spins = 0; !mbar_try_wait(bar, parity); ++spins) {
     if ((spins & 1023u) != 1023u) continue;
-    if (ld_relaxed_s32(status) == (int)TB200_ERR_WAIT_TIMEOUT) return;
-    if (spins >= kSpinLimit) {
+    if (spins >= (*gave_up ? kSpinLimit / 64 : kSpinLimit)) {
+      *gave_up = 1;
       note_timeout(status, kSiteMbarrier, smem_u32(bar), parity);
       return;
     }
@@ -392,6 +394,7 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
   __shared__ float s_heads[SHARED && BACK ? kWarps : 1][SHARED && BACK ? R : 1][kWarp + 1];
   __shared__ unsigned long long s_landed[kStages];  // a stage's boxes
   __shared__ unsigned long long s_ready[2];         // the maps of all warps' stretches, by the parity of the tile
+  __shared__ int s_gave_up;                         // a wait for one of these ran out
   auto* s_word = reinterpret_cast<unsigned(*)[kWarps][WIDTH]>(s_dynamic + kStages * S::kStage);
   auto* s_b = reinterpret_cast<float(*)[kWarps][WIDTH]>(s_dynamic + kStages * S::kStage + 2 * S::kJoin);
 
@@ -496,6 +499,7 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
     for (int k = 0; k < kStages; ++k) mbar_init(&s_landed[k], 1);
     for (int k = 0; k < 2; ++k) mbar_init(&s_ready[k], kWarps);
     mbar_init_fence();
+    s_gave_up = 0;
   }
   if (threadIdx.x == kThreads) describe_tile(chained ? draw(0) : blockIdx.x, 0);
   __syncthreads();
@@ -579,7 +583,7 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
       bool need = false;
       if (some) {
         tile = s_tiles[i & 7].tile;
-        mbar_wait(maps_ready, i >> 1 & 1, &p.hdr->status);
+        mbar_wait(maps_ready, i >> 1 & 1, &p.hdr->status, &s_gave_up);
         // all warps are done with the tile before the parked one: its stage is free
         if (S::BOXES && threadIdx.x == ASKS && s_tiles[(i + 2) & 7].id < total) fetch_boxes(s_tiles[(i + 2) & 7], (i + 2) % kStages);
         const unsigned long long kinds = *reinterpret_cast<const unsigned long long*>(s_kinds[k]);
@@ -683,7 +687,7 @@ recurrence_kernel(const __grid_constant__ RecArgs p, const __grid_constant__ CUt
       }
 
       // ---- first pass: the stretch's A and B ----------------------------------------------------------------
-      if constexpr (S::BOXES) mbar_wait(&s_landed[stage], i / kStages & 1, &p.hdr->status);
+      if constexpr (S::BOXES) mbar_wait(&s_landed[stage], i / kStages & 1, &p.hdr->status, &s_gave_up);
       else asm volatile("cp.async.wait_group 1;" ::: "memory");  // all but the copies of the tile behind
       // all values first: nothing below comes between the loads
       Pack<G, GV> gate[R];
