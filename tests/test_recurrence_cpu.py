@@ -1,6 +1,7 @@
 """Refusals of the recurrence's entry points: nothing here touches a GPU."""
 import ctypes as C
 
+import numpy as np
 import pytest
 import torch
 
@@ -128,3 +129,62 @@ def test_a_call_within_a_call_keeps_its_arrays(monkeypatch, interrupted):
             for got, t in zip(found[0], inputs):
                 assert got == (t.data_ptr(), t.stride(-2), t.stride(0) if t.dim() == 3 else 0), (what, interrupted)
     assert 1 <= len(all_rooms) <= 2  # given back and used again
+
+
+def cells(t):
+    """The bytes of a tensor, one by one."""
+    at = np.array([t.data_ptr()])
+    for s, n in zip(t.stride(), t.shape):
+        at = (at[:, None] + np.arange(n) * s * t.element_size()).reshape(-1)
+    return (at[:, None] + np.arange(t.element_size())).reshape(-1)
+
+
+def test_arrays_that_share_memory_are_found():
+    """Against the sets of bytes: never called apart when they are not, and slices as they are made are called apart."""
+    ops, rng = tb.model_ops, np.random.default_rng(0)
+    buffer = torch.zeros(4000)
+    shared = apart = known = 0
+    for _ in range(4000):
+        a, b = (torch.as_strided(buffer, (int(rng.integers(1, 4)), int(rng.integers(1, 6)), int(rng.integers(1, 7))),
+                                 (int(rng.integers(0, 40)), int(rng.integers(0, 12)), 1), int(rng.integers(0, 60))) for _ in range(2))
+        if rng.random() < 0.4:
+            b = torch.as_strided(buffer, (*a.shape[:2], b.shape[2]), a.stride(), b.storage_offset())
+        if rng.random() < 0.3:
+            b = b.view(torch.float16)
+        ca, cb = cells(a), cells(b)
+        if ops._rows_apart(a):
+            assert len(set(ca)) == len(ca)
+        together = bool(set(ca) & set(cb))
+        shared += together
+        apart += not together
+        if ops._disjoint(a, b):
+            known += 1
+            assert not together, (a.shape, a.stride(), a.storage_offset(), b.shape, b.stride(), b.storage_offset())
+    assert shared > 500 and known > 0.7 * apart
+    wide = torch.zeros(3, 20, 24)
+    for a, b in ((wide[:, :, :8], wide[:, :, 8:16]), (wide[:, :10, :8], wide[:, 10:, :8]), (wide[:, ::2], wide[:, 1::2]),
+                 (wide[0], wide[1]), (wide[:, :, :8].transpose(0, 1), wide[:, :, 16:].transpose(0, 1)), (wide[:, :5], wide[:, 10:15]),
+                 (wide[:, :, :4], wide[:, :, 4:12]), (wide[:2, :, :8], wide[1:, :, 8:16]), (wide[:, :0], wide[:, :0])):
+        assert ops._disjoint(a, b) and ops._disjoint(b, a) and ops._rows_apart(a) and ops._rows_apart(b)
+    for a, b in ((wide[:, :-1], wide[:, 1:]), (wide[..., :8], wide[..., 7:15]), (wide, wide), (wide[:2], wide[1:])):
+        assert not ops._disjoint(a, b) and not ops._disjoint(b, a)
+
+
+def test_outputs_that_race_are_refused():
+    ops = tb.model_ops
+    buffer = torch.zeros(2, 30, 16)
+    x = buffer[:, :20, :8]
+    assert ops._output(x, x, "x") is x and ops._output(None, x, "x").shape == x.shape
+    same = buffer[:, :20, :8]
+    assert ops._output(same, x, "x") is same
+    one = torch.as_strided(x, (1, 20, 8), (7, 16, 1))  # the distance of one sequence means nothing
+    assert ops._output(one, x[:1], "x") is one
+    assert ops._output(buffer[:, 5:25, 8:], x, "x", buffer[:, 6:26, :8], None) is not None
+    square = torch.zeros(3, 3, 4)
+    for out, like, others in ((buffer[:, 1:21, :8], x, ()), (buffer[:, :20, 4:12], x, ()), (square.transpose(0, 1), square, ()),
+                              (torch.as_strided(torch.zeros(400), (2, 20, 8), (200, 7, 1)), x, ()),
+                              (torch.as_strided(torch.zeros(400), (2, 20, 8), (0, 8, 1)), x, ()),
+                              (torch.as_strided(torch.zeros(400), (2, 20, 8), (159, 8, 1)), x, ()),
+                              (buffer[:, :20, 8:], x, (buffer[..., 7:9],)), (buffer[:, :20, 8:], x, (None, buffer[0, 3:5]))):
+        with pytest.raises(ValueError, match="share"):
+            ops._output(out, like, "x", *others)

@@ -8,6 +8,7 @@ here records itself for autograd.
 from __future__ import annotations
 
 import ctypes as C
+import math
 from functools import lru_cache
 from typing import List, Optional, Tuple
 
@@ -126,13 +127,75 @@ def _new(shape, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
     return torch.empty_strided(shape, (1,) if len(shape) == 1 else (shape[1], 1), dtype=dtype, device=device)
 
 
-def _output(out: Optional[torch.Tensor], like: torch.Tensor, name: str) -> torch.Tensor:
+def _lead(t: torch.Tensor) -> List[Tuple[int, int]]:
+    """(bytes apart, how many) of the dimensions that rows of t are counted in, the largest distance first."""
+    size = t.element_size()
+    return sorted(((s * size, n) for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1), reverse=True)
+
+
+def _rows_apart(t: torch.Tensor) -> bool:
+    """Whether no two rows of t share memory: every distance reaches over all that is counted in smaller ones."""
+    if t.is_contiguous():
+        return True
+    width = t.shape[-1] * t.element_size()
+    for apart, n in reversed(_lead(t)):
+        if apart < width:
+            return False
+        width += (n - 1) * apart
+    return True
+
+
+def _reach(t: torch.Tensor) -> int:
+    """Bytes from the first element of t to behind its last one."""
+    return t.nbytes if t.is_contiguous() else (sum(s * (n - 1) for s, n in zip(t.stride(), t.shape)) + 1) * t.element_size()
+
+
+def _disjoint(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two arrays of rows share no memory. False also where they lie in one another's way in an order that does
+    not show it."""
+    at, bt = a.data_ptr(), b.data_ptr()
+    if at + _reach(a) <= bt or bt + _reach(b) <= at or a.numel() == 0 or b.numel() == 0:
+        return True
+    la, lb = _lead(a), _lead(b)
+    wa, wb = a.shape[-1] * a.element_size(), b.shape[-1] * b.element_size()
+    # columns side by side: no two rows meet, whichever they are
+    apart = math.gcd(*(s for s, _ in la + lb))
+    if apart and (bt - at) % apart >= wa and (at - bt) % apart >= wb:
+        return True
+    if la != lb or any(s == 0 for s, _ in la):
+        return False
+
+    # the same distances: rows meet where b lies behind a by some of each distance and less than a row
+    def meet(lead, p) -> bool:
+        if not lead:
+            return -wb < p < wa
+        (s, n), reach = lead[0], sum(d * (m - 1) for d, m in lead[1:])
+        first, last = -((reach + wa - p) // s), (p + reach + wb) // s
+        return any(meet(lead[1:], p - i * s) for i in range(max(first, 1 - n), min(last, n - 1) + 1))
+
+    return not meet(la, bt - at)
+
+
+def _output(out: Optional[torch.Tensor], like: torch.Tensor, name: str, *others: Optional[torch.Tensor]) -> torch.Tensor:
+    """A fresh output, or the caller's: it may be `like` itself, and shares memory with nothing else."""
     if out is None:
         return _empty_like(like)
     if out.shape != like.shape or out.dtype != like.dtype:
         raise ValueError(f"out must have the shape and type of {name}")
-    if any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
+    if not _rows_apart(out):
         raise ValueError("the rows of out share memory")
+    begin = out.data_ptr()
+    end = begin + _reach(out)
+    for t in others if out is like else (like, *others):
+        if t is None:
+            continue
+        at = t.data_ptr()
+        if end <= at or at + _reach(t) <= begin or _disjoint(out, t):
+            continue
+        if t is not like:
+            raise ValueError(f"out must not share memory with other arguments than {name}")
+        if at != begin or any(n > 1 and s != d for n, s, d in zip(out.shape, out.stride(), t.stride())):
+            raise ValueError(f"out must be {name} itself or share no memory with it")
     return out
 
 
@@ -181,8 +244,8 @@ def linear_recurrence(x: torch.Tensor, gate: torch.Tensor, initial: Optional[tor
     x's rows with a gate for each channel, or for each of ``heads`` groups of neighbouring channels; x's type or
     float32. initial: float32 [sequences, channels], y in front of the first row (None: zero). The final states have
     that shape and type; that of an empty sequence is its initial one. States are held in 32 bits, y is rounded once.
-    ``out`` may be x. Packed rows behind the last sequence are left as they were in ``out``, and zero in a fresh y.
-    Results are reproducible from run to run. A value that is not finite makes the rows behind it, in its sequence and
+    ``out`` may be x itself and shares no memory with anything else. Packed rows behind the last sequence are left as
+    they were in ``out``, and zero in a fresh y. Results are reproducible from run to run. A value that is not finite makes the rows behind it, in its sequence and
     channel, not finite."""
     index = _device_of("x", x)
     for name, t in (("gate", gate), ("initial", initial), ("offsets", offsets), ("out", out), ("temp", temp)):
@@ -190,7 +253,7 @@ def linear_recurrence(x: torch.Tensor, gate: torch.Tensor, initial: Optional[tor
     dims, optr = _shape(x, gate, offsets, log_gate, out is None, "x")
     states = (dims[0], dims[2])
     iptr = _states(initial, states, "initial")
-    out = _output(out, x, "x")
+    out = _output(out, x, "x", gate, initial)
     room, arrays = _arrays(_rows(gate, "gate"), _rows(x, "x"), _rows(out, "out"))
     final = _new(states, torch.float32, x.device)
     temp = _scratch(_recurrence_bytes(False, *dims), x, temp)
@@ -239,8 +302,8 @@ def linear_recurrence_step(state: torch.Tensor, x: torch.Tensor, gate: torch.Ten
     state: float32 [slots, channels], a pool of states with adjacent channels. x: [rows, channels], gate: [rows,
     channels or heads], as in ``linear_recurrence``. Row r works on state slots[r] (int32 or int64, at most 65536 of
     them; None: state r). A row whose slot lies outside the pool (a negative one, say, where a batch is padded) gets a
-    zero y and changes nothing; rows that name the same slot are applied in their order. Enqueues one kernel and
-    returns without waiting."""
+    zero y and changes nothing; rows that name the same slot are applied in their order. ``out`` may be x itself and
+    shares no memory with anything else. Enqueues one kernel and returns without waiting."""
     index = _device_of("x", x)
     _same_device(index, "state", state)
     _same_device(index, "gate", gate)
@@ -265,7 +328,7 @@ def linear_recurrence_step(state: torch.Tensor, x: torch.Tensor, gate: torch.Ten
         apart = channels
     elif apart < channels:
         raise ValueError("the states of the pool overlap")
-    out = _output(out, x, "x")
+    out = _output(out, x, "x", gate, state)
     room, arrays = _arrays(_rows(gate, "gate"), _rows(x, "x"), _rows(out, "out"))
     _call(capi.lib.tb200_linear_recurrence_step, "tb200_linear_recurrence_step", index, pool, ss[0], apart, sptr, sbytes,
           *arrays, rows, channels, gs[1], xd, gd, 1 if log_gate else 0, _raw_stream(index))
@@ -381,14 +444,14 @@ def balance_loss_backward(logits: torch.Tensor, weights: torch.Tensor, dloss: to
                           out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Gradient of ``balance_loss`` by the logits, in their type, from its weights and dloss (float32 [sequences], the
     gradient of the losses); mask and offsets as in the forward call. Zero for masked rows and rows of no sequence.
-    ``out`` may be logits. Enqueues one kernel and returns without waiting."""
+    ``out`` may be logits itself and shares no memory with anything else. Enqueues one kernel and returns without waiting."""
     index = _device_of("logits", logits)
     for name, t in (("weights", weights), ("dloss", dloss), ("mask", mask), ("offsets", offsets), ("out", out)):
         _same_device(index, name, t)
     dtype, obytes, optr, sequences, rows, experts = _logits(logits, offsets)
     wptr = _states(weights, (sequences, experts), "weights")
     lptr = _states(dloss, (sequences,), "dloss")
-    out = _output(out, logits, "logits")
+    out = _output(out, logits, "logits", weights)
     mptr, (room, arrays) = _mask(mask, rows), _arrays(_rows(logits, "logits"), _rows(out, "out"))
     _call(capi.lib.tb200_balance_loss_backward, "tb200_balance_loss_backward", index, arrays[0], dtype, wptr, lptr, mptr,
           optr, obytes, sequences, rows, experts, arrays[1], _raw_stream(index))
