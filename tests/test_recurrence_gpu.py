@@ -318,6 +318,26 @@ def test_bad_offsets_are_reported(cuda_device):
             tb.linear_recurrence_backward(x, x, x, offsets=offsets)
 
 
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_bad_offsets_without_rows_or_sequences(cuda_device, dtype):
+    some, none = torch.randn(5, 8, device=cuda_device), torch.zeros(0, 8, device=cuda_device)
+    cases = [(none, [0, 3], True), (none, [0, 0, 1, 0], True), (none, [-1, 0], True), (none, [1], True), (some, [7], True),
+             (some, [-2], True), (some, [3], True), (none, [0, 0, 0], False), (none, [0], False), (some, [0], False),
+             (none, [0] * 700, False), (none, [0] * 600 + [1] + [0] * 99, True)]
+    for x, values, bad in cases:
+        offsets = torch.tensor(values, dtype=dtype, device=cuda_device)
+        ids = torch.zeros(x.shape[0], 2, dtype=torch.int64, device=cuda_device)
+        for call in (lambda: tb.linear_recurrence(x, x, offsets=offsets), lambda: tb.balance_loss(x, ids, offsets=offsets),
+                     lambda: tb.linear_recurrence(x, x, offsets=offsets, out=torch.empty_like(x)),
+                     lambda: tb.linear_recurrence_backward(x, x, x, offsets=offsets)):
+            if bad:
+                with pytest.raises(tb.Tb200Error) as e:
+                    call()
+                assert e.value.code == capi.ERR_INVALID_ARGUMENT
+            else:
+                call()
+
+
 @pytest.mark.parametrize("rows,slots,channels,heads,dtype,gate_dtype,log_gate", [
     (1, 1, 1, 1, "f32", "f32", False), (5, 9, 128, 128, "bf16", "f32", True), (33, 40, 1000, 25, "f16", "f16", False),
     (7, 7, 51, 17, "bf16", "bf16", True), (130, 300, 2048, 8, "bf16", "f32", False)])

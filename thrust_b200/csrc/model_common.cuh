@@ -168,6 +168,26 @@ inline RowsOf rows_of(const tb200_rows* r, bool packed) {
 inline bool rows_on(const RowsOf& r, int elem, int bytes) {
   return (reinterpret_cast<uintptr_t>(r.data) | (r.row * elem) | (r.seq * elem)) % bytes == 0;
 }
+// The status of a call on packed sequences that has no rows or no sequences, and so no kernel that looks at its offsets.
+template <typename O>
+__global__ void __launch_bounds__(256) offsets_kernel(TempHeader* hdr, const O* offsets, uint64_t sequences, uint64_t rows) {
+  bool bad = false;
+  for (uint64_t i = threadIdx.x; i <= sequences; i += 256) {
+    const int64_t v = offsets[i];
+    bad = bad || v < 0 || (uint64_t)v > rows || (i == 0 ? v != 0 : v < (int64_t)offsets[i - 1]);
+  }
+  bad = __syncthreads_or(bad);
+  if (threadIdx.x == 0) hdr->status = bad ? TB200_ERR_INVALID_ARGUMENT : TB200_OK;
+}
+inline int status_without_rows(void* d_temp, const void* offsets, int offset_bytes, uint64_t sequences, uint64_t rows,
+                               cudaStream_t stream) {
+  TempHeader* hdr = static_cast<TempHeader*>(d_temp);
+  if (offset_bytes == 0) return (int)cudaMemsetAsync(hdr, 0, kHeaderBytes, stream);
+  if (offset_bytes == 4) offsets_kernel<<<1, 256, 0, stream>>>(hdr, static_cast<const int32_t*>(offsets), sequences, rows);
+  else offsets_kernel<<<1, 256, 0, stream>>>(hdr, static_cast<const int64_t*>(offsets), sequences, rows);
+  trace_mark(stream);
+  return (int)cudaGetLastError();
+}
 inline int model_bytes(int dtype) { return dtype == TB200_F32 ? 4 : dtype == TB200_F16 || dtype == TB200_BF16 ? 2 : 0; }
 
 }  // namespace tb200

@@ -1163,7 +1163,8 @@ extern "C" int tb200_linear_recurrence(void* d_temp, size_t* temp_bytes, const t
   if (some && !(good_rows(gate, model_bytes(k.shape.gate_dtype)) && good_rows(x, tb) && good_rows(y, tb)))
     return TB200_ERR_INVALID_ARGUMENT;
   if (!some) {
-    TB200_CUDA_TRY(cudaMemsetAsync(d_temp, 0, kHeaderBytes, stream));
+    const int rc = status_without_rows(d_temp, d_offsets, k.shape.offset_bytes, k.shape.sequences, k.rows, stream);
+    if (rc) return rc;
     return hand_through(k, d_initial, d_final, stream);
   }
   RecArgs& p = k.args;
@@ -1192,7 +1193,8 @@ extern "C" int tb200_linear_recurrence_backward(void* d_temp, size_t* temp_bytes
   if (some && !(good_rows(gate, gb) && good_rows(y, tb) && good_rows(dy, tb) && good_rows(dx, tb) && good_rows(dgate, gb)))
     return TB200_ERR_INVALID_ARGUMENT;
   if (!some) {
-    TB200_CUDA_TRY(cudaMemsetAsync(d_temp, 0, kHeaderBytes, stream));
+    const int rc = status_without_rows(d_temp, d_offsets, k.shape.offset_bytes, k.shape.sequences, k.rows, stream);
+    if (rc) return rc;
     return hand_through(k, d_dfinal, d_dinitial, stream);
   }
   RecArgs& p = k.args;

@@ -615,8 +615,8 @@ extern "C" int tb200_balance_loss(void* d_temp, size_t* temp_bytes, const tb200_
   if (reinterpret_cast<uintptr_t>(d_counts) % 8 ||
       (reinterpret_cast<uintptr_t>(d_loss) | reinterpret_cast<uintptr_t>(d_weights)) % 4) return TB200_ERR_INVALID_ARGUMENT;
   if (rows == 0 || sequences == 0) {
-    TB200_CUDA_TRY(cudaMemsetAsync(d_temp, 0, kHeaderBytes, stream));
-    if (sequences == 0) return TB200_OK;
+    rc = status_without_rows(d_temp, d_offsets, offset_bytes, sequences, rows, stream);
+    if (rc || sequences == 0) return rc;
     TB200_CUDA_TRY(cudaMemsetAsync(d_loss, 0, sequences * sizeof(float), stream));
     TB200_CUDA_TRY(cudaMemsetAsync(d_counts, 0, cells * sizeof(uint64_t), stream));
     return (int)cudaMemsetAsync(d_weights, 0, cells * sizeof(float), stream);
