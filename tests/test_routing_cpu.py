@@ -56,3 +56,18 @@ def test_python_front_end_refuses_cpu_tensors():
     for call in (lambda: tb.expert_counts(ids, 8), lambda: tb.balance_loss(z, ids), lambda: tb.balance_loss_backward(z, z, z)):
         with pytest.raises(ValueError, match="CUDA"):
             call()
+
+
+def test_numbers_beyond_32_bits_are_refused():
+    """The library takes experts and ids a row in 32 bits: 2^32 + 8 experts must not be taken for 8."""
+    ops, wide = tb.model_ops, (1 << 32) + 8
+    assert ops._counts_bytes(8) >= 256
+    for experts in (wide, -1, 8 - (1 << 32)):
+        with pytest.raises(ValueError):
+            ops._counts_bytes(experts)
+    assert ops._ids(torch.empty(3, 8, dtype=torch.int32, device="meta")) == (3, 8, 8, 4)
+    assert ops._logits(torch.empty(3, 8, device="meta"), None)[-1] == 8
+    with pytest.raises(ValueError):
+        ops._ids(torch.empty(3, wide, dtype=torch.int32, device="meta"))
+    with pytest.raises(ValueError):
+        ops._logits(torch.empty(3, wide, device="meta"), None)

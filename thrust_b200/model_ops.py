@@ -345,8 +345,8 @@ def _ids(ids: torch.Tensor) -> Tuple[int, int, int, int]:
     if len(shape) == 1:
         return shape[0], 1, stride[0] if shape[0] > 1 else 1, width
     rows, k = shape
-    if k == 0 or (rows and k > 1 and stride[1] != 1) or (rows > 1 and stride[0] < k):
-        raise ValueError("the ids of a row must be adjacent in memory, at least one, and rows must not overlap")
+    if k == 0 or k >> 32 or (rows and k > 1 and stride[1] != 1) or (rows > 1 and stride[0] < k):
+        raise ValueError("the ids of a row must be adjacent in memory, at least one, less than 2^32, and rows must not overlap")
     return rows, k, stride[0] if rows > 1 else k, width
 
 
@@ -360,6 +360,8 @@ def _mask(mask: Optional[torch.Tensor], rows: int) -> Optional[int]:
 
 @lru_cache(maxsize=512)
 def _counts_bytes(experts: int) -> int:
+    if experts >> 32:  # the library would see the lower 32 bits
+        raise ValueError("at most 8192 experts")
     need = C.c_size_t(0)
     capi.check(capi.lib.tb200_expert_counts(None, C.byref(need), None, 0, 1, 1, 8, None, experts, None, None, None),
                "tb200_expert_counts(size)")
@@ -399,7 +401,7 @@ def expert_counts(ids: torch.Tensor, experts: int, mask: Optional[torch.Tensor] 
 
 def _logits(logits: torch.Tensor, offsets: Optional[torch.Tensor]):
     shape = logits.shape
-    if len(shape) != 2 or shape[1] == 0:
+    if len(shape) != 2 or shape[1] == 0 or shape[1] >> 32:
         raise ValueError("logits must be [rows, experts]")
     obytes, optr = _offsets(offsets)
     return _float_code(logits, "logits"), obytes, optr, 1 if offsets is None else offsets.shape[0] - 1, shape[0], shape[1]
