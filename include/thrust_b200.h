@@ -263,6 +263,7 @@ int tb200_histogram_sorted(const void* d_sorted, uint64_t n, int dtype, const vo
  * sequences allowed). Rows behind the last sequence are left as they were, or written as zeros
  * where fill_outside != 0. A tb200_rows names an array by its first element and its strides in
  * elements (row strides up to 2^28); the channels of a row are adjacent; sequence_stride is ignored for packed rows.
+ * Up to 2^24 channels, 2^31 - 1 sequences and 2^40 rows of all sequences.
  * heads gates a row: heads == channels is a gate for each channel, otherwise heads divides
  * channels and channels / heads neighbouring channels share a gate. dtype (x, y and their
  * gradients): F32, F16 or BF16; gate_dtype: dtype or F32. d_initial, d_final and their

@@ -32,6 +32,17 @@ def test_size_queries_answer_without_a_gpu():
     assert capi.lib.tb200_linear_recurrence(None, None, C.byref(shape()), *(None,) * 7) == capi.ERR_INVALID_ARGUMENT
 
 
+def test_rows_of_all_sequences_stay_in_range():
+    """Their number is a product: one that passes 64 bits must not come back as a small scratch."""
+    for back in (False, True):
+        for sequences, rows in (((1 << 31) - 1, 1 << 40), (1 << 30, 1 << 34), (1 << 20, (1 << 20) + 1), (3, 1 << 39)):
+            assert size(shape(sequences=sequences, rows=rows), back)[0] == capi.ERR_UNSUPPORTED
+        for sequences, rows, offsets in ((1 << 20, 1 << 20, 0), (1, 1 << 40, 0), ((1 << 31) - 1, 1 << 40, 8), ((1 << 31) - 1, 0, 0)):
+            rc, need = size(shape(sequences=sequences, rows=rows, offset_bytes=offsets), back)
+            # a tile of 64 rows of 8 channels takes 12 bytes a channel at least
+            assert rc == 0 and need >= (rows if offsets else rows * sequences) // 64 * 8 * 12
+
+
 def test_arguments_are_checked_before_any_device_work():
     s, need = shape(), C.c_size_t(1 << 20)
     fake = 0x7f0000000100  # never dereferenced

@@ -1088,6 +1088,7 @@ int prepare(void* d_temp, size_t* temp_bytes, const tb200_recurrence_shape* shap
   if (s.offset_bytes != 0 && s.offset_bytes != 4 && s.offset_bytes != 8) return TB200_ERR_INVALID_ARGUMENT;
   if (s.channels == 0 || s.heads == 0 || s.channels % s.heads) return TB200_ERR_INVALID_ARGUMENT;
   if (s.channels > (1u << 24) || s.sequences > 0x7fffffffull || s.rows > (1ull << 40)) return TB200_ERR_UNSUPPORTED;
+  if (s.offset_bytes == 0 && s.sequences != 0 && s.rows > (1ull << 40) / s.sequences) return TB200_ERR_UNSUPPORTED;
   k.shape = s;
   k.rows = s.offset_bytes ? s.rows : s.sequences * s.rows;
   RecArgs& p = k.args;
