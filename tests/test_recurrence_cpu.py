@@ -73,6 +73,24 @@ def test_arguments_are_checked_before_any_device_work():
     assert one(state=fake + 2) == capi.ERR_INVALID_ARGUMENT
 
 
+def test_states_off_their_boundary_are_refused():
+    s, need, fake = shape(), C.c_size_t(1 << 20), 0x7f0000000100  # never dereferenced
+    # an array that is refused later on, so that nothing reaches a device whichever check comes first
+    good, none = C.byref(capi.Rows(fake, 8, 80)), C.byref(capi.Rows(None, 8, 80))
+    for rows in (10, 0):
+        s = shape(rows=rows)
+        for which in range(2):
+            states = [None, None]
+            states[which] = fake + 2
+            assert capi.lib.tb200_linear_recurrence(fake, C.byref(need), C.byref(s), None, good, good, none, *states,
+                                                    None) == capi.ERR_INVALID_ARGUMENT
+        for which in range(3):
+            states = [None] * 3
+            states[which] = fake + 1
+            assert capi.lib.tb200_linear_recurrence_backward(fake, C.byref(need), C.byref(s), None, good, good, good, good, none,
+                                                             *states, None) == capi.ERR_INVALID_ARGUMENT
+
+
 def test_python_front_end_refuses_cpu_tensors():
     z = torch.zeros(2, 3, 4)
     with pytest.raises(ValueError, match="CUDA"):

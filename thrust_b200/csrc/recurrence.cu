@@ -1138,6 +1138,12 @@ int prepare(void* d_temp, size_t* temp_bytes, const tb200_recurrence_shape* shap
   return TB200_OK;
 }
 
+bool good_states(std::initializer_list<const float*> states) {  // each may be absent
+  uintptr_t all = 0;
+  for (const float* s : states) all |= reinterpret_cast<uintptr_t>(s);
+  return all % sizeof(float) == 0;
+}
+
 // States of sequences that have no rows at all.
 int hand_through(const Call& k, const float* from, float* to, cudaStream_t stream) {
   const size_t bytes = k.shape.sequences * k.shape.channels * sizeof(float);
@@ -1157,6 +1163,7 @@ extern "C" int tb200_linear_recurrence(void* d_temp, size_t* temp_bytes, const t
   Call k{};
   const int rc = prepare(d_temp, temp_bytes, shape, false, dense(shape, {gate, x, y}), k);
   if (rc || d_temp == nullptr) return rc;
+  if (!good_states({d_initial, d_final})) return TB200_ERR_INVALID_ARGUMENT;
   const bool packed = k.shape.offset_bytes != 0;
   if (packed && (!d_offsets || reinterpret_cast<uintptr_t>(d_offsets) % k.shape.offset_bytes)) return TB200_ERR_INVALID_ARGUMENT;
   const bool some = k.rows != 0 && k.shape.sequences + (packed && k.shape.fill_outside) != 0;
@@ -1187,6 +1194,7 @@ extern "C" int tb200_linear_recurrence_backward(void* d_temp, size_t* temp_bytes
   Call k{};
   const int rc = prepare(d_temp, temp_bytes, shape, true, dense(shape, {gate, y, dy, dx, dgate}), k);
   if (rc || d_temp == nullptr) return rc;
+  if (!good_states({d_initial, d_dfinal, d_dinitial})) return TB200_ERR_INVALID_ARGUMENT;
   const bool packed = k.shape.offset_bytes != 0;
   if (packed && (!d_offsets || reinterpret_cast<uintptr_t>(d_offsets) % k.shape.offset_bytes)) return TB200_ERR_INVALID_ARGUMENT;
   const bool some = k.rows != 0 && k.shape.sequences + (packed && k.shape.fill_outside) != 0;
