@@ -217,3 +217,14 @@ def test_outputs_that_race_are_refused():
                               (buffer[:, :20, 8:], x, (buffer[..., 7:9],)), (buffer[:, :20, 8:], x, (None, buffer[0, 3:5]))):
         with pytest.raises(ValueError, match="share"):
             ops._output(out, like, "x", *others)
+
+
+def test_scratch_with_gaps_is_refused():
+    """The library writes to all bytes from the first one on: an expanded tensor has one of them."""
+    ops, like = tb.model_ops, torch.zeros(1)
+    whole = torch.zeros(4096, dtype=torch.uint8)
+    assert ops._scratch(4096, like, whole) is whole
+    assert ops._scratch(5000, like, whole).numel() == 5000 and ops._scratch(300, like, None).numel() == 300
+    for temp in (whole[:1].expand(4096), whole[::2], whole.view(64, 64).T):
+        with pytest.raises(ValueError, match="contiguous"):
+            ops._scratch(1000, like, temp)

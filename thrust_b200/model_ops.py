@@ -201,6 +201,8 @@ def _output(out: Optional[torch.Tensor], like: torch.Tensor, name: str, *others:
 
 def _scratch(need: int, like: torch.Tensor, temp: Optional[torch.Tensor]) -> torch.Tensor:
     if temp is not None and temp.numel() >= need:
+        if not temp.is_contiguous():
+            raise ValueError("temp must be contiguous")
         return temp
     return _new((need,), torch.uint8, like.device)
 
