@@ -139,6 +139,22 @@ def test_loss_and_gradient(cuda_device, case, masked):
     assert ((got - want).abs() <= 2 * REL * size + half * want.abs() * (1 + 1e-5) + tiny)[inside].all()
 
 
+@pytest.mark.parametrize("lengths,experts,k", [
+    ([16] * 256, 8, 8), ([1, 0, 2] * 150, 64, 6), ([2000, 2096], 8, 2), ([4096], 8, 2), ([1024], 8, 8), ([1025], 8, 8), ([31] * 33, 32, 1)])
+def test_small_calls_on_one_cta_and_on_many(cuda_device, lengths, experts, k):
+    """Either side of what one CTA takes alone, as one sequence and as many: the same counts, losses within the bound."""
+    z, ids, mask, offsets, _ = build((lengths, experts, k, "bf16"), cuda_device, True)
+    loss, counts, weights = tb.balance_loss(z, ids, mask=mask, offsets=offsets)
+    wl, wc, ww = plain_loss(z, ids, mask, offsets)
+    assert torch.equal(counts.cpu(), wc)
+    assert ((weights.cpu().double() - ww).abs() <= 2 ** -23 * ww).all()
+    bound = REL + (64 + z.shape[0] / 100) * 2 ** -24
+    assert ((loss.cpu().double() - wl).abs() <= bound * wl).all()
+    whole, per_expert, _ = tb.balance_loss(z, ids, mask=mask)
+    assert torch.equal(per_expert[0], counts.sum(0))
+    assert abs(float(whole) - float(plain_loss(z, ids, mask, None)[0])) <= bound * float(whole)
+
+
 def test_gradient_agrees_with_differences(cuda_device):
     z, ids, mask, offsets, rng = build(([5, 0, 8], 6, 2, "f32"), cuda_device, True)
     z = torch.where(torch.isinf(z), torch.zeros_like(z), z)

@@ -652,9 +652,13 @@ extern "C" int tb200_balance_loss(void* d_temp, size_t* temp_bytes, const tb200_
     const uint64_t slots = (uint64_t)per_sm * sms, least = (uint64_t)kRouteWarps * (kWarp / decltype(l)::value);
     a.rows_of_cta = (rows + slots - 1) / slots;
     if (a.rows_of_cta < least) a.rows_of_cta = least;
-    // Up to 2^15 probabilities one CTA does it all: no clear of the scratch in front, nothing to join behind. 1024 rows
-    // of 8 experts: kernel 9.4 us instead of 8.4 us on four CTAs, the call 17.7 us instead of 20.3 us.
-    if (rows * experts <= 32768) a.rows_of_cta = rows;
+    // One CTA does all of one sequence with up to 2^15 probabilities and 2^13 ids: no clear of the scratch in front. That
+    // saves a call 2 to 3 us, and costs up to 3 us where the GPU has work queued or replays a graph. Measured, one CTA
+    // against many, a call / in a graph: 1024 x 8 with 2 ids a row 17.5 against 19.5 / 7.4 against 10.0 us, 4096 x 8 with 2
+    // ids 17.7 against 19.5 / 12.0 against 10.2, 128 x 256 with 8 ids 17.6 against 21.1 / 10.8 against 7.6. Not more ids
+    // (4096 x 8 with 8: 22.7 against 19.4 / 21.8 against 10.4) nor more sequences, which a CTA takes one after the
+    // other (4096 x 8 with 2 ids in 16 sequences: 92 against 20 / 90 against 11).
+    if (sequences == 1 && rows * experts <= 32768 && rows * k <= 8192) a.rows_of_cta = rows;
     const unsigned grid = (unsigned)((rows + a.rows_of_cta - 1) / a.rows_of_cta);
     if (grid > 1) TB200_CUDA_TRY(cudaMemsetAsync(d_temp, 0, need, stream));
     kernel<<<grid, kRouteThreads, 0, stream>>>(a);
