@@ -155,6 +155,21 @@ def test_small_calls_on_one_cta_and_on_many(cuda_device, lengths, experts, k):
     assert abs(float(whole) - float(plain_loss(z, ids, mask, None)[0])) <= bound * float(whole)
 
 
+@pytest.mark.parametrize("lengths,experts", [
+    ([0] * 700 + [50] + [0] * 300, 64), ([0, 0, 9000, 0] * 3 + [0] * 70, 160), ([0] * 33, 8), ([0] * 31 + [1], 1000), ([3] * 40 + [0] * 4000, 24)])
+def test_outputs_of_empty_sequences(cuda_device, lengths, experts):
+    """Many of them, in front, between and behind, over one CTA and over many: zeros, in outputs that held something else."""
+    z, ids, mask, offsets, _ = build((lengths, experts, 2, "bf16"), cuda_device, False)
+    for _ in range(2):  # what these blocks held is what the next outputs begin with
+        full = [torch.full((len(lengths), experts), 7, dtype=t, device=cuda_device) for t in (torch.int64, torch.float32)]
+        del full
+        loss, counts, weights = tb.balance_loss(z, ids, offsets=offsets)
+    wl, wc, ww = plain_loss(z, ids, None, offsets)
+    assert torch.equal(counts.cpu(), wc)
+    assert ((weights.cpu().double() - ww).abs() <= 2 ** -23 * ww).all()
+    assert ((loss.cpu().double() - wl).abs() <= (REL + (64 + z.shape[0] / 100) * 2 ** -24) * wl).all()
+
+
 def test_gradient_agrees_with_differences(cuda_device):
     z, ids, mask, offsets, rng = build(([5, 0, 8], 6, 2, "f32"), cuda_device, True)
     z = torch.where(torch.isinf(z), torch.zeros_like(z), z)

@@ -275,6 +275,33 @@ struct BalanceArgs {
   unsigned* poison;            // [sequences] a probability was NaN
 };
 
+// Outputs of empty sequences, which belong to no CTA's rows, and the report of bad offsets: a warp for 32 sequences.
+__device__ __noinline__ void empty_sequences(Spans spans, uint32_t experts, float* loss, uint64_t* counts, float* weights,
+                                             int* status) {
+  const unsigned lane = lane_id();
+  bool bad = blockIdx.x == 0 && threadIdx.x == 0 &&
+             raw_offset(spans, spans.sequences) != (int64_t)begin_of(spans, spans.sequences);
+  for (uint64_t base = (blockIdx.x * (uint64_t)kRouteWarps + threadIdx.x / kWarp) * kWarp; base < spans.sequences;
+       base += (uint64_t)gridDim.x * kRouteThreads) {
+    const uint64_t s = base + lane;
+    bool empty = false;
+    if (s < spans.sequences) {
+      const uint64_t b = begin_of(spans, s), e = begin_of(spans, s + 1);
+      bad = bad || raw_offset(spans, s) != (int64_t)b || (s == 0 && b != 0) || e < b;
+      empty = e <= b;
+      if (empty) loss[s] = 0.0f;
+    }
+    for (unsigned left = __ballot_sync(0xffffffffu, empty); left != 0; left &= left - 1) {
+      const uint64_t row = (base + __ffs(left) - 1) * experts;
+      for (uint32_t i = lane; i < experts; i += kWarp) {
+        counts[row + i] = 0;
+        weights[row + i] = 0.0f;
+      }
+    }
+  }
+  if (bad) atomicExch(status, (int)TB200_ERR_INVALID_ARGUMENT);
+}
+
 template <typename T, int J, int L, bool VEC>
 __global__ void __launch_bounds__(kRouteThreads, J == 1 ? 3 : 1) balance_kernel(BalanceArgs a) {
   __shared__ unsigned s_count[kMaxBalanceExperts];
@@ -295,20 +322,8 @@ __global__ void __launch_bounds__(kRouteThreads, J == 1 ? 3 : 1) balance_kernel(
     __threadfence();
     __syncthreads();
   }
-  if (blockIdx.x == 0 && a.spans.bytes) {  // empty sequences belong to no CTA's rows; bad offsets are reported
-    bool bad = threadIdx.x == 0 && raw_offset(a.spans, a.spans.sequences) != (int64_t)begin_of(a.spans, a.spans.sequences);
-    for (uint64_t s = threadIdx.x; s < a.spans.sequences; s += kRouteThreads) {
-      const uint64_t b = begin_of(a.spans, s), e = begin_of(a.spans, s + 1);
-      bad = bad || raw_offset(a.spans, s) != (int64_t)b || (s == 0 && b != 0) || e < b;
-      if (e > b) continue;
-      for (uint32_t i = 0; i < a.experts; ++i) {
-        a.counts[s * a.experts + i] = 0;
-        a.weights[s * a.experts + i] = 0.0f;
-      }
-      a.loss[s] = 0.0f;
-    }
-    if (bad) atomicExch(&a.hdr->status, (int)TB200_ERR_INVALID_ARGUMENT);
-  }
+  if (a.spans.bytes && blockIdx.x * (uint64_t)kRouteThreads < a.spans.sequences)
+    empty_sequences(a.spans, a.experts, a.loss, a.counts, a.weights, &a.hdr->status);
   if (r0 >= r1) return;
 
   for (uint64_t s = sequence_of(a.spans, r0); s < a.spans.sequences; ++s) {
