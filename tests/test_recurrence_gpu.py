@@ -7,6 +7,8 @@ one) or of 1 - a (near one), and the products over stretches by a rounding a row
 8 * 2^-24 * min(m, rows) * max|state|, to which an output of fewer bits adds half a step of its own. Gradients of gates
 are products of two such values, summed over the channels that share a gate.
 """
+from concurrent.futures import ThreadPoolExecutor
+
 import numpy as np
 import pytest
 import torch
@@ -438,6 +440,85 @@ def test_short_sequences_that_lie_apart(cuda_device):
         for g in (ga, gb):
             close(g[0], wx, x.dtype, rows, what="dx")
             close(g[1], wg, gate.dtype, rows, float(wx.abs().max() * a[0].float().abs().max().cpu()) + float(size.max()), "dgate")
+
+
+@pytest.mark.parametrize("case", [
+    (400, 40, 520, 520, "bf16", "bf16", True),         # tiles that wait for none: each is a whole sequence
+    (400, 40, 523, 523, "bf16", "f32", False),         # the same with one channel a lane
+    (300, 33, 640, 20, "f16", "f32", True),            # heads of 32
+    (300, 31, 1001, 1001, "f32", "f32", True),         # short ones behind one another, a chain of hundreds of tiles
+    (1, 20011, 301, 301, "bf16", "bf16", False),       # one channel a lane in long chains: values through registers
+    (1, 20011, 299, 299, "f32", "f32", True),          # and by asynchronous copies
+    (2, 9001, 350, 10, "f16", "f16", True),            # heads of 35, over two blocks of channels each
+    (1, 15013, 306, 102, "bf16", "f32", False),        # heads of 3
+    (1, 15013, 640, 16, "f32", "f32", True),           # heads of 40 in boxes
+    ([3000, 0, 1, 64, 4001, 0, 7, 6000, 31], None, 333, 333, "bf16", "f32", True),
+    ([1000] * 16 + [0] * 40 + [3] * 50, None, 520, 520, "f32", "f32", False),
+], ids=lambda c: "-".join(map(str, c)).replace(" ", "")[:60])
+def test_many_tiles_for_each_cta(cuda_device, case):
+    """Nine tiles and more for every one of 148 CTAs, so that all rings of the pipeline wrap: against 64 bits, and the same to
+    the bit every time."""
+    x, gate, initial, offsets, rng = build(case, cuda_device, 21)
+    log_gate, per = case[6], case[2] // case[3]
+    y, final = tb.linear_recurrence(x, gate, initial=initial, offsets=offsets, log_gate=log_gate)
+    wy, wf = reference(x, gate, initial, offsets, log_gate)
+    m = memory_of(gate, log_gate, x.shape[-2])
+    scale = max(float(wy.abs().max()), float(wf.abs().max()))
+    close(y, wy, x.dtype, m, scale, "y")
+    close(final, wf, torch.float32, m, scale, "final")
+    dy = torch.from_numpy(rng.standard_normal(tuple(x.shape))).to(cuda_device, x.dtype)
+    dfinal = torch.from_numpy(rng.standard_normal(tuple(final.shape)).astype(np.float32)).to(cuda_device)
+    args = dict(initial=initial, dfinal=dfinal, offsets=offsets, log_gate=log_gate)
+    got = tb.linear_recurrence_backward(gate, y, dy, **args)
+    wx, wg, wi, size = reference_backward(gate, y, dy, initial, dfinal, offsets, log_gate)
+    back = max(float(wx.abs().max()), float(wi.abs().max()))
+    close(got[0], wx, dy.dtype, m, back, "dx")
+    close(got[1], wg, gate.dtype, m, back * max(float(y.abs().max()), float(initial.abs().max())) * per + float(size.max()), "dgate")
+    close(got[2], wi, torch.float32, m, back, "dinitial")
+    for _ in range(3):
+        again = tb.linear_recurrence(x, gate, initial=initial, offsets=offsets, log_gate=log_gate)
+        assert torch.equal(again[0], y) and torch.equal(again[1], final)
+        assert all(torch.equal(a, b) for a, b in zip(got, tb.linear_recurrence_backward(gate, y, dy, **args)))
+
+
+def test_calls_from_several_threads(cuda_device):
+    """Four threads with a stream each, all operators of a layer over arrays of different strides: nobody's arguments or
+    results are another one's."""
+    def layer(i):
+        rng = np.random.default_rng(i)
+        channels, experts = 64 + 8 * i, 8 + i
+        wide = torch.from_numpy(rng.standard_normal((200 + 30 * i, channels + 8 * i))).to(cuda_device, torch.float32)
+        x, gate = wide[:, :channels], -wide[:, :channels].abs() - 0.01
+        offsets = torch.tensor([0, 50 + i, 190 + i], dtype=torch.int32, device=cuda_device)
+        ids = torch.from_numpy(rng.integers(0, experts, size=(x.shape[0], 2))).to(cuda_device)
+        dloss = torch.ones(2, device=cuda_device)
+        pool = torch.zeros(4 + i, channels, device=cuda_device)
+
+        def run():
+            pool.zero_()
+            y, final = tb.linear_recurrence(x, gate, offsets=offsets, log_gate=True)
+            grads = tb.linear_recurrence_backward(gate, y, x, offsets=offsets, log_gate=True)
+            z = y[:, :experts]
+            loss, counts, weights = tb.balance_loss(z, ids, offsets=offsets)
+            dz = tb.balance_loss_backward(z, weights, dloss, offsets=offsets)
+            step = tb.linear_recurrence_step(pool, x[:3], gate[:3], log_gate=True)
+            return [y, final, *grads, loss, counts, weights, dz, step, pool.clone(), *tb.expert_counts(ids, experts)]
+        return run
+
+    layers = [layer(i) for i in range(4)]
+    want = [run() for run in layers]
+    torch.cuda.synchronize()
+
+    def work(i):
+        with torch.cuda.device(cuda_device), torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(30):
+                for a, b in zip(layers[i](), want[i]):
+                    if not torch.equal(a, b):
+                        return f"thread {i}"
+        return None
+
+    with ThreadPoolExecutor(4) as pool:
+        assert list(pool.map(work, range(4))) == [None] * 4
 
 
 @pytest.mark.parametrize("heads", [96, 3])

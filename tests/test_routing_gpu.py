@@ -315,6 +315,27 @@ def test_captured_and_replayed(cuda_device):
         assert torch.equal(got[1][0], got[3])
 
 
+def test_two_streams_at_once(cuda_device):
+    """The same calls under way on two streams: scratch and outputs of their own."""
+    z, ids, mask, offsets, _ = build(([4000, 0, 9000, 70, 2000], 160, 6, "bf16"), cuda_device, True)
+    dloss = torch.full((5,), 1000.0, device=cuda_device)
+
+    def step():
+        loss, counts, weights = tb.balance_loss(z, ids, mask=mask, offsets=offsets, sync=False)
+        return (loss, counts, weights, *tb.expert_counts(ids, 160, mask=mask, sync=False),
+                tb.balance_loss_backward(z, weights, dloss, mask=mask, offsets=offsets))
+
+    want = step()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for s in streams * 10:
+        with torch.cuda.stream(s):
+            got.append(step())
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
+
+
 def test_layer_of_recurrence_and_routing(cuda_device):
     """A training step of one layer on packed sequences: recurrence, router, dispatch order, balance loss, and back."""
     rng = np.random.default_rng(8)
