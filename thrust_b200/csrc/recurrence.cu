@@ -25,8 +25,11 @@
 //
 // Measured (one B200, 6.56 TB/s copy): forward 65536 x 2048 bf16 with 32-bit log gates 281 us, 3.8 TB/s, with one
 // sequence only 9 tiles of each block of channels are in work at once and 14 % of the looks wait for the tile in
-// front; backward of 8 x 4096 x 2048 bf16 141 us, 4.8 TB/s, bound by latency in the compute warps (12 warps an SM, issue
-// slots a third busy). Tried and slower: rows parked in registers (spills; 707 us), one tile a CTA (452 us), 16-byte
+// front (float32 521 us, 3.1 TB/s); backward of 8 x 4096 x 2048 bf16 141 us, 4.8 TB/s, bound by latency in the compute warps
+// (12 warps an SM, issue slots 37 % busy). 4 x 4096 x 2048 forward and backward: bf16 70 and 82 us (floors 31 and 51), float32
+// 126 and 151 us (61 and 102). Rows that are not on 16 bytes take one channel a lane, a quarter of the bytes for the same
+// latency: 4 x 4096 x 2047 bf16 212 and 691 us (its values go through registers, which the backward pass spills: 460 to 472
+// bytes stored a thread), float32 230 and 234 us. Tried and slower: rows parked in registers (spills; 707 us), one tile a CTA (452 us), 16-byte
 // cp.async for the rows (373 us: the copies' issue took as long as a pass), 16 tiles looked at every time (327 us), sums
 // over a head by shuffles (the compiler's form of them in this loop takes 300 cycles each).
 #include <cuda.h>

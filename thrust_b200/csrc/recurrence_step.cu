@@ -3,9 +3,11 @@
 // Bound by HBM where there are many rows (a state is read and written in 32 bits, which no order of work avoids) and by
 // the launch where there are few. Threads take four channels of one row; a CTA works on one row, so that rows which
 // name the same state are put in order by a CTA alone: the CTA of the first of them applies them all. Looking through the
-// slots of all rows costs a CTA two loads a thread for 512 rows. Measured: one row of 2048 channels 3.6 us, 512 rows of
-// 4096 channels 8.4 us (3.0 TB/s of 25 MB; half of that time is a kernel's own latency). A single step uses the exact
-// forms of a gate near one, since every step rounds the gate anew.
+// slots of all rows costs a CTA two loads a thread for 512 rows, and grows with their square: 4096 rows of 4096 channels
+// 80 us (39 without slots), 16384 x 2048 463 us (75), 65536 x 2048 6.9 ms (0.28). Measured: one row of 2048 channels 3.6 us,
+// 512 rows of 4096 channels 8.4 us (3.0 TB/s of 25 MB; half of that time is a kernel's own latency). A single step uses the
+// series of a gate near one, since every step rounds the gate anew; a log gate g below -0.3 takes the fast exponential, off
+// by 2 + 1.2 |g| units of 2^-23 of the gate, which a state with such gates has forgotten after four steps.
 #include <cuda_runtime.h>
 
 #include <cstdint>
