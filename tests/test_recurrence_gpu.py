@@ -481,6 +481,42 @@ def test_many_tiles_for_each_cta(cuda_device, case):
         assert all(torch.equal(a, b) for a, b in zip(got, tb.linear_recurrence_backward(gate, y, dy, **args)))
 
 
+def test_arrays_of_more_than_32_bits(cuda_device):
+    """More than 2^32 elements an array: the last rows are those of a run over the last rows alone, since decays of at most
+    exp(-0.02) leave nothing of what lies 6000 rows back. Both runs are within the bound of an exact one, and round once."""
+    channels, far, near = 2048, (1 << 32) // 2048 + 5000, 6000
+    block = torch.randn(1, 4099, channels, device=cuda_device).bfloat16()
+    rate = torch.empty(1, 4099, channels, device=cuda_device).uniform_(0.02, 1.0)
+
+    def many(rows):
+        return rows.repeat(1, -(-far // rows.shape[1]), 1)[:, :far].contiguous()
+
+    x, gate = many(block), many(torch.exp(-rate).clamp(max=0.98).bfloat16())
+    y, final = tb.linear_recurrence(x, gate)
+    ly, lf = tb.linear_recurrence(x[:, -2 * near:], gate[:, -2 * near:])
+
+    def agree(a, b, scale):
+        bound = 2 * (8 * EPS * 60 * scale + torch.finfo(a.dtype).eps / 2 * (1 + 1e-6) * b.float().abs())
+        return bool(((a.float() - b.float()).abs() <= bound).all())
+
+    top = float(ly.abs().max())
+    assert agree(y[:, -near:], ly[:, -near:], top) and agree(final, lf, top)
+    dx, dgate, dinitial = tb.linear_recurrence_backward(gate, y, x)
+    lx, lg, _ = tb.linear_recurrence_backward(gate[:, -2 * near:], y[:, -2 * near:], x[:, -2 * near:])
+    assert agree(dx[:, -near:], lx[:, -near:], float(lx.abs().max()))
+    assert agree(dgate[:, -near:], lg[:, -near:], float(lx.abs().max()) * top)
+    fx, fg, fi = tb.linear_recurrence_backward(gate[:, :2 * near], y[:, :2 * near], x[:, :2 * near])
+    assert agree(dx[:, :near], fx[:, :near], float(fx.abs().max())) and agree(dinitial, fi, float(fx.abs().max()))
+    assert agree(dgate[:, :near], fg[:, :near], float(fx.abs().max()) * top)
+    del x, gate, y, dx, dgate
+    pool = torch.zeros((1 << 32) // channels + 3, channels, device=cuda_device)  # and a pool of such states
+    pool[-2:] = 1.0
+    slots = torch.tensor([pool.shape[0] - 1, 0, pool.shape[0] - 2, 1], device=cuda_device)
+    step = torch.arange(4.0, device=cuda_device)[:, None].expand(4, channels).contiguous()
+    out = tb.linear_recurrence_step(pool, step, torch.full_like(step, 0.5), slots=slots)
+    assert torch.equal(out[:, 0], torch.tensor([0.5, 1.0, 2.5, 3.0], device=cuda_device)) and torch.equal(pool[slots], out)
+
+
 def test_calls_from_several_threads(cuda_device):
     """Four threads with a stream each, all operators of a layer over arrays of different strides: nobody's arguments or
     results are another one's."""

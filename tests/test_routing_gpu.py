@@ -315,6 +315,23 @@ def test_captured_and_replayed(cuda_device):
         assert torch.equal(got[1][0], got[3])
 
 
+def test_logits_of_more_than_32_bits(cuda_device):
+    """More than 2^32 logits, the same 4096 rows over and over: their loss and counts, and the gradient of the last rows."""
+    times, experts = (1 << 32) // (4096 * 256) + 3, 256
+    z, ids, _, _, _ = build((4096, experts, 2, "bf16"), cuda_device, False)
+    wl, wc, _ = plain_loss(z, ids, None, None)
+    many, all_ids = z.repeat(times, 1), ids.to(torch.int32).repeat(times, 1)
+    loss, counts, weights = tb.balance_loss(many, all_ids)
+    assert torch.equal(counts.cpu(), wc * times)
+    assert torch.equal(tb.expert_counts(all_ids, experts)[0].cpu(), wc[0] * times)
+    # a lane adds a row in eight of a CTA's, of at least 132 SMs with a CTA each, in 32 bits
+    assert abs(float(loss) - float(wl[0])) <= (REL + many.shape[0] / 132 / 8 * 2 ** -24) * float(wl[0])
+    dloss = torch.full((1,), float(many.shape[0]), device=cuda_device)
+    grad = tb.balance_loss_backward(many, weights, dloss)
+    want = tb.balance_loss_backward(z, weights, dloss)
+    assert want.any() and torch.equal(grad[-4096:], want) and torch.equal(grad[:4096], want)
+
+
 def test_two_streams_at_once(cuda_device):
     """The same calls under way on two streams: scratch and outputs of their own."""
     z, ids, mask, offsets, _ = build(([4000, 0, 9000, 70, 2000], 160, 6, "bf16"), cuda_device, True)

@@ -361,8 +361,8 @@ __device__ __forceinline__ void barrier_arrive(int id, int count) {
 
 // Waits for a phase of one of the CTA's own barriers; where that takes about a second, carries on with the status raised.
 // Boxes land and warps arrive whatever became of other CTAs, so nothing that the status says ends a wait: boxes may be on
-// their way, and in scratch that no tile waits in the status is whatever was there until block 0, one of its first
-// instructions, sets it. Once a wait of the CTA ran out, its others wait a 64th of that.
+// their way, and in scratch that no tile waits in the status is whatever was there until block 0 sets it, among its first
+// instructions and so long before a wait can run out. Once a wait of the CTA ran out, its others wait a 64th of that.
 __device__ __forceinline__ void mbar_wait(unsigned long long* bar, unsigned parity, int* status, volatile int* gave_up) {
   for (unsigned spins = 0; !mbar_try_wait(bar, parity); ++spins) {
     if ((spins & 1023u) != 1023u) continue;
